@@ -41,9 +41,9 @@ def listed():
         # the 8B benchmark's training step (6 x 4096 tokens), way up
         {"name": "train-24576x4096x14336", "op": "train", "m": 24576,
          "k": 4096, "n": "14336", "dtype": "bf16"},
-        # q, k and v of the 1B model from one packed input, 4096 tokens
-        {"name": "train-4096x2048x2048+512+512", "op": "train", "m": 4096,
-         "k": 2048, "n": "2048+512+512", "dtype": "bf16"},
+        # gate and up of the 1B model from one packed input, 4096 tokens
+        {"name": "train-4096x2048x8192+8192", "op": "train", "m": 4096,
+         "k": 2048, "n": "8192+8192", "dtype": "bf16"},
         # nothing a multiple of a tile: a ragged batch, odd widths
         {"name": "train-1001x1111x777", "op": "train", "m": 1001, "k": 1111,
          "n": "777", "dtype": "bf16"},
