@@ -8,6 +8,7 @@ scaled_dot_product_attention, which on ROCm dispatches to the fused
 otherwise.  The 288 GB HBM3E per GPU fits the full 8B model + Adam states
 without sharding, so plain DP is the natural parallelism.
 """
+import functools
 import math
 from dataclasses import dataclass
 
@@ -15,6 +16,12 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from maggy_amd.ops.block8 import (
+    Linear8Group,
+    MaggyFeedForward8,
+    MaggyRMSNorm8,
+    groups8,
+)
 from maggy_amd.ops.fused_rms import (  # noqa: F401
     MaggyRMSNorm,
     rope_bthd,
@@ -34,6 +41,9 @@ class LlamaConfig:
     max_seq_len: int = 8192
     rope_theta: float = 500000.0
     norm_eps: float = 1e-5
+    # the layers' projections, feed-forwards and norms on the 8-bit block
+    # operators (ops/block8.py); embeddings, attention and lm_head stay
+    eight_bit: bool = False
 
     @staticmethod
     def llama3_8b():
@@ -126,14 +136,25 @@ class Attention(nn.Module):
         self.wk = MaggyLinear(cfg.dim, cfg.n_kv_heads * self.head_dim)
         self.wv = MaggyLinear(cfg.dim, cfg.n_kv_heads * self.head_dim)
         self.wo = MaggyLinear(cfg.n_heads * self.head_dim, cfg.dim)
+        self.qkv8 = self.out8 = None
+        if cfg.eight_bit:
+            self.qkv8 = Linear8Group(self.wq, self.wk, self.wv)
+            self.out8 = Linear8Group(self.wo)
+
+    def _project_out(self, x):
+        return self.wo(x) if self.out8 is None else self.out8(x)
 
     def forward(self, x, cos, sin, cache=None, pos=0):
         B, T, _ = x.shape
         # RoPE applies on the [B, T, H, D] layout BEFORE the head
         # transpose (one fused bf16 pass, ops/fused_rms.py::rope_bthd)
-        q = self.wq(x).view(B, T, self.n_heads, self.head_dim)
-        k = self.wk(x).view(B, T, self.n_kv_heads, self.head_dim)
-        v = self.wv(x).view(B, T, self.n_kv_heads, self.head_dim).transpose(1, 2)
+        if self.qkv8 is None:
+            q, k, v = self.wq(x), self.wk(x), self.wv(x)
+        else:
+            q, k, v = self.qkv8(x)
+        q = q.view(B, T, self.n_heads, self.head_dim)
+        k = k.view(B, T, self.n_kv_heads, self.head_dim)
+        v = v.view(B, T, self.n_kv_heads, self.head_dim).transpose(1, 2)
         q = rope_bthd(q, cos, sin, pos).transpose(1, 2)
         k = rope_bthd(k, cos, sin, pos).transpose(1, 2)
         if cache is not None:
@@ -164,7 +185,7 @@ class Attention(nn.Module):
         causal = T > 1
         out = _sdpa(q, k, v, causal, self.n_kv_heads != self.n_heads)
         out = out.transpose(1, 2).reshape(B, T, -1)
-        return self.wo(out)
+        return self._project_out(out)
 
     def _masked_decode_step(self, B, q, k, v, cache):
         """Capture-safe single-token attention: in-place index_copy of
@@ -185,7 +206,7 @@ class Attention(nn.Module):
         probs = scores.float().softmax(-1).to(q.dtype)
         outh = torch.einsum("bkrs,bksd->bkrd", probs, vbuf)
         out = outh.reshape(B, 1, self.n_heads * self.head_dim)
-        return self.wo(out)
+        return self._project_out(out)
 
 
 class FeedForward(MaggyFeedForward):
@@ -199,15 +220,35 @@ class FeedForward(MaggyFeedForward):
 class Block(nn.Module):
     def __init__(self, cfg):
         super().__init__()
-        self.attn_norm = RMSNorm(cfg.dim, cfg.norm_eps)
+        norm = MaggyRMSNorm8 if cfg.eight_bit else RMSNorm
+        self.attn_norm = norm(cfg.dim, cfg.norm_eps)
         self.attn = Attention(cfg)
-        self.ffn_norm = RMSNorm(cfg.dim, cfg.norm_eps)
-        self.ffn = FeedForward(cfg)
+        self.ffn_norm = norm(cfg.dim, cfg.norm_eps)
+        self.ffn = MaggyFeedForward8(cfg.dim, cfg.ffn_hidden) \
+            if cfg.eight_bit else FeedForward(cfg)
 
     def forward(self, x, cos, sin, cache=None, pos=0):
         x = x + self.attn(self.attn_norm(x), cos, sin, cache=cache, pos=pos)
         x = x + self.ffn(self.ffn_norm(x))
         return x
+
+
+def _packed_while(generate):
+    """Decode with the 8-bit weights packed once a call, unless the caller
+    has packed them (``pack8_model``)."""
+    @functools.wraps(generate)
+    def run(self, *args, **kw):
+        fresh = [g for g in groups8(self) if g.packed is None]
+        if not fresh:
+            return generate(self, *args, **kw)
+        try:
+            for g in fresh:
+                g.pack()
+            return generate(self, *args, **kw)
+        finally:
+            for g in fresh:
+                g.drop()
+    return run
 
 
 class LlamaModel(nn.Module):
@@ -250,6 +291,7 @@ class LlamaModel(nn.Module):
         return sum(p.numel() for p in self.parameters())
 
     @torch.no_grad()
+    @_packed_while
     def generate(self, tokens, max_new_tokens, temperature=0.0, top_k=None):
         """KV-cached autoregressive decoding (greedy at temperature 0).
 
@@ -284,6 +326,7 @@ class LlamaModel(nn.Module):
         return out
 
     @torch.no_grad()
+    @_packed_while
     def generate_captured(self, tokens, max_new_tokens, use_graph=True):
         """Greedy decode with a hipGraph-captured per-token step
         (EXPERIMENTAL: measured 868 vs 929 tok/s against the eager

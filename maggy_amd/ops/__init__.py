@@ -53,9 +53,27 @@ def has_ext():
 
 
 from maggy_amd.ops.fused_adam import FusedAdam, FusedSGD  # noqa: E402,F401
+from maggy_amd.ops.block8 import (  # noqa: E402,F401
+    Block8,
+    MaggyFeedForward8,
+    MaggyLinear8,
+    MaggyRMSNorm8,
+    Weight8,
+    drop8_model,
+    linear8,
+    pack8,
+    pack8_model,
+    pack_weight8,
+    rms_norm8,
+    swiglu8,
+    unpack8,
+)
 from maggy_amd.ops.reduce import grad_l2norm, metric_mean, metric_sum  # noqa: E402,F401
 
 __all__ = [
     "FusedAdam", "FusedSGD", "grad_l2norm", "metric_mean", "metric_sum",
     "require_ext", "ext_or_none", "has_ext",
+    "pack8", "unpack8", "swiglu8", "rms_norm8", "linear8", "pack_weight8",
+    "Block8", "Weight8", "MaggyLinear8", "MaggyRMSNorm8",
+    "MaggyFeedForward8", "pack8_model", "drop8_model",
 ]

@@ -1,0 +1,536 @@
+"""8-bit block operators: products, activations and norms of the Llama path
+that read, and keep for the backward pass, 8 bits a value.
+
+The format (``Block8``) is OCP e4m3 codes with one power-of-two scale for 128
+neighbouring values of a row: the scale is the smallest 2^t, t >= -126, with
+max|x| <= 448 * 2^t over the block's finite values, a code is x * 2^-t
+rounded to nearest even.  A value keeps 4 significant bits (an error of at
+most 1/16 of itself) down to 2^-14 of its block's largest.  Infinities and
+NaN are held as NaN and leave their neighbours alone.
+
+    pack8, unpack8   a tensor held in 8 bits, and read back
+    swiglu8          silu(g) * u; g and u are kept in 8 bits
+    rms_norm8        RMSNorm; x is kept in 8 bits
+    linear8          x @ W^T of 8-bit operands with both gradients; what is
+                     kept of x for dW is the operand that the product read
+    pack_weight8     weights packed once, for serving
+
+Forward results of ``swiglu8`` and ``rms_norm8`` come from the exact inputs;
+only their gradients see the 8-bit values.  On the GPU they take bfloat16,
+float16 and float32, ``linear8`` takes bfloat16 (weights also float32): the
+matrix unit aligns the products of 8-bit numbers before it adds them, which
+is worth about 16 bits, well inside bfloat16 but not float32.
+
+All run as HIP kernels on GPU tensors and raise without the extension; on the
+CPU the same definitions run in torch.
+"""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from maggy_amd import ops
+from maggy_amd.ops.fused_rms import MaggyRMSNorm
+from maggy_amd.ops.linear import MaggyFeedForward, MaggyLinear
+
+BLOCK = 128
+MAX_WEIGHTS = 4  # kMaxParts in block8_api.h
+
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _up(n, to):
+    return (n + to - 1) // to * to
+
+
+# ------------------------------------------------------- the format in torch
+def _scale_exponents(top):
+    """t of 2^t from the largest magnitudes of the blocks (float32)."""
+    frac, e = torch.frexp(top)  # top = frac * 2^e, 448 = 0.875 * 2^9
+    t = (e - 9 + (frac > 0.875)).clamp(min=-126)
+    return torch.where(top == 0, -126, t).int()
+
+
+def _power(t):
+    return ((t + 127) << 23).view(torch.float32)
+
+
+def _tops(blocks, dims):
+    a = blocks.abs()
+    return torch.where(a.isfinite(), a, 0).amax(dims, keepdim=True)
+
+
+def _encode(blocks, t):
+    v = blocks * _power(-t)
+    v = torch.where(v.isfinite(), v, float("nan"))
+    return v.to(torch.float8_e4m3fn)
+
+
+def _blocks(x):
+    """[R, C] -> float32 [R, Cp / 128, 128], padded with zeros."""
+    pad = -x.shape[1] % BLOCK
+    x = nn.functional.pad(x.float(), (0, pad))
+    return x.reshape(x.shape[0], x.shape[1] // BLOCK, BLOCK)
+
+
+def _held(x):
+    """The float32 values of the 2-D ``x`` in blocks along its rows."""
+    b = _blocks(x)
+    t = _scale_exponents(_tops(b, -1))
+    v = _encode(b, t).float() * _power(t)
+    return v.flatten(1)[:, :x.shape[1]]
+
+
+def _held_weight(w):
+    """The float32 values of ``w`` in blocks of 128 x 128."""
+    n, k = w.shape
+    p = nn.functional.pad(w.float(), (0, -k % BLOCK, 0, -n % BLOCK))
+    b = p.view(p.shape[0] // BLOCK, BLOCK, p.shape[1] // BLOCK, BLOCK)
+    t = _scale_exponents(_tops(b, (1, 3)))
+    v = _encode(b, t).float() * _power(t)
+    return v.view(p.shape)[:n, :k]
+
+
+def _pack_cpu(x):
+    R = x.shape[0]
+    b = _blocks(x)
+    t = _scale_exponents(_tops(b, -1))
+    codes = _encode(b, t).view(torch.uint8).flatten(1)
+    E = (t + 127).to(torch.uint8).flatten(1)
+    E = nn.functional.pad(E, (0, -E.shape[1] % 4), value=1)
+    scales = torch.ones(E.shape[1] // 4, _up(R, 256), 4, dtype=torch.uint8)
+    scales[:, :R] = E.unflatten(1, (-1, 4)).transpose(0, 1)
+    return codes, scales
+
+
+def _unpack_cpu(codes, scales, C, dtype):
+    R, Cp = codes.shape
+    E = scales[:, :R].transpose(0, 1).flatten(1)[:, :Cp // BLOCK]
+    v = codes.view(torch.float8_e4m3fn).float().unflatten(1, (-1, BLOCK))
+    v = v * _power(E.int()[..., None] - 127)
+    most = torch.finfo(dtype).max
+    # a value next to the type's largest may have been rounded up past it
+    v = torch.where(v.isnan(), v, v.clamp(-most, most))
+    return v.flatten(1)[:, :C].to(dtype)
+
+
+# -------------------------------------------------------------- pack, unpack
+class Block8:
+    """A tensor held in 8 bits a value (``pack8``), read by ``unpack8``.
+
+    ``codes`` [rows, C up to 128] and ``scales`` are uint8 tensors; leading
+    axes are flattened into rows.  ``shape`` and ``dtype`` are those of the
+    tensor that was packed."""
+
+    __slots__ = ("codes", "scales", "shape", "dtype")
+
+    def __init__(self, codes, scales, shape, dtype):
+        self.codes = codes
+        self.scales = scales
+        self.shape = shape
+        self.dtype = dtype
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def __repr__(self):
+        return "Block8(shape={}, dtype={}, device={})".format(
+            tuple(self.shape), self.dtype, self.device)
+
+
+def _check_float(x, what):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("{} must be a tensor, got {}".format(
+            what, type(x).__name__))
+    if x.dtype not in _FLOATS:
+        raise TypeError("{} must be bfloat16, float16 or float32, got "
+                        "{}".format(what, x.dtype))
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("{} needs a last axis of at least 1, got shape "
+                         "{}".format(what, tuple(x.shape)))
+
+
+def _rows(x):
+    """[..., C] as a matrix; a view where the strides allow it."""
+    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+
+
+@torch.no_grad()
+def pack8(x):
+    """Hold ``x`` [..., C] in 8 bits, blocks of 128 along the last axis."""
+    _check_float(x, "x")
+    x2 = _rows(x)
+    if x.is_cuda:
+        codes, scales = ops.require_ext().pack8(x2)
+    else:
+        codes, scales = _pack_cpu(x2)
+    return Block8(codes, scales, x.shape, x.dtype)
+
+
+@torch.no_grad()
+def unpack8(held, dtype=None):
+    """The tensor that ``held`` (a ``Block8``) stands for."""
+    if not isinstance(held, Block8):
+        raise TypeError("unpack8 takes a Block8, got {}".format(
+            type(held).__name__))
+    dtype = held.dtype if dtype is None else dtype
+    if dtype not in _FLOATS:
+        raise TypeError("dtype must be bfloat16, float16 or float32, got "
+                        "{}".format(dtype))
+    C = held.shape[-1]
+    if held.codes.is_cuda:
+        out = ops.require_ext().unpack8(held.codes, held.scales, C, dtype)
+    else:
+        out = _unpack_cpu(held.codes, held.scales, C, dtype)
+    return out.view(held.shape)
+
+
+# -------------------------------------------------------------------- swiglu
+def _swiglu_cpu(g, u):
+    gf = g.float()
+    return (gf * torch.sigmoid(gf) * u.float()).to(g.dtype)
+
+
+class _SwiGLU8Function(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, u):
+        if g.is_cuda:
+            h, *kept = ops.require_ext().swiglu8_fwd(g, u, True)
+        else:
+            h = _swiglu_cpu(g, u)
+            kept = (*_pack_cpu(g), *_pack_cpu(u))
+        ctx.save_for_backward(*kept)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        if dh.is_cuda:
+            dg, du = ops.require_ext().swiglu8_bwd(dh, *ctx.saved_tensors)
+        else:
+            gc, gs, uc, us = ctx.saved_tensors
+            C, d = dh.shape[1], dh.float()
+            g = _unpack_cpu(gc, gs, C, torch.float32)
+            u = _unpack_cpu(uc, us, C, torch.float32)
+            s = torch.sigmoid(g)
+            dg = (d * u * s * (1 + g * (1 - s))).to(dh.dtype)
+            du = (d * g * s).to(dh.dtype)
+        return dg, du
+
+
+def swiglu8(g, u):
+    """silu(g) * u over [..., C]; the backward pass reads ``g`` and ``u`` as
+    they are held in 8 bits (2 bytes a pair, where ``swiglu`` keeps 4)."""
+    _check_float(g, "g")
+    _check_float(u, "u")
+    if g.shape != u.shape or g.dtype != u.dtype or g.device != u.device:
+        raise ValueError("g and u must agree in shape, type and device: "
+                         "{} {} {}, {} {} {}".format(
+                             tuple(g.shape), g.dtype, g.device,
+                             tuple(u.shape), u.dtype, u.device))
+    shape, g, u = g.shape, _rows(g), _rows(u)
+    if torch.is_grad_enabled() and (g.requires_grad or u.requires_grad):
+        h = _SwiGLU8Function.apply(g, u)
+    elif g.is_cuda:
+        h, = ops.require_ext().swiglu8_fwd(g, u, False)
+    else:
+        h = _swiglu_cpu(g, u)
+    return h.view(shape)
+
+
+# ------------------------------------------------------------------- RMSNorm
+def _inv_rms(x, eps):
+    x = x.float()
+    return torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps)
+
+
+class _RMSNorm8Function(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps):
+        if x.is_cuda:
+            y, codes, scales, inv = ops.require_ext().rms8_fwd(
+                x, weight, eps, True)
+        else:
+            inv = _inv_rms(x, eps)
+            y = (x.float() * inv * weight).to(x.dtype)
+            codes, scales = _pack_cpu(x)
+        ctx.save_for_backward(codes, scales, inv, weight)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, scales, inv, weight = ctx.saved_tensors
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        if dy.is_cuda:
+            dx, dw = ops.require_ext().rms8_bwd(
+                dy, codes, scales, weight, inv, need_dx, need_dw)
+        else:
+            d = dy.float()
+            n = _unpack_cpu(codes, scales, d.shape[1], torch.float32) * inv
+            a = d * weight
+            dx = inv * (a - n * (a * n).mean(-1, keepdim=True))
+            dx, dw = dx.to(dy.dtype), (d * n).sum(0)
+        return dx if need_dx else None, dw if need_dw else None, None
+
+
+def rms_norm8(x, weight, eps=1e-5):
+    """RMSNorm of ``x`` [..., C] with ``weight`` [C], C up to 16384 on the
+    GPU; the backward pass reads ``x`` as it is held in 8 bits."""
+    _check_float(x, "x")
+    _check_float(weight, "weight")
+    if weight.shape != x.shape[-1:] or weight.device != x.device:
+        raise ValueError("weight must be [{}] on {}, got {} on {}".format(
+            x.shape[-1], x.device, tuple(weight.shape), weight.device))
+    # the kernels take a float32 weight; .float() is differentiable
+    weight = weight.float().contiguous()
+    shape, x = x.shape, _rows(x)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        y = _RMSNorm8Function.apply(x, weight, eps)
+    elif x.is_cuda:
+        y, = ops.require_ext().rms8_fwd(x, weight, eps, False)
+    else:
+        y = (x.float() * _inv_rms(x, eps) * weight).to(x.dtype)
+    return y.view(shape)
+
+
+# -------------------------------------------------------------------- linear
+class Weight8:
+    """Weights packed once (``pack_weight8``) for ``linear8`` in serving."""
+
+    __slots__ = ("codes", "scales", "counts", "columns")
+
+    def __init__(self, codes, scales, counts, columns):
+        self.codes = codes
+        self.scales = scales
+        self.counts = counts
+        self.columns = columns
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def __repr__(self):
+        return "Weight8(rows={}, columns={}, device={})".format(
+            self.counts, self.columns, self.device)
+
+
+def _check_weights(weights):
+    if not 1 <= len(weights) <= MAX_WEIGHTS:
+        raise ValueError("1 to {} weights, got {}".format(
+            MAX_WEIGHTS, len(weights)))
+    first = weights[0]
+    for w in weights:
+        _check_float(w, "weight")
+        if w.dim() != 2 or w.shape[0] == 0:
+            raise ValueError("a weight must be [N, K], got {}".format(
+                tuple(w.shape)))
+        if w.dtype == torch.float16:
+            raise TypeError("weights must be bfloat16 or float32")
+        if (w.shape[1], w.dtype, w.device) != (
+                first.shape[1], first.dtype, first.device):
+            raise ValueError("weights must agree in columns, type and "
+                             "device")
+
+
+@torch.no_grad()
+def pack_weight8(*weights):
+    """Pack one to four weights [N_i, K] that read the same input, blocks of
+    128 x 128, for ``linear8(x, packed)`` under no_grad."""
+    _check_weights(weights)
+    counts = [w.shape[0] for w in weights]
+    K = weights[0].shape[1]
+    if weights[0].is_cuda:
+        codes, scales = ops.require_ext().pack8_weights(list(weights))
+    else:
+        # every weight starts at a multiple of 128 rows
+        rows = torch.cat([nn.functional.pad(
+            _held_weight(w), (0, 0, 0, -w.shape[0] % BLOCK))
+            for w in weights])
+        codes, scales = _pack_cpu(rows)
+    return Weight8(codes, scales, counts, K)
+
+
+class _Linear8Function(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, *weights):
+        if x.is_cuda:
+            *ys, codes, scales = ops.require_ext().linear8_fwd(
+                x, list(weights))
+        else:
+            held = _held(x)
+            ys = [(held @ _held_weight(w).t()).to(x.dtype) for w in weights]
+            codes, scales = _pack_cpu(x)
+        if any(ctx.needs_input_grad[1:]):
+            ctx.save_for_backward(codes, scales, *weights)
+        else:  # dX does not read x
+            ctx.save_for_backward(None, None, *weights)
+        return tuple(ys)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *dys):
+        codes, scales, *weights = ctx.saved_tensors
+        need_dx, need_dw = ctx.needs_input_grad[0], \
+            any(ctx.needs_input_grad[1:])
+        if dys[0].is_cuda:
+            dx, *dws = ops.require_ext().linear8_bwd(
+                list(dys), codes, scales, weights, need_dx, need_dw)
+        else:
+            dx, dws = _linear8_backward_cpu(dys, codes, scales, weights,
+                                            need_dx, need_dw)
+        if not need_dw:
+            dws = [None] * len(weights)
+        return (dx if need_dx else None,
+                *(d if need else None
+                  for d, need in zip(dws, ctx.needs_input_grad[1:])))
+
+
+def _linear8_backward_cpu(dys, codes, scales, weights, need_dx, need_dw):
+    dx, dws = None, []
+    if need_dx:
+        dx = sum(_held(d) @ _held_weight(w) for d, w in zip(dys, weights))
+        dx = dx.to(dys[0].dtype)
+    if need_dw:
+        x = _unpack_cpu(codes, scales, weights[0].shape[1], torch.float32)
+        xt = _held(x.t())
+        dws = [(_held(d.t()) @ xt.t()).to(w.dtype)
+               for d, w in zip(dys, weights)]
+    return dx, dws
+
+
+def linear8(x, *weights):
+    """``x`` [..., K] times the transpose of one to four ``weights``
+    [N_i, K], all operands in 8 bits: one result, or a tuple of as many as
+    there are weights (they share one packed ``x`` and one product).
+
+    dX = dY W and dW = dY^T X are 8-bit products too: dY is packed along the
+    axis each of them sums over, and x is kept for dW in the 8 bits that the
+    forward product read.  With one ``Weight8`` in the place of the weights
+    nothing is packed but x, and there is no backward pass."""
+    _check_float(x, "x")
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        x = x.to(torch.get_autocast_dtype("cuda"))
+    if any(isinstance(w, Weight8) for w in weights):
+        if len(weights) > 1:
+            raise TypeError("pack weights that share an input together: "
+                            "pack_weight8(w1, w2, ...)")
+        _check_input(x, weights[0].columns, weights[0].device)
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("packed weights have no backward pass: call "
+                               "linear8 with the weights, or under no_grad")
+        ys = _linear8_packed(_rows(x), weights[0])
+    else:
+        _check_weights(weights)
+        _check_input(x, weights[0].shape[1], weights[0].device)
+        if torch.is_grad_enabled() and (
+                x.requires_grad or any(w.requires_grad for w in weights)):
+            ys = _Linear8Function.apply(_rows(x), *weights)
+        else:
+            ys = _linear8_packed(_rows(x), pack_weight8(*weights))
+    if x.dim() != 2:
+        ys = tuple(y.view(*x.shape[:-1], y.shape[-1]) for y in ys)
+    return tuple(ys) if len(ys) > 1 else ys[0]
+
+
+def _check_input(x, K, device):
+    if x.shape[-1] != K or x.device != device:
+        raise ValueError("x must be [..., {}] on {}, got {} on {}".format(
+            K, device, tuple(x.shape), x.device))
+    if x.is_cuda and x.dtype != torch.bfloat16:
+        raise TypeError("linear8 takes bfloat16 on the GPU, got {}".format(
+            x.dtype))
+
+
+@torch.no_grad()
+def _linear8_packed(x, w):
+    if x.is_cuda:
+        return ops.require_ext().linear8_packed(x, w.codes, w.scales,
+                                                w.counts, w.columns)
+    values = _unpack_cpu(w.codes, w.scales, w.columns, torch.float32)
+    held, ys, at = _held(x), [], 0
+    for n in w.counts:
+        ys.append((held @ values[at:at + n].t()).to(x.dtype))
+        at += _up(n, BLOCK)
+    return ys
+
+
+# ------------------------------------------------------------------- modules
+class Linear8Group:
+    """Bias-free linear modules that read the same input, run as one
+    ``linear8``.  ``pack`` keeps their weights packed for calls without
+    gradients, until ``drop``; it belongs after the last weight update."""
+
+    def __init__(self, *linears):
+        for m in linears:
+            if m.bias is not None:
+                raise ValueError("linear8 has no bias")
+        self.linears = linears
+        self.packed = None
+
+    def pack(self):
+        self.packed = pack_weight8(*(m.weight for m in self.linears))
+
+    def drop(self):
+        self.packed = None
+
+    def __call__(self, x):
+        if self.packed is not None and not torch.is_grad_enabled():
+            return linear8(x, self.packed)
+        return linear8(x, *(m.weight for m in self.linears))
+
+
+class MaggyLinear8(MaggyLinear):
+    """Drop-in bias-free nn.Linear on ``linear8``."""
+
+    def __init__(self, in_features, out_features, bias=False, **kw):
+        super().__init__(in_features, out_features, bias=bias, **kw)
+        self.group = Linear8Group(self)
+
+    def forward(self, x):
+        return self.group(x)
+
+
+class MaggyRMSNorm8(MaggyRMSNorm):
+    """Drop-in MaggyRMSNorm on ``rms_norm8``."""
+
+    def forward(self, x):
+        return rms_norm8(x, self.weight, self.eps)
+
+
+class MaggyFeedForward8(MaggyFeedForward):
+    """Llama FFN w2(silu(w1 x) * w3 x) in 8 bits: w1 and w3 share one packed
+    input and one product, and all that the backward pass keeps is 8-bit
+    (x, both halves and their product), 1 byte a value."""
+
+    def __init__(self, dim, ffn_hidden):
+        super().__init__(dim, ffn_hidden)
+        self.up8 = Linear8Group(self.w1, self.w3)
+        self.down8 = Linear8Group(self.w2)
+
+    def forward(self, x):
+        return self.down8(swiglu8(*self.up8(x)))
+
+
+def groups8(module):
+    """The ``Linear8Group``s of a model."""
+    return [g for m in module.modules() for g in vars(m).values()
+            if isinstance(g, Linear8Group)]
+
+
+def pack8_model(module):
+    """Pack the weights of every 8-bit linear of a model for serving; after
+    a weight update call it again, or ``drop8_model``."""
+    for g in groups8(module):
+        g.pack()
+
+
+def drop8_model(module):
+    for g in groups8(module):
+        g.drop()

@@ -21,11 +21,18 @@ SOURCES = [
     os.path.join(HIP_DIR, "fused_bn.hip"),
     os.path.join(HIP_DIR, "fused_rms.hip"),
     os.path.join(HIP_DIR, "gemm.hip"),
+    os.path.join(HIP_DIR, "bindings8.cpp"),
+    os.path.join(HIP_DIR, "block8.hip"),
+    os.path.join(HIP_DIR, "gemm8.hip"),
+]
+HEADERS = [
+    os.path.join(HIP_DIR, "block8.h"),
+    os.path.join(HIP_DIR, "block8_api.h"),
 ]
 
 
 def _sources_mtime():
-    return max(os.path.getmtime(s) for s in SOURCES)
+    return max(os.path.getmtime(s) for s in SOURCES + HEADERS)
 
 
 def is_built():
@@ -41,12 +48,22 @@ def build(verbose=False, force=False):
     os.makedirs(BUILD_DIR, exist_ok=True)
     from torch.utils.cpp_extension import load
 
+    # the generated ninja file knows no header of a .hip source
+    newest = max(os.path.getmtime(h) for h in HEADERS)
+    for f in os.listdir(BUILD_DIR):
+        path = os.path.join(BUILD_DIR, f)
+        if f.endswith(".cuda.o") and os.path.getmtime(path) < newest:
+            os.remove(path)
     load(
         name=SO_NAME,
         sources=SOURCES,
         build_directory=BUILD_DIR,
         extra_cflags=["-O3"],
-        extra_cuda_cflags=["-O3", "--offload-arch=gfx950"],
+        # packed fp32 arithmetic is off: some of its forms have given wrong
+        # results on this hardware
+        extra_cuda_cflags=["-O3", "--offload-arch=gfx950", "-Xclang",
+                           "-target-feature", "-Xclang",
+                           "-packed-fp32-ops"],
         verbose=verbose,
         is_python_module=True,
         keep_intermediates=True,

@@ -291,7 +291,10 @@ torch::Tensor rope(torch::Tensor x, torch::Tensor cost, torch::Tensor sint,
 
 }  // namespace
 
+void bind_block8(pybind11::module_& m);  // bindings8.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_block8(m);
   m.def("multi_l2norm_sq", &multi_l2norm_sq,
         "sum of squares over the chunk table -> norm_sq[0]");
   m.def("multi_fused_adam", &multi_fused_adam,

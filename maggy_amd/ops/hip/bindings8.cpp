@@ -1,0 +1,499 @@
+// pybind11 bindings of the 8-bit block operators (block8.hip, gemm8.hip).
+//
+// Everything that the kernels assume is checked here: device, type, shape,
+// and the strides and alignment that choose the 16-byte loads.  Matrices
+// come with any row stride; the last axis is made contiguous if it is not.
+// Outputs and workspaces come from torch's allocator, on the tensors' own
+// device and the current stream of that device.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <limits>
+
+#include "block8_api.h"
+
+namespace {
+
+using torch::Tensor;
+using c10::cuda::CUDAGuard;
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+hipStream_t stream_of(const Tensor& t) {
+  return at::cuda::getCurrentCUDAStream(t.get_device()).stream();
+}
+
+int type_of(const Tensor& t, const char* name) {
+  if (t.scalar_type() == torch::kBFloat16) return 0;
+  if (t.scalar_type() == torch::kFloat16) return 1;
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32, name,
+              " must be bfloat16, float16 or float32, got ", t.scalar_type());
+  return 2;
+}
+
+// a 2-D matrix on the GPU whose columns are contiguous
+Tensor matrix(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
+  TORCH_CHECK(t.dim() == 2, name, " must be 2-D, got ", t.dim(), "-D");
+  type_of(t, name);
+  TORCH_CHECK(t.size(1) >= 1, name, " has no columns");
+  TORCH_CHECK(t.size(0) < (int64_t)1 << 31 && t.size(1) < (int64_t)1 << 30,
+              name, " is too large");
+  if (t.size(1) > 1 && t.stride(1) != 1) return t.contiguous();
+  return t;
+}
+
+// whether rows of t can be read in groups of 8 by 16-byte loads
+bool vec8(const Tensor& t) {
+  return t.size(1) % 8 == 0 && (t.size(0) <= 1 || t.stride(0) % 8 == 0) &&
+         (uintptr_t)t.data_ptr() % 16 == 0;
+}
+
+// rows of one element or none may carry any stride
+int64_t ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+
+void same_device(const Tensor& a, const Tensor& b, const char* name) {
+  TORCH_CHECK(a.device() == b.device(), name, " is on ", b.device(),
+              ", expected ", a.device());
+}
+
+struct Packed {
+  Tensor codes, scales;  // [rows][Cp], [Q][Rp][4]
+  uint8_t* c() const { return codes.data_ptr<uint8_t>(); }
+  uint32_t* s() const { return (uint32_t*)scales.data_ptr<uint8_t>(); }
+  int64_t Cp() const { return codes.size(1); }
+  int64_t Rp() const { return scales.size(1); }
+};
+
+Packed new_packed(int64_t rows, int64_t C, const Tensor& like) {
+  const auto o = like.options().dtype(torch::kUInt8).requires_grad(false);
+  const int64_t Cp = up(C, 128);
+  return {torch::empty({rows, Cp}, o),
+          torch::empty({(Cp + 511) / 512, up(rows, 256), 4}, o)};
+}
+
+Packed packed(const Tensor& codes, const Tensor& scales, const char* name) {
+  TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == torch::kUInt8 &&
+                  codes.dim() == 2 && codes.is_contiguous() &&
+                  codes.size(1) % 128 == 0,
+              name, ": codes must be contiguous uint8 [rows][128 n]");
+  TORCH_CHECK(scales.scalar_type() == torch::kUInt8 && scales.dim() == 3 &&
+                  scales.is_contiguous() &&
+                  scales.size(0) == (codes.size(1) + 511) / 512 &&
+                  scales.size(1) == up(codes.size(0), 256) &&
+                  scales.size(2) == 4,
+              name, ": scales do not fit the codes");
+  same_device(codes, scales, name);
+  return {codes, scales};
+}
+
+Packed pack_rows(const Tensor& x) {
+  Packed p = new_packed(x.size(0), x.size(1), x);
+  if (x.size(0))
+    launch_b8_pack(type_of(x, "x"), vec8(x), x.data_ptr(), ld(x), x.size(0),
+                   (int)x.size(1), p.c(), (int)p.Cp(), p.s(), p.Rp(),
+                   stream_of(x));
+  return p;
+}
+
+std::vector<Tensor> pack8(Tensor x) {
+  x = matrix(x, "x");
+  const CUDAGuard guard(x.device());
+  const Packed p = pack_rows(x);
+  return {p.codes, p.scales};
+}
+
+Tensor unpack8(Tensor codes, Tensor scales, int64_t C,
+               torch::ScalarType dtype) {
+  const Packed p = packed(codes, scales, "unpack8");
+  TORCH_CHECK(C >= 1 && up(C, 128) == p.Cp(), "unpack8: ", C,
+              " columns do not fit the codes");
+  const CUDAGuard guard(codes.device());
+  const int64_t R = codes.size(0);
+  Tensor out = torch::empty({R, C}, codes.options().dtype(dtype));
+  if (R)
+    launch_b8_unpack(type_of(out, "out"), C % 8 == 0, p.c(), (int)p.Cp(),
+                     p.s(), p.Rp(), R, (int)C, out.data_ptr(),
+                     stream_of(codes));
+  return out;
+}
+
+// ------------------------------------------------------------------ swiglu
+std::vector<Tensor> swiglu8_fwd(Tensor g, Tensor u, bool keep) {
+  g = matrix(g, "g");
+  u = matrix(u, "u");
+  TORCH_CHECK(g.sizes() == u.sizes() && g.scalar_type() == u.scalar_type(),
+              "swiglu8: g and u must agree in shape and type");
+  same_device(g, u, "u");
+  const CUDAGuard guard(g.device());
+  const int64_t R = g.size(0), C = g.size(1);
+  Tensor h = torch::empty({R, C}, g.options().requires_grad(false));
+  Packed pg, pu;
+  if (keep) pg = new_packed(R, C, g), pu = new_packed(R, C, g);
+  if (R)
+    launch_b8_swiglu_fwd(type_of(g, "g"), vec8(g) && vec8(u), g.data_ptr(),
+                         ld(g), u.data_ptr(), ld(u), R, (int)C, h.data_ptr(),
+                         keep ? pg.c() : nullptr, keep ? pu.c() : nullptr,
+                         (int)up(C, 128), keep ? pg.s() : nullptr,
+                         keep ? pu.s() : nullptr, keep ? pg.Rp() : 0,
+                         stream_of(g));
+  if (!keep) return {h};
+  return {h, pg.codes, pg.scales, pu.codes, pu.scales};
+}
+
+std::vector<Tensor> swiglu8_bwd(Tensor dh, Tensor gc, Tensor gs, Tensor uc,
+                                Tensor us) {
+  dh = matrix(dh, "dh");
+  const Packed g = packed(gc, gs, "swiglu8"), u = packed(uc, us, "swiglu8");
+  const int64_t R = dh.size(0), C = dh.size(1);
+  TORCH_CHECK(gc.sizes() == uc.sizes() && gc.size(0) == R &&
+                  gc.size(1) == up(C, 128),
+              "swiglu8: the gradient does not fit what was kept");
+  same_device(dh, gc, "g");
+  same_device(dh, uc, "u");
+  const CUDAGuard guard(dh.device());
+  const auto o = dh.options().requires_grad(false);
+  Tensor dg = torch::empty({R, C}, o), du = torch::empty({R, C}, o);
+  if (R)
+    launch_b8_swiglu_bwd(type_of(dh, "dh"), vec8(dh), dh.data_ptr(), ld(dh),
+                         g.c(), u.c(), (int)g.Cp(), g.s(), u.s(), g.Rp(), R,
+                         (int)C, dg.data_ptr(), du.data_ptr(), stream_of(dh));
+  return {dg, du};
+}
+
+// ----------------------------------------------------------------- RMSNorm
+constexpr int64_t kRmsMost = 16384;  // columns that rms_fwd/rms_bwd hold
+
+void check_rms_weight(const Tensor& x, const Tensor& w) {
+  TORCH_CHECK(w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous() &&
+                  w.scalar_type() == torch::kFloat32,
+              "rms_norm8: weight must be contiguous float32 [", x.size(1),
+              "]");
+  same_device(x, w, "weight");
+}
+
+std::vector<Tensor> rms8_fwd(Tensor x, Tensor w, double eps, bool keep) {
+  x = matrix(x, "x");
+  const int64_t R = x.size(0), C = x.size(1);
+  TORCH_CHECK(C <= kRmsMost, "rms_norm8: at most ", kRmsMost,
+              " columns, got ", C);
+  check_rms_weight(x, w);
+  const CUDAGuard guard(x.device());
+  const auto o = x.options().requires_grad(false);
+  Tensor y = torch::empty({R, C}, o);
+  Packed p;
+  Tensor inv;
+  if (keep) {
+    p = new_packed(R, C, x);
+    inv = torch::empty({R}, o.dtype(torch::kFloat32));
+  }
+  if (R)
+    launch_b8_rms_fwd(type_of(x, "x"),
+                      vec8(x) && (uintptr_t)w.data_ptr() % 16 == 0,
+                      x.data_ptr(), ld(x), w.data_ptr<float>(), R, (int)C,
+                      (float)eps, y.data_ptr(),
+                      keep ? inv.data_ptr<float>() : nullptr,
+                      keep ? p.c() : nullptr, (int)up(C, 128),
+                      keep ? p.s() : nullptr, keep ? p.Rp() : 0,
+                      stream_of(x));
+  if (!keep) return {y};
+  return {y, p.codes, p.scales, inv};
+}
+
+std::vector<c10::optional<Tensor>> rms8_bwd(Tensor dy, Tensor codes,
+                                            Tensor scales, Tensor w,
+                                            Tensor inv, bool need_dx,
+                                            bool need_dw) {
+  dy = matrix(dy, "dy");
+  const Packed p = packed(codes, scales, "rms_norm8");
+  const int64_t R = dy.size(0), C = dy.size(1);
+  TORCH_CHECK(C <= kRmsMost && codes.size(0) == R &&
+                  codes.size(1) == up(C, 128),
+              "rms_norm8: the gradient does not fit what was kept");
+  TORCH_CHECK(inv.numel() == R && inv.is_contiguous() &&
+                  inv.scalar_type() == torch::kFloat32,
+              "rms_norm8: inv must be float32 [", R, "]");
+  check_rms_weight(dy, w);
+  same_device(dy, codes, "codes");
+  same_device(dy, inv, "inv");
+  const CUDAGuard guard(dy.device());
+  const auto f32 = dy.options().dtype(torch::kFloat32).requires_grad(false);
+  c10::optional<Tensor> dx, dw;
+  Tensor partials;
+  if (need_dx)
+    dx = torch::empty({R, C}, dy.options().requires_grad(false));
+  if (need_dw) {
+    if (R == 0) {
+      dw = torch::zeros({C}, f32);
+    } else {
+      dw = torch::empty({C}, f32);
+      partials = torch::empty({b8_rms_bwd_partials(R, (int)C), C}, f32);
+    }
+  }
+  if (R && (need_dx || need_dw))
+    launch_b8_rms_bwd(type_of(dy, "dy"),
+                      vec8(dy) && (uintptr_t)w.data_ptr() % 16 == 0,
+                      dy.data_ptr(), ld(dy), p.c(), (int)p.Cp(), p.s(),
+                      p.Rp(), w.data_ptr<float>(), inv.data_ptr<float>(), R,
+                      (int)C, dx ? dx->data_ptr() : nullptr,
+                      need_dw ? partials.data_ptr<float>() : nullptr,
+                      need_dw ? dw->data_ptr<float>() : nullptr,
+                      stream_of(dy));
+  return {dx, dw};
+}
+
+// ----------------------------------------------------------------- linear8
+// the first row of each weight when they are stacked, and the total
+std::vector<int64_t> firsts(const std::vector<int64_t>& counts) {
+  std::vector<int64_t> f{0};
+  for (int64_t n : counts) f.push_back(f.back() + up(n, 128));
+  return f;
+}
+
+void check_counts(const std::vector<int64_t>& counts) {
+  TORCH_CHECK(counts.size() >= 1 && counts.size() <= b8::kMaxParts,
+              "linear8 takes 1 to ", b8::kMaxParts, " weights, got ",
+              counts.size());
+}
+
+enum Tiles {
+  kBoth = 0,
+  kCols = 1,
+  kOneRows = 2,
+  kOneCols = 3,
+  kFrom8 = 4,
+  kRows = 5
+};
+
+// packs t by 128 x 128 tiles into rows and/or into the transposed cols, its
+// first value landing at row r0 and column c0 of each
+void run_tiles(Tiles what, const Tensor& t, Packed* rows, int64_t row_r0,
+               int64_t row_c0, Packed* cols, int64_t col_r0,
+               int64_t col_c0) {
+  const bool by_rows = what == kBoth || what == kOneRows || what == kRows;
+  const bool by_cols = what == kBoth || what == kOneCols || what == kCols;
+  TORCH_CHECK(by_rows == (rows != nullptr) && by_cols == (cols != nullptr),
+              "run_tiles: outputs do not match the kernel");
+  b8::TileArgs a{};
+  a.x = t.data_ptr();
+  a.ldx = ld(t);
+  a.R = t.size(0);
+  a.C = (int)t.size(1);
+  if (rows) {
+    a.row_codes = rows->c();
+    a.row_scales = (uint8_t*)rows->s();
+    a.row_ld = rows->Cp();
+    a.row_sp = rows->Rp();
+    a.row_r0 = row_r0;
+    a.row_c0 = row_c0;
+  }
+  if (cols) {
+    a.col_codes = cols->c();
+    a.col_scales = (uint8_t*)cols->s();
+    a.col_ld = cols->Cp();
+    a.col_sp = cols->Rp();
+    a.col_r0 = col_r0;
+    a.col_c0 = col_c0;
+  }
+  TORCH_CHECK((a.R + 127) / 128 * ((a.C + 127) / 128) < (int64_t)1 << 31,
+              "matrix is too large");
+  launch_b8_tiles(what, type_of(t, "matrix"), vec8(t), &a, stream_of(t));
+}
+
+Packed pack_stacked(const std::vector<Tensor>& ws,
+                    const std::vector<int64_t>& first) {
+  Packed p = new_packed(first.back(), ws[0].size(1), ws[0]);
+  for (size_t i = 0; i < ws.size(); ++i)
+    run_tiles(kOneRows, ws[i], &p, first[i], 0, nullptr, 0, 0);
+  return p;
+}
+
+std::vector<Tensor> weights_of(const std::vector<Tensor>& weights,
+                               std::vector<int64_t>* counts) {
+  std::vector<Tensor> ws;
+  for (const Tensor& w : weights) {
+    ws.push_back(matrix(w, "weight"));
+    TORCH_CHECK(w.size(0) >= 1, "weight has no rows");
+    TORCH_CHECK(w.size(1) == weights[0].size(1) &&
+                    w.scalar_type() == weights[0].scalar_type(),
+                "linear8: weights must agree in columns and type");
+    TORCH_CHECK(w.scalar_type() != torch::kFloat16,
+                "linear8: weights must be bfloat16 or float32");
+    same_device(weights[0], w, "weight");
+    counts->push_back(w.size(0));
+  }
+  check_counts(*counts);
+  return ws;
+}
+
+std::vector<Tensor> product(const Packed& x, const Packed& w, int64_t M,
+                            const std::vector<int64_t>& counts,
+                            torch::ScalarType dtype) {
+  const auto first = firsts(counts);
+  TORCH_CHECK(x.Cp() == w.Cp(), "linear8: columns do not match");
+  b8::GemmArgs a{};
+  a.x = x.c();
+  a.xs = x.s();
+  a.ldx = x.Cp();
+  a.xsp = x.Rp();
+  a.w = w.c();
+  a.ws = w.s();
+  a.ldw = w.Cp();
+  a.wsp = w.Rp();
+  TORCH_CHECK(M < (int64_t)1 << 30 && first.back() < (int64_t)1 << 30,
+              "linear8: too many rows");
+  a.M = (int)M;
+  a.N = (int)std::min(first.back(), w.codes.size(0));
+  a.KT = (int)(x.Cp() / 128);
+  a.parts = (int)counts.size();
+  a.f32 = dtype == torch::kFloat32;
+  std::vector<Tensor> out;
+  for (size_t i = 0; i < counts.size(); ++i) {
+    out.push_back(torch::empty({M, counts[i]}, x.codes.options().dtype(dtype)));
+    a.out[i] = out[i].data_ptr();
+    a.first[i] = (int)first[i];
+    a.count[i] = (int)counts[i];
+  }
+  if (M) launch_b8_gemm(&a, stream_of(x.codes));
+  return out;
+}
+
+void check_bf16(const Tensor& x) {
+  TORCH_CHECK(x.scalar_type() == torch::kBFloat16,
+              "linear8 runs in bfloat16 on the GPU, got ", x.scalar_type());
+}
+
+// the stacked weights by their rows
+std::vector<Tensor> pack8_weights(std::vector<Tensor> weights) {
+  std::vector<int64_t> counts;
+  const auto ws = weights_of(weights, &counts);
+  const CUDAGuard guard(ws[0].device());
+  const Packed p = pack_stacked(ws, firsts(counts));
+  return {p.codes, p.scales};
+}
+
+// outputs, then the codes and scales of x
+std::vector<Tensor> linear8_fwd(Tensor x, std::vector<Tensor> weights) {
+  check_bf16(x);
+  x = matrix(x, "x");
+  std::vector<int64_t> counts;
+  const auto ws = weights_of(weights, &counts);
+  TORCH_CHECK(ws[0].size(1) == x.size(1), "linear8: x has ", x.size(1),
+              " columns, the weights ", ws[0].size(1));
+  same_device(x, ws[0], "weight");
+  const CUDAGuard guard(x.device());
+  const Packed p = pack_rows(x);
+  auto out = product(p, pack_stacked(ws, firsts(counts)), x.size(0), counts,
+                     torch::kBFloat16);
+  out.push_back(p.codes);
+  out.push_back(p.scales);
+  return out;
+}
+
+std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
+                                   std::vector<int64_t> counts, int64_t K) {
+  check_bf16(x);
+  x = matrix(x, "x");
+  check_counts(counts);
+  const Packed w = packed(wcodes, wscales, "linear8");
+  TORCH_CHECK(firsts(counts).back() == w.codes.size(0) &&
+                  up(K, 128) == w.Cp(),
+              "linear8: the packed weights do not have these shapes");
+  TORCH_CHECK(x.size(1) == K, "linear8: x has ", x.size(1),
+              " columns, the weights ", K);
+  same_device(x, wcodes, "weight");
+  const CUDAGuard guard(x.device());
+  return product(pack_rows(x), w, x.size(0), counts, torch::kBFloat16);
+}
+
+// dx and one dw a weight; dx empty or no dw where they are not asked for
+std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys,
+                                c10::optional<Tensor> codes,
+                                c10::optional<Tensor> scales,
+                                std::vector<Tensor> weights, bool need_dx,
+                                bool need_dw) {
+  std::vector<int64_t> counts;
+  const auto ws = weights_of(weights, &counts);
+  TORCH_CHECK(dys.size() == ws.size(), "linear8: one gradient an output");
+  const auto first = firsts(counts);
+  const int64_t K = ws[0].size(1), M = dys[0].size(0), N = first.back();
+  for (size_t i = 0; i < dys.size(); ++i) {
+    check_bf16(dys[i]);
+    dys[i] = matrix(dys[i], "dy");
+    TORCH_CHECK(dys[i].size(0) == M && dys[i].size(1) == counts[i],
+                "linear8: gradient ", i, " has the wrong shape");
+    same_device(ws[0], dys[i], "dy");
+  }
+  const CUDAGuard guard(ws[0].device());
+  const auto o = ws[0].options().requires_grad(false);
+  std::vector<Tensor> out(1);
+  if (M == 0) {
+    if (need_dx) out[0] = torch::empty({0, K}, dys[0].options());
+    if (need_dw)
+      for (int64_t n : counts) out.push_back(torch::zeros({n, K}, o));
+    return out;
+  }
+  Packed rows, cols;
+  if (need_dx) rows = new_packed(M, N, dys[0]);
+  if (need_dw) cols = new_packed(N, M, dys[0]);
+  if (need_dx || need_dw)
+    for (size_t i = 0; i < dys.size(); ++i)
+      run_tiles(need_dx && need_dw ? kBoth : need_dx ? kRows : kCols, dys[i],
+                need_dx ? &rows : nullptr, 0, first[i],
+                need_dw ? &cols : nullptr, first[i], 0);
+  if (need_dx) {
+    // W^T, [K][N]: each weight's columns side by side
+    Packed wt = new_packed(up(K, 128), N, ws[0]);
+    for (size_t i = 0; i < ws.size(); ++i)
+      run_tiles(kOneCols, ws[i], nullptr, 0, 0, &wt, 0, first[i]);
+    out[0] = product(rows, wt, M, {K}, torch::kBFloat16)[0];
+  }
+  if (need_dw) {
+    TORCH_CHECK(codes && scales, "linear8: nothing was kept of x");
+    const Packed x = packed(*codes, *scales, "linear8");
+    TORCH_CHECK(x.codes.size(0) == M && x.Cp() == up(K, 128),
+                "linear8: the gradient does not fit what was kept");
+    same_device(ws[0], x.codes, "x");
+    Packed xt = new_packed(x.Cp(), M, x.codes);
+    b8::TileArgs a{};
+    a.x = x.c();
+    a.xs = x.s();
+    a.ldx = x.Cp();
+    a.xsp = x.Rp();
+    a.R = M;
+    a.C = (int)x.Cp();
+    a.col_codes = xt.c();
+    a.col_scales = (uint8_t*)xt.s();
+    a.col_ld = xt.Cp();
+    a.col_sp = xt.Rp();
+    launch_b8_tiles(kFrom8, 2, 0, &a, stream_of(x.codes));
+    // dW [N][K], all weights' rows in one product; the weights' own rows of
+    // it are contiguous
+    const Tensor all = product(cols, xt, first[counts.size() - 1] +
+                                             counts.back(),
+                               {K}, ws[0].scalar_type())[0];
+    for (size_t i = 0; i < counts.size(); ++i)
+      out.push_back(counts.size() == 1
+                        ? all
+                        : torch::empty({0}, o).set_(
+                              all.storage(), first[i] * K, {counts[i], K},
+                              {K, 1}));
+  }
+  return out;
+}
+
+}  // namespace
+
+void bind_block8(pybind11::module_& m) {
+  m.def("pack8", &pack8, "matrix -> 8-bit block codes and scales");
+  m.def("unpack8", &unpack8, "8-bit block codes and scales -> matrix");
+  m.def("swiglu8_fwd", &swiglu8_fwd, "silu(g)*u, g and u kept in 8 bits");
+  m.def("swiglu8_bwd", &swiglu8_bwd, "gradients of swiglu8");
+  m.def("rms8_fwd", &rms8_fwd, "RMSNorm, x kept in 8 bits");
+  m.def("rms8_bwd", &rms8_bwd, "gradients of rms_norm8");
+  m.def("pack8_weights", &pack8_weights, "stacked weights in 8 bits");
+  m.def("linear8_fwd", &linear8_fwd, "x @ W^T of 8-bit operands");
+  m.def("linear8_packed", &linear8_packed, "x @ W^T on packed weights");
+  m.def("linear8_bwd", &linear8_bwd, "gradients of linear8");
+}

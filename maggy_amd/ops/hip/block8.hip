@@ -1,0 +1,599 @@
+// Packing to the 8-bit block format and the operators that keep their
+// inputs in it: silu(g) * u and RMSNorm.  All are bound by memory: one pass
+// over the data, 8 values a lane in one 16-byte load, no value read twice.
+#include <hip/hip_runtime.h>
+
+#include "block8.h"
+#include "block8_api.h"
+
+namespace b8 {
+
+constexpr int kThreads = 256;
+
+// one wave's unit of work: 512 columns (one scale dword) of one row
+struct Unit {
+  long long row;
+  int q;
+};
+__device__ __forceinline__ Unit unit_of(long long u, int Q) {
+  const long long row = u / Q;
+  return {row, (int)(u - row * Q)};
+}
+
+// ------------------------------------------------------------ pack, unpack
+template <class T, bool VEC>
+__global__ __launch_bounds__(kThreads) void pack_rows(
+    const typename T::raw* __restrict__ x, long long ldx, long long R, int C,
+    uint8_t* __restrict__ codes, int Cp, uint32_t* __restrict__ scales,
+    long long Rp, int Q) {
+  const int lane = threadIdx.x & 63;
+  const long long waves = (long long)gridDim.x * (kThreads / 64);
+  const long long units = R * Q;
+  for (long long u = (long long)blockIdx.x * (kThreads / 64) +
+                     (threadIdx.x >> 6);
+       u < units; u += waves) {
+    const Unit at = unit_of(u, Q);
+    const int c = at.q * 512 + lane * 8;
+    float v[8];
+    load8<T, VEC>(x + at.row * ldx, c, C, v);
+    pack512(v, lane, c, Cp, codes + at.row * Cp,
+            scales + at.q * Rp + at.row);
+  }
+}
+
+template <class T, bool VEC>
+__global__ __launch_bounds__(kThreads) void unpack_rows(
+    const uint8_t* __restrict__ codes, int Cp,
+    const uint32_t* __restrict__ scales, long long Rp, int Q, long long R,
+    int C, typename T::raw* __restrict__ out, float most) {
+  const int lane = threadIdx.x & 63;
+  const long long waves = (long long)gridDim.x * (kThreads / 64);
+  const long long units = R * Q;
+  for (long long u = (long long)blockIdx.x * (kThreads / 64) +
+                     (threadIdx.x >> 6);
+       u < units; u += waves) {
+    const Unit at = unit_of(u, Q);
+    const int c = at.q * 512 + lane * 8;
+    if (c >= Cp) continue;
+    const uint32_t E =
+        scales[at.q * Rp + at.row] >> (8 * (lane >> 4)) & 255u;
+    float v[8];
+    decode8(*(const u32x2*)(codes + at.row * Cp + c), scale_value(E), v);
+    // a value next to the type's largest may have been rounded up past it
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = v[i] > most ? most : v[i] < -most ? -most : v[i];
+    store8<T, VEC>(out + at.row * C, c, C, v);
+  }
+}
+
+// --------------------------------------------- 128 x 128 tiles, transposed
+// Reads a 128 x 128 tile once and writes its codes by rows (blocks along the
+// columns), by columns ([C][Rp] codes, blocks along the rows) or both.  With
+// ONE_SCALE the whole tile shares one scale, so that both orders stand for
+// the same values.  FROM8 reads a packed matrix instead of plain numbers.
+//
+// 512 threads: thread (cg, rg) = (t % 16, t / 16) holds 8 columns of 4
+// neighbouring rows, so that four rows of one column make one dword of the
+// transposed codes, and 16 lanes (one DPP row) hold a whole row of the tile.
+template <class T, bool VEC, bool FROM8, bool ONE_SCALE, bool ROWS, bool COLS>
+__global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
+  constexpr int kPitch = 33;  // dwords a transposed row of 128 codes
+  __shared__ uint32_t turned[COLS ? 128 * kPitch : 1];
+  __shared__ uint32_t tops[8][128];
+  const int t = threadIdx.x, cg = t & 15, rg = t >> 4, wave = t >> 6;
+  const long long tr = blockIdx.x / tiles_c;
+  const int tc = blockIdx.x % tiles_c;
+  const long long r0 = tr * 128 + rg * 4;
+  const int c0 = tc * 128 + cg * 8;
+
+  float v[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long r = r0 + i;
+    if (r < a.R) {
+      if constexpr (FROM8) {
+        const uint32_t E = ((const uint8_t*)a.xs)
+            [4 * ((tc >> 2) * a.xsp + r) + (tc & 3)];
+        decode8(*(const u32x2*)((const uint8_t*)a.x + r * a.ldx + c0),
+                scale_value(E), v[i]);
+      } else {
+        load8<T, VEC>((const typename T::raw*)a.x + r * a.ldx, c0, a.C,
+                      v[i]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+  }
+
+  uint32_t tile_E = 0;
+  if constexpr (ONE_SCALE) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, finite_bits(v[i][j]));
+    m = max16(m);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+    if ((t & 63) == 0) tops[wave][0] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, tops[w][0]);
+    tile_E = scale_of(m);
+  }
+
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long r = r0 + i;
+      const uint32_t E = ONE_SCALE ? tile_E : scale_of(block_top(v[i]));
+      const u32x2 code = encode8(v[i], scale_inverse(E));
+      if (r < a.R) {
+        *(u32x2*)(a.row_codes + (a.row_r0 + r) * a.row_ld + a.row_c0 + c0) =
+            code;
+        const long long b = a.row_c0 / 128 + tc;
+        if (cg == 0)
+          a.row_scales[4 * ((b >> 2) * a.row_sp + a.row_r0 + r) + (b & 3)] =
+              (uint8_t)E;
+      }
+    }
+  }
+
+  if constexpr (COLS) {
+    uint32_t E[8];
+    if constexpr (ONE_SCALE) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) E[j] = tile_E;
+    } else {
+      uint32_t m[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        m[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[j] = max(m[j], finite_bits(v[i][j]));
+        m[j] = max(m[j], (uint32_t)__shfl_xor((int)m[j], 16));
+        m[j] = max(m[j], (uint32_t)__shfl_xor((int)m[j], 32));
+      }
+      if ((t & 63) < 16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tops[wave][cg * 8 + j] = m[j];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) top = max(top, tops[w][cg * 8 + j]);
+        E[j] = scale_of(top);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float s = scale_inverse(E[j]);
+      turned[(cg * 8 + j) * kPitch + rg] =
+          encode4(v[0][j] * s, v[1][j] * s, v[2][j] * s, v[3][j] * s);
+    }
+    const long long b = a.col_c0 / 128 + tr;
+    if (rg == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        a.col_scales[4 * ((b >> 2) * a.col_sp + a.col_r0 + c0 + j) +
+                     (b & 3)] = (uint8_t)E[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = h * 64 + (t >> 3), k = (t & 7) * 4;
+      const uint32_t* s = turned + c * kPitch + k;
+      *(u32x4*)(a.col_codes + (a.col_r0 + tc * 128 + c) * a.col_ld +
+                b * 128 + k * 4) = u32x4{s[0], s[1], s[2], s[3]};
+    }
+  }
+}
+
+// ------------------------------------------------------------ silu(g) * u
+// h = g s u with s = 1 / (1 + exp(-g)); the backward pass uses the 8-bit g~
+// and u~:  dg = dh u~ s (1 + g~ (1 - s)),  du = dh g~ s.
+template <class T>
+__device__ __forceinline__ float sigmoid(float g) {
+  if constexpr (sizeof(typename T::raw) == 4)
+    return 1.f / (1.f + expf(-g));
+  else  // within 2^-20: far below a half step of the 16-bit types
+    return __builtin_amdgcn_rcpf(1.f + __expf(-g));
+}
+
+template <class T, bool VEC>
+__global__ __launch_bounds__(kThreads) void swiglu_fwd(
+    const typename T::raw* __restrict__ g, long long ldg,
+    const typename T::raw* __restrict__ u, long long ldu, long long R, int C,
+    typename T::raw* __restrict__ h, uint8_t* __restrict__ gc,
+    uint8_t* __restrict__ uc, int Cp, uint32_t* __restrict__ gs,
+    uint32_t* __restrict__ us, long long Rp, int Q) {
+  const int lane = threadIdx.x & 63;
+  const long long waves = (long long)gridDim.x * (kThreads / 64);
+  const long long units = R * Q;
+  for (long long n = (long long)blockIdx.x * (kThreads / 64) +
+                     (threadIdx.x >> 6);
+       n < units; n += waves) {
+    const Unit at = unit_of(n, Q);
+    const int c = at.q * 512 + lane * 8;
+    float a[8], b[8], o[8];
+    load8<T, VEC>(g + at.row * ldg, c, C, a);
+    load8<T, VEC>(u + at.row * ldu, c, C, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = a[i] * sigmoid<T>(a[i]) * b[i];
+    store8<T, VEC>(h + at.row * C, c, C, o);
+    if (gc) {
+      const long long s = at.q * Rp + at.row;
+      pack512(a, lane, c, Cp, gc + at.row * Cp, gs + s);
+      pack512(b, lane, c, Cp, uc + at.row * Cp, us + s);
+    }
+  }
+}
+
+template <class T, bool VEC>
+__global__ __launch_bounds__(kThreads) void swiglu_bwd(
+    const typename T::raw* __restrict__ dh, long long ldh,
+    const uint8_t* __restrict__ gc, const uint8_t* __restrict__ uc, int Cp,
+    const uint32_t* __restrict__ gs, const uint32_t* __restrict__ us,
+    long long Rp, int Q, long long R, int C,
+    typename T::raw* __restrict__ dg, typename T::raw* __restrict__ du) {
+  const int lane = threadIdx.x & 63;
+  const long long waves = (long long)gridDim.x * (kThreads / 64);
+  const long long units = R * Q;
+  for (long long n = (long long)blockIdx.x * (kThreads / 64) +
+                     (threadIdx.x >> 6);
+       n < units; n += waves) {
+    const Unit at = unit_of(n, Q);
+    const int c = at.q * 512 + lane * 8;
+    if (c >= Cp) continue;
+    const long long s = at.q * Rp + at.row;
+    const int shift = 8 * (lane >> 4);
+    float a[8], b[8], d[8];
+    load8<T, VEC>(dh + at.row * ldh, c, C, d);
+    decode8(*(const u32x2*)(gc + at.row * Cp + c),
+            scale_value(gs[s] >> shift & 255u), a);
+    decode8(*(const u32x2*)(uc + at.row * Cp + c),
+            scale_value(us[s] >> shift & 255u), b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float sg = sigmoid<T>(a[i]);
+      b[i] = d[i] * b[i] * sg * (1.f + a[i] * (1.f - sg));
+      a[i] = d[i] * a[i] * sg;
+    }
+    store8<T, VEC>(dg + at.row * C, c, C, b);
+    store8<T, VEC>(du + at.row * C, c, C, a);
+  }
+}
+
+// ---------------------------------------------------------------- RMSNorm
+// y = x inv w, inv = (mean x^2 + eps)^(-1/2), kept in fp32 from the exact x;
+// the backward pass uses n = x~ inv of the 8-bit x~:
+//   dx = inv (dy w - n mean(dy w n)),  dw = sum over rows of dy n.
+// A row belongs to WPR waves (1 up to 2048 columns, else 4), each lane
+// keeping its 8 * NI values in registers between the sum and the use.
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
+  return x;
+}
+
+template <int WPR>
+__device__ __forceinline__ float row_sum(float x, float (*part)[4],
+                                         int parity) {
+  x = wave_sum(x);
+  if constexpr (WPR == 1) return x;
+  // two buffers in turn: one barrier a row is enough
+  if ((threadIdx.x & 63) == 0) part[parity][threadIdx.x >> 6] = x;
+  __syncthreads();
+  return part[parity][0] + part[parity][1] + part[parity][2] +
+         part[parity][3];
+}
+
+template <class T, bool VEC, int WPR, int NI>
+__global__ __launch_bounds__(kThreads) void rms_fwd(
+    const typename T::raw* __restrict__ x, long long ldx,
+    const float* __restrict__ w, long long R, int C, float eps,
+    typename T::raw* __restrict__ y, float* __restrict__ inv_rms,
+    uint8_t* __restrict__ codes, int Cp, uint32_t* __restrict__ scales,
+    long long Rp) {
+  __shared__ float part[2][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int q0 = WPR == 1 ? 0 : wave;
+  const long long step = (long long)gridDim.x * (4 / WPR);
+  int parity = 0;
+  for (long long r = (long long)blockIdx.x * (4 / WPR) +
+                     (WPR == 1 ? wave : 0);
+       r < R; r += step, parity ^= 1) {
+    float v[NI][8], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      load8<T, VEC>(x + r * ldx, (q0 + i * WPR) * 512 + lane * 8, C, v[i]);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += v[i][j] * v[i][j];
+    sum = row_sum<WPR>(sum, part, parity);
+    const float inv = 1.f / sqrtf(sum / C + eps);
+    if (inv_rms && lane == 0 && q0 == 0) inv_rms[r] = inv;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int q = q0 + i * WPR, c = q * 512 + lane * 8;
+      if (q * 512 >= Cp) continue;  // the same for the whole wave
+      if (codes)
+        pack512(v[i], lane, c, Cp, codes + r * Cp, scales + q * Rp + r);
+      float g[8];
+      load8<Fp32, VEC>(w, c, C, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] *= v[i][j] * inv;
+      store8<T, VEC>(y + r * C, c, C, g);
+    }
+  }
+}
+
+// dw: every wave adds up its rows in registers and writes one row of
+// partials; the fold sums them in a fixed order, so results repeat.
+template <class T, bool VEC, int WPR, int NI>
+__global__ __launch_bounds__(kThreads) void rms_bwd(
+    const typename T::raw* __restrict__ dy, long long ldy,
+    const uint8_t* __restrict__ codes, int Cp,
+    const uint32_t* __restrict__ scales, long long Rp,
+    const float* __restrict__ w, const float* __restrict__ inv_rms,
+    long long R, int C, typename T::raw* __restrict__ dx,
+    float* __restrict__ partials) {
+  __shared__ float part[2][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int q0 = WPR == 1 ? 0 : wave;
+  const long long first =
+      (long long)blockIdx.x * (4 / WPR) + (WPR == 1 ? wave : 0);
+  const long long step = (long long)gridDim.x * (4 / WPR);
+  float g[NI][8], dw[NI][8];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    load8<Fp32, VEC>(w, (q0 + i * WPR) * 512 + lane * 8, C, g[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
+  }
+  int parity = 0;
+  for (long long r = first; r < R; r += step, parity ^= 1) {
+    float n[NI][8], d[NI][8], sum = 0.f;
+    const float inv = inv_rms[r];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int q = q0 + i * WPR, c = q * 512 + lane * 8;
+      load8<T, VEC>(dy + r * ldy, c, C, d[i]);
+      u32x2 code = {0, 0};
+      uint32_t E = 1;
+      if (c < Cp) {
+        code = *(const u32x2*)(codes + r * Cp + c);
+        E = scales[q * Rp + r] >> (8 * (lane >> 4)) & 255u;
+      }
+      decode8(code, scale_value(E), n[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        n[i][j] *= inv;
+        dw[i][j] += d[i][j] * n[i][j];
+        d[i][j] *= g[i][j];
+        sum += d[i][j] * n[i][j];
+      }
+    const float mean = row_sum<WPR>(sum, part, parity) / C;
+    if (dx) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[i][j] = inv * (d[i][j] - n[i][j] * mean);
+        store8<T, VEC>(dx + r * C, (q0 + i * WPR) * 512 + lane * 8, C, d[i]);
+      }
+    }
+  }
+  if (!partials) return;
+  const long long row = WPR == 1 ? first : blockIdx.x;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = (q0 + i * WPR) * 512 + lane * 8;
+    store8<Fp32, VEC>(partials + row * C, c, C, dw[i]);
+  }
+}
+
+// out[c] = sum over rows of partials[row][c]: 64 columns a workgroup, 16
+// waves each adding every 16th row, joined in order
+__global__ __launch_bounds__(1024) void fold_rows(
+    const float* __restrict__ partials, int P, int C,
+    float* __restrict__ out) {
+  __shared__ float part[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < C)
+    for (int p = wave; p < P; p += 16) s += partials[(long long)p * C + c];
+  part[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < C) {
+    s = part[0][lane];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += part[k][lane];
+    out[c] = s;
+  }
+}
+
+// ---------------------------------------------------------------- launches
+static inline int unit_blocks(long long R, int Q) {
+  const long long want = (R * Q + 3) / 4;
+  return (int)(want < 8192 ? want : 8192);
+}
+
+// dtype: 0 bf16, 1 fp16, 2 fp32
+#define B8_TYPED(dtype, vec, ...)                   \
+  do {                                              \
+    if (dtype == 0) {                               \
+      using T = Bf16;                               \
+      if (vec) { constexpr bool V = true; __VA_ARGS__; }   \
+      else { constexpr bool V = false; __VA_ARGS__; }      \
+    } else if (dtype == 1) {                        \
+      using T = Fp16;                               \
+      if (vec) { constexpr bool V = true; __VA_ARGS__; }   \
+      else { constexpr bool V = false; __VA_ARGS__; }      \
+    } else {                                        \
+      using T = Fp32;                               \
+      if (vec) { constexpr bool V = true; __VA_ARGS__; }   \
+      else { constexpr bool V = false; __VA_ARGS__; }      \
+    }                                               \
+  } while (0)
+
+template <class T, bool V, int WPR, int NI>
+static void rms_fwd_run(int blocks, hipStream_t st, const void* x,
+                        long long ldx, const float* w, long long R, int C,
+                        float eps, void* y, float* inv, uint8_t* codes,
+                        int Cp, uint32_t* scales, long long Rp) {
+  launch(rms_fwd<T, V, WPR, NI>, blocks, kThreads, st, 
+      (const typename T::raw*)x, ldx, w, R, C, eps, (typename T::raw*)y, inv,
+      codes, Cp, scales, Rp);
+}
+
+template <class T, bool V, int WPR, int NI>
+static void rms_bwd_run(int blocks, hipStream_t st, const void* dy,
+                        long long ldy, const uint8_t* codes, int Cp,
+                        const uint32_t* scales, long long Rp, const float* w,
+                        const float* inv, long long R, int C, void* dx,
+                        float* partials) {
+  launch(rms_bwd<T, V, WPR, NI>, blocks, kThreads, st, 
+      (const typename T::raw*)dy, ldy, codes, Cp, scales, Rp, w, inv, R, C,
+      (typename T::raw*)dx, partials);
+}
+
+// rows of up to 16384 columns: the caller refuses longer ones
+#define B8_ROWS(RUN, C, ...)                                   \
+  do {                                                         \
+    if (C <= 512) RUN<T, V, 1, 1>(__VA_ARGS__);                \
+    else if (C <= 1024) RUN<T, V, 1, 2>(__VA_ARGS__);          \
+    else if (C <= 2048) RUN<T, V, 1, 4>(__VA_ARGS__);          \
+    else if (C <= 4096) RUN<T, V, 4, 2>(__VA_ARGS__);          \
+    else if (C <= 8192) RUN<T, V, 4, 4>(__VA_ARGS__);          \
+    else RUN<T, V, 4, 8>(__VA_ARGS__);                         \
+  } while (0)
+
+}  // namespace b8
+
+using namespace b8;
+
+extern "C" void launch_b8_pack(int dtype, int vec, const void* x,
+                               long long ldx, long long R, int C,
+                               uint8_t* codes, int Cp, uint32_t* scales,
+                               long long Rp, hipStream_t st) {
+  const int Q = (Cp + 511) / 512;
+  B8_TYPED(dtype, vec,
+           (launch(pack_rows<T, V>, unit_blocks(R, Q), kThreads, st, 
+               (const T::raw*)x, ldx, R, C, codes, Cp, scales, Rp, Q)));
+}
+
+extern "C" void launch_b8_unpack(int dtype, int vec, const uint8_t* codes,
+                                 int Cp, const uint32_t* scales,
+                                 long long Rp, long long R, int C, void* out,
+                                 hipStream_t st) {
+  const int Q = (Cp + 511) / 512;
+  const float most =
+      dtype == 0 ? 0x1.fep127f : dtype == 1 ? 65504.f : 0x1.fffffep127f;
+  B8_TYPED(dtype, vec,
+           (launch(unpack_rows<T, V>, unit_blocks(R, Q), kThreads, st, 
+               codes, Cp, scales, Rp, Q, R, C, (T::raw*)out, most)));
+}
+
+// what: 0 rows and columns by their own blocks, 1 columns only,
+//       2 one scale a tile by rows, 3 one scale a tile by columns,
+//       4 columns of a packed matrix, 5 rows only
+extern "C" void launch_b8_tiles(int what, int dtype, int vec,
+                                const TileArgs* args, hipStream_t st) {
+  const TileArgs a = *args;
+  const int tc = (a.C + 127) / 128;
+  const long long blocks = (a.R + 127) / 128 * tc;
+  if (what == 4) {
+    launch(pack_tile<Fp32, false, true, false, false, true>, blocks, 512, st, a,
+             tc);
+    return;
+  }
+  B8_TYPED(dtype, vec, {
+    if (what == 0)
+      launch(pack_tile<T, V, false, false, true, true>, blocks, 512, st, a,
+             tc);
+    else if (what == 1)
+      launch(pack_tile<T, V, false, false, false, true>, blocks, 512, st, a,
+             tc);
+    else if (what == 2)
+      launch(pack_tile<T, V, false, true, true, false>, blocks, 512, st, a,
+             tc);
+    else if (what == 5)
+      launch(pack_tile<T, V, false, false, true, false>, blocks, 512, st, a,
+             tc);
+    else
+      launch(pack_tile<T, V, false, true, false, true>, blocks, 512, st, a,
+             tc);
+  });
+}
+
+extern "C" void launch_b8_swiglu_fwd(int dtype, int vec, const void* g,
+                                     long long ldg, const void* u,
+                                     long long ldu, long long R, int C,
+                                     void* h, uint8_t* gc, uint8_t* uc,
+                                     int Cp, uint32_t* gs, uint32_t* us,
+                                     long long Rp, hipStream_t st) {
+  const int Q = (Cp + 511) / 512;
+  B8_TYPED(dtype, vec,
+           (launch(swiglu_fwd<T, V>, unit_blocks(R, Q), kThreads, st, 
+               (const T::raw*)g, ldg, (const T::raw*)u, ldu, R, C,
+               (T::raw*)h, gc, uc, Cp, gs, us, Rp, Q)));
+}
+
+extern "C" void launch_b8_swiglu_bwd(int dtype, int vec, const void* dh,
+                                     long long ldh, const uint8_t* gc,
+                                     const uint8_t* uc, int Cp,
+                                     const uint32_t* gs, const uint32_t* us,
+                                     long long Rp, long long R, int C,
+                                     void* dg, void* du, hipStream_t st) {
+  const int Q = (Cp + 511) / 512;
+  B8_TYPED(dtype, vec,
+           (launch(swiglu_bwd<T, V>, unit_blocks(R, Q), kThreads, st, 
+               (const T::raw*)dh, ldh, gc, uc, Cp, gs, us, Rp, Q, R, C,
+               (T::raw*)dg, (T::raw*)du)));
+}
+
+extern "C" void launch_b8_rms_fwd(int dtype, int vec, const void* x,
+                                  long long ldx, const float* w, long long R,
+                                  int C, float eps, void* y, float* inv,
+                                  uint8_t* codes, int Cp, uint32_t* scales,
+                                  long long Rp, hipStream_t st) {
+  const long long groups = C <= 2048 ? (R + 3) / 4 : R;
+  const int blocks = (int)(groups < 8192 ? groups : 8192);
+  B8_TYPED(dtype, vec,
+           B8_ROWS(rms_fwd_run, C, blocks, st, x, ldx, w, R, C, eps, y, inv,
+                   codes, Cp, scales, Rp));
+}
+
+// the workgroups of the backward pass, and the rows of partials they write
+extern "C" int b8_rms_bwd_blocks(long long R, int C) {
+  const long long groups = C <= 2048 ? (R + 3) / 4 : R;
+  return (int)(groups < 512 ? groups : 512);
+}
+extern "C" int b8_rms_bwd_partials(long long R, int C) {
+  return b8_rms_bwd_blocks(R, C) * (C <= 2048 ? 4 : 1);
+}
+
+extern "C" void launch_b8_rms_bwd(int dtype, int vec, const void* dy,
+                                  long long ldy, const uint8_t* codes,
+                                  int Cp, const uint32_t* scales,
+                                  long long Rp, const float* w,
+                                  const float* inv, long long R, int C,
+                                  void* dx, float* partials, float* dw,
+                                  hipStream_t st) {
+  const int blocks = b8_rms_bwd_blocks(R, C);
+  B8_TYPED(dtype, vec,
+           B8_ROWS(rms_bwd_run, C, blocks, st, dy, ldy, codes, Cp, scales,
+                   Rp, w, inv, R, C, dx, partials));
+  if (partials)
+    launch(fold_rows, (C + 63) / 64, 1024, st, 
+        partials, b8_rms_bwd_partials(R, C), C, dw);
+}

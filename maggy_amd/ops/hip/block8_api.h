@@ -1,0 +1,87 @@
+// What the launchers of block8.hip and gemm8.hip take; plain C++, shared
+// with the bindings.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <cstdint>
+
+namespace b8 {
+
+// one matrix through the 128 x 128 tiles (block8.hip)
+struct TileArgs {
+  const void* x;        // plain numbers, or codes
+  const uint32_t* xs;   // codes: their scales
+  long long ldx;        // elements a row (codes: bytes)
+  long long xsp;        // codes: padded rows of xs
+  long long R;
+  int C;
+  uint8_t* row_codes;   // [..][row_ld]; row 0, column 0 of this matrix lie
+  uint8_t* row_scales;  // at (row_r0, row_c0), both multiples of 128
+  long long row_ld, row_sp, row_c0, row_r0;
+  uint8_t* col_codes;   // transposed: value (r, c) is at row col_r0 + c,
+  uint8_t* col_scales;  // column col_c0 + r
+  long long col_ld, col_sp, col_r0, col_c0;
+};
+
+// Y[m][n] = sum_k X[m][k] W[n][k], X and W packed along k (gemm8.hip).
+// The rows of W are up to four matrices, each padded to a multiple of 128
+// rows; each has a contiguous output of its own.
+constexpr int kMaxParts = 4;
+struct GemmArgs {
+  const uint8_t* x;
+  const uint32_t* xs;
+  long long ldx, xsp;
+  const uint8_t* w;
+  const uint32_t* ws;
+  long long ldw, wsp;
+  int M, N;  // rows of x and of w
+  int KT;    // K steps of 128
+  void* out[kMaxParts];
+  int first[kMaxParts];  // first row of w
+  int count[kMaxParts];  // columns of the output
+  int parts;
+  int f32;  // outputs are fp32, else bf16
+};
+
+#ifdef __HIPCC__
+// arguments are converted to what the kernel takes
+template <class... P, class... A>
+static inline void launch(void (*kernel)(P...), long long blocks, int threads,
+                          hipStream_t st, A... args) {
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st,
+                     static_cast<P>(args)...);
+}
+#endif
+
+}  // namespace b8
+
+extern "C" {
+void launch_b8_pack(int dtype, int vec, const void* x, long long ldx,
+                    long long R, int C, uint8_t* codes, int Cp,
+                    uint32_t* scales, long long Rp, hipStream_t st);
+void launch_b8_unpack(int dtype, int vec, const uint8_t* codes, int Cp,
+                      const uint32_t* scales, long long Rp, long long R,
+                      int C, void* out, hipStream_t st);
+void launch_b8_tiles(int what, int dtype, int vec, const b8::TileArgs* args,
+                     hipStream_t st);
+void launch_b8_swiglu_fwd(int dtype, int vec, const void* g, long long ldg,
+                          const void* u, long long ldu, long long R, int C,
+                          void* h, uint8_t* gc, uint8_t* uc, int Cp,
+                          uint32_t* gs, uint32_t* us, long long Rp,
+                          hipStream_t st);
+void launch_b8_swiglu_bwd(int dtype, int vec, const void* dh, long long ldh,
+                          const uint8_t* gc, const uint8_t* uc, int Cp,
+                          const uint32_t* gs, const uint32_t* us,
+                          long long Rp, long long R, int C, void* dg,
+                          void* du, hipStream_t st);
+void launch_b8_rms_fwd(int dtype, int vec, const void* x, long long ldx,
+                       const float* w, long long R, int C, float eps, void* y,
+                       float* inv, uint8_t* codes, int Cp, uint32_t* scales,
+                       long long Rp, hipStream_t st);
+int b8_rms_bwd_partials(long long R, int C);
+void launch_b8_rms_bwd(int dtype, int vec, const void* dy, long long ldy,
+                       const uint8_t* codes, int Cp, const uint32_t* scales,
+                       long long Rp, const float* w, const float* inv,
+                       long long R, int C, void* dx, float* partials,
+                       float* dw, hipStream_t st);
+void launch_b8_gemm(const b8::GemmArgs* args, hipStream_t st);
+}

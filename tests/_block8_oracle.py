@@ -1,0 +1,135 @@
+"""The 8-bit block operators from their definitions, in 64 bits and apart
+from the package's own code, with bounds on what a kernel may be off by.
+
+A bound counts, relative to the value rounded: half a step of the output type
+(``finfo.eps / 2``), fp32 arithmetic at 2^-24 an operation, the fast exp and
+reciprocal of the 16-bit types at 2^-20, and for products the matrix unit.
+That unit adds the products of 8 neighbouring k after cutting each below 2^-13
+of the largest one's power of two, so a group of 8 is off by less than
+7 * 2^-13 of its largest product; groups are added in fp32.
+"""
+import torch
+
+
+def power(t):
+    return ((t.long() + 1023) << 52).view(torch.float64)
+
+
+def e4m3(v):
+    """fp64 of magnitude at most 448 to the nearest e4m3, ties to even."""
+    _, e = torch.frexp(v)
+    step = power((e - 1).clamp(min=-6) - 3)
+    return torch.round(v / step) * step
+
+
+def block_value(b, dims):
+    """What a block stands for; infinities and NaN become NaN."""
+    b = b.double()
+    a = torch.where(b.isfinite(), b.abs(), torch.zeros_like(b))
+    top = a.amax(dims, keepdim=True)
+    t = torch.full_like(top, -126).long()
+    # count up to the smallest scale that fits
+    while True:
+        small = top > 448 * power(t)
+        if not small.any():
+            break
+        t = t + small.long()
+    s = power(t)
+    v = e4m3(torch.where(b.isfinite(), b, torch.zeros_like(b)) / s) * s
+    return torch.where(b.isfinite(), v, torch.full_like(b, float("nan")))
+
+
+def held(x, axis=1):
+    """[R, C] as held in blocks of 128 along ``axis``."""
+    if axis == 0:
+        return held(x.t(), 1).t()
+    if x.shape[0] == 0:
+        return x.double()
+    return torch.cat([block_value(x[:, i:i + 128], (1,))
+                      for i in range(0, x.shape[1], 128)], 1)
+
+
+def held_weight(w):
+    return torch.cat([torch.cat([
+        block_value(w[i:i + 128, j:j + 128], (0, 1))
+        for j in range(0, w.shape[1], 128)], 1)
+        for i in range(0, w.shape[0], 128)], 0)
+
+
+def product_bound(a, b):
+    """Off by at most this: a [M, K] b [N, K] as held, products over K."""
+    def tops(x):
+        pad = -x.shape[1] % 8
+        x = torch.nn.functional.pad(x.abs(), (0, pad))
+        return x.view(x.shape[0], -1, 8).amax(-1)
+
+    K = a.shape[1]
+    return tops(a) @ tops(b).t() * 7 * 2.0 ** -13 + \
+        a.abs() @ b.abs().t() * (K / 8 + 16) * 2.0 ** -24
+
+
+def assert_within(got, want, bound, what=""):
+    """|got - want| <= half a step of got's type + bound, NaN where want is
+    NaN."""
+    half = torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(got.dtype).smallest_normal * half
+    got, want = got.detach().double(), want.to(got.device)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert torch.equal(got.isnan(), want.isnan()), \
+        (what, int(got.isnan().sum()), int(want.isnan().sum()))
+    limit = (want.abs() + bound) * half + bound + tiny
+    over = ((got - want).abs() - limit).nan_to_num(-1.0)
+    worst = over.max().item() if over.numel() else -1.0
+    assert worst <= 0, (what, worst, int((over > 0).sum()), over.numel())
+
+
+def swiglu(g, u, dh):
+    """h, dg, du and their bounds (16-bit types; fp32 is inside them)."""
+    eps = 2.0 ** -20 if g.dtype != torch.float32 else 2.0 ** -21
+    g, u, d = g.double(), u.double(), dh.double()
+    h = g * torch.sigmoid(g) * u
+    gq, uq = held(g), held(u)
+    s = torch.sigmoid(gq)
+    dg = d * uq * s * (1 + gq * (1 - s))
+    # 1 + g (1 - s) cancels near its zero: the bound is on its terms
+    return [(h, h.abs() * 4 * eps),
+            (dg, (d * uq * s).abs() * (1 + (gq * (1 - s)).abs()) * 4 * eps +
+             (d * uq * s * s * gq).abs() * 4 * eps),
+            (d * gq * s, (d * gq * s).abs() * 4 * eps)]
+
+
+def rms(x, w, dy, eps):
+    x, w, d = x.double(), w.double(), dy.double()
+    R, C = x.shape
+    u = 2.0 ** -24
+    inv = 1 / torch.sqrt(x.pow(2).mean(1, keepdim=True) + eps)
+    y, n = x * inv * w, held(x) * inv
+    a = d * w
+    mean = (a * n).mean(1, keepdim=True)
+    size = (a * n).abs().mean(1, keepdim=True)
+    dx = inv * (a - n * mean)
+    # a row's sum: at most 64 values a lane, then 6 + 3 joins
+    rel = (64 + 9 + 8) * u
+    return [(y, y.abs() * rel),
+            (dx, inv * (a.abs() * 8 * u + n.abs() * (size + mean.abs()) *
+                        2 * rel)),
+            ((d * n).sum(0), (d * n).abs().sum(0) * (R + 40 + rel / u) * u)]
+
+
+def linear(x, ws, dys):
+    """ys, dx, dws and their bounds."""
+    xq = held(x)
+    xt = held(xq, 0).t()
+    wq = [held_weight(w) for w in ws]
+    ys = [(xq @ w.t(), product_bound(xq, w)) for w in wq]
+    dx, bound = 0, 0
+    for w, dy in zip(wq, dys):
+        d = held(dy)
+        dx = dx + d @ w
+        bound = bound + product_bound(d, w.t())
+    # the parts are added in fp32 with the rest
+    dws = []
+    for dy in dys:
+        d = held(dy, 0).t()
+        dws.append((d @ xt.t(), product_bound(d, xt)))
+    return ys, (dx, bound * 1.01), dws

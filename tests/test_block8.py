@@ -1,0 +1,263 @@
+"""The 8-bit block operators on the CPU: definitions, refusals, modules."""
+import copy
+
+import pytest
+import torch
+
+from maggy_amd import ops
+from maggy_amd.exceptions import HipExtensionMissingError  # noqa: F401
+from tests import _block8_oracle as oracle
+
+
+def _normal(*shape, seed=0, std=1.0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).mul(std).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16,
+                                   torch.float32])
+@pytest.mark.parametrize("R,C", [(1, 1), (3, 127), (5, 129), (2, 700),
+                                 (300, 64)])
+def test_pack_is_the_definition(R, C, dtype):
+    x = _normal(R, C, dtype=dtype) * \
+        torch.exp2(_normal(R, 1, seed=1) * 4).to(dtype)
+    got = ops.unpack8(ops.pack8(x))
+    assert torch.equal(got.double(), oracle.held(x).to(dtype).double())
+
+
+def test_pack_extremes():
+    x = torch.zeros(4, 200)
+    x[0, 1], x[0, 2] = torch.finfo().max, 1.0
+    x[1, 3], x[1, 4] = float("inf"), 2.0
+    x[2, 5], x[2, 6] = float("nan"), -3.0
+    got = ops.unpack8(ops.pack8(x))
+    assert got[0, 1] == torch.finfo().max and got[0, 2] == 0
+    assert got[1, 3].isnan() and got[1, 4] == 2
+    assert got[2, 5].isnan() and got[2, 6] == -3
+    assert torch.equal(got[3], x[3])
+
+
+def test_held_bytes():
+    h = ops.pack8(_normal(256, 512, dtype=torch.bfloat16))
+    assert h.nbytes() == 256 * 512 + 256 * 4
+    assert "Block8" in repr(h)
+
+
+def test_swiglu8():
+    g, u = (_normal(9, 300, seed=s).requires_grad_(True) for s in (1, 2))
+    dh = _normal(9, 300, seed=3)
+    h = ops.swiglu8(g, u)
+    h.backward(dh)
+    for got, (want, bound) in zip((h, g.grad, u.grad),
+                                  oracle.swiglu(g.detach(), u.detach(), dh)):
+        oracle.assert_within(got, want, bound)
+
+
+def test_rms_norm8():
+    x = _normal(9, 300, seed=1).requires_grad_(True)
+    w = _normal(300, seed=2).requires_grad_(True)
+    dy = _normal(9, 300, seed=3)
+    y = ops.rms_norm8(x, w)
+    y.backward(dy)
+    for got, (want, bound) in zip(
+            (y, x.grad, w.grad),
+            oracle.rms(x.detach(), w.detach(), dy, 1e-5)):
+        oracle.assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("M,K,Ns", [(1, 64, (32,)), (17, 130, (77, 129)),
+                                    (5, 300, (64, 1, 200, 3))])
+def test_linear8(M, K, Ns):
+    x = _normal(M, K, seed=1).requires_grad_(True)
+    ws = [_normal(n, K, seed=2 + i, std=0.1).requires_grad_(True)
+          for i, n in enumerate(Ns)]
+    dys = [_normal(M, n, seed=8 + i) for i, n in enumerate(Ns)]
+    ys = ops.linear8(x, *ws)
+    ys = ys if isinstance(ys, tuple) else (ys,)
+    grads = torch.autograd.grad(ys, [x, *ws], dys)
+    want_y, want_dx, want_dw = oracle.linear(
+        x.detach(), [w.detach() for w in ws], dys)
+    for got, (want, bound) in zip(
+            (*ys, *grads), (*want_y, want_dx, *want_dw)):
+        oracle.assert_within(got, want, bound)
+    with torch.no_grad():
+        again = ops.linear8(x, ops.pack_weight8(*ws))
+        again = again if isinstance(again, tuple) else (again,)
+        for a, b in zip(again, ys):
+            torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-6)
+
+
+def test_a_gradient_against_differences():
+    """Where everything is exact in 8 bits the gradient is the slope."""
+    # small whole numbers times a power of two fit e4m3 under any scale
+    x = torch.randint(-7, 8, (6, 40), generator=torch.Generator()
+                      .manual_seed(0)).float().requires_grad_(True)
+    w = torch.randint(-7, 8, (5, 40), generator=torch.Generator()
+                      .manual_seed(1)).float().requires_grad_(True)
+    d = torch.randint(-7, 8, (6, 5), generator=torch.Generator()
+                      .manual_seed(2)).float()
+    ops.linear8(x, w).backward(d)
+
+    def loss(x, w):
+        return (ops.linear8(x, w) * d).sum()
+
+    with torch.no_grad():
+        for t, grad, other in ((x, x.grad, lambda t: loss(t, w)),
+                               (w, w.grad, lambda t: loss(x, t))):
+            for i, j in ((0, 0), (3, 17), (4, 39)):
+                hi, lo = t.detach().clone(), t.detach().clone()
+                hi[i, j] += 1
+                lo[i, j] -= 1
+                slope = (other(hi) - other(lo)) / 2
+                assert slope == grad[i, j]
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    x, w = _normal(4, 32), _normal(8, 32)
+    with pytest.raises(TypeError):
+        ops.pack8(x.double())
+    with pytest.raises(TypeError):
+        ops.pack8([1.0])
+    with pytest.raises(ValueError):
+        ops.pack8(torch.tensor(1.0))
+    with pytest.raises(ValueError):
+        ops.pack8(torch.zeros(3, 0))
+    with pytest.raises(TypeError):
+        ops.unpack8(x)
+    with pytest.raises(TypeError):
+        ops.unpack8(ops.pack8(x), torch.int32)
+    with pytest.raises(ValueError):
+        ops.swiglu8(x, x[:2])
+    with pytest.raises(ValueError):
+        ops.swiglu8(x, x.bfloat16())
+    with pytest.raises(ValueError):
+        ops.rms_norm8(x, torch.ones(31))
+    with pytest.raises(ValueError):
+        ops.linear8(x)
+    with pytest.raises(ValueError):
+        ops.linear8(x, *[w] * 5)
+    with pytest.raises(ValueError):
+        ops.linear8(x, _normal(8, 31))
+    with pytest.raises(ValueError):
+        ops.linear8(x, w, w[:, :16])
+    with pytest.raises(ValueError):
+        ops.linear8(x, w[:0])
+    with pytest.raises(ValueError):
+        ops.linear8(x, w[0])
+    with pytest.raises(TypeError):
+        ops.linear8(x, w.half())
+    with pytest.raises(TypeError):
+        ops.linear8(x, w.int())
+
+
+def test_packed_weights_refuse_gradients_and_company():
+    x, w = _normal(4, 32).requires_grad_(True), _normal(8, 32)
+    packed = ops.pack_weight8(w)
+    with pytest.raises(RuntimeError):
+        ops.linear8(x, packed)
+    with pytest.raises(TypeError):
+        ops.linear8(x, packed, w)
+    with pytest.raises(ValueError):
+        ops.linear8(_normal(4, 31), packed)
+    assert ops.linear8(x.detach(), packed).shape == (4, 8)
+
+
+def test_second_derivatives_are_refused():
+    x = _normal(4, 32).requires_grad_(True)
+    w = _normal(8, 32).requires_grad_(True)
+    y = ops.linear8(x, w)
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+# ------------------------------------------------------------------- modules
+def test_modules_share_state_with_the_16_bit_ones():
+    from maggy_amd.ops.linear import MaggyFeedForward
+
+    torch.manual_seed(0)
+    a, b = MaggyFeedForward(64, 96), ops.MaggyFeedForward8(64, 96)
+    b.load_state_dict(a.state_dict())
+    x = _normal(7, 64).requires_grad_(True)
+    y = b(x)
+    # 8 bits: 1/16 a value, far less over sums of 64
+    assert (y - a(x)).norm() < 0.1 * a(x).norm()
+    y.sum().backward()
+    assert x.grad is not None
+    assert all(p.grad is not None for p in b.parameters())
+    c = copy.deepcopy(b)
+    assert c.up8.linears[0] is c.w1 and c.up8.linears[0] is not b.w1
+
+
+def test_module_packs_and_drops():
+    lin = ops.MaggyLinear8(40, 30)
+    x = _normal(3, 40)
+    with torch.no_grad():
+        before = lin(x)
+        ops.pack8_model(lin)
+        assert torch.equal(lin(x), before)
+        lin.weight.mul_(2)
+        assert torch.equal(lin(x), before)  # packed weights stay
+        ops.drop8_model(lin)
+        assert torch.equal(lin(x), before * 2)
+    with pytest.raises(ValueError):
+        from maggy_amd.ops.block8 import Linear8Group
+
+        Linear8Group(torch.nn.Linear(3, 3))
+
+
+def test_norm_module():
+    n = ops.MaggyRMSNorm8(48)
+    x = _normal(5, 48).requires_grad_(True)
+    n(x).sum().backward()
+    assert n.weight.grad.shape == (48,) and x.grad.shape == x.shape
+
+
+# --------------------------------------------------------------------- Llama
+def _llama(eight_bit, seed=0):
+    from maggy_amd.models import LlamaConfig, LlamaModel
+
+    torch.manual_seed(seed)
+    cfg = LlamaConfig.tiny(vocab_size=97)
+    cfg.eight_bit = eight_bit
+    return LlamaModel(cfg)
+
+
+def test_llama_in_8_bits_is_near_the_16_bit_one():
+    a, b = _llama(False), _llama(True)
+    assert a.state_dict().keys() == b.state_dict().keys()
+    b.load_state_dict(a.state_dict())
+    tokens = torch.randint(0, 97, (2, 16))
+    with torch.no_grad():
+        want, got = a(tokens), b(tokens)
+    assert (got - want).norm() < 0.1 * want.norm()
+    la, lb = a(tokens, tokens), b(tokens, tokens)
+    la.backward()
+    lb.backward()
+    for (name, p), q in zip(a.named_parameters(), b.parameters()):
+        # 4 significant bits an operand: the gradients point the same way
+        cos = torch.nn.functional.cosine_similarity(
+            p.grad.flatten(), q.grad.flatten(), dim=0)
+        assert cos > 0.95, (name, cos)
+
+
+def test_llama_in_8_bits_decodes():
+    from maggy_amd.ops.block8 import groups8
+
+    m = _llama(True).eval()
+    prompt = torch.randint(0, 97, (2, 5))
+    out = m.generate(prompt, max_new_tokens=6)
+    assert all(g.packed is None for g in groups8(m))  # dropped again
+    assert len(groups8(m)) == 8
+    seq = prompt
+    with torch.no_grad():
+        for _ in range(6):
+            nxt = m(seq)[:, -1, :].argmax(-1, keepdim=True)
+            seq = torch.cat([seq, nxt], 1)
+    assert torch.equal(out, seq)
+    ops.pack8_model(m)
+    assert torch.equal(m.generate(prompt, max_new_tokens=6), out)
+    assert all(g.packed is not None for g in groups8(m))  # the caller's
+    got = m.generate_captured(prompt, max_new_tokens=6, use_graph=False)
+    assert torch.equal(got, out)
