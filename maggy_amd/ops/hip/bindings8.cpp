@@ -327,34 +327,45 @@ std::vector<Tensor> weights_of(const std::vector<Tensor>& weights,
   return ws;
 }
 
-std::vector<Tensor> product(const Packed& x, const Packed& w, int64_t M,
-                            const std::vector<int64_t>& counts,
-                            torch::ScalarType dtype) {
+// the product of packed w with x, packed (M rows) or, for a few rows, plain
+// bf16 that the kernel packs on the way
+b8::GemmArgs gemm_args(const Packed& w, int64_t M,
+                       const std::vector<int64_t>& counts,
+                       torch::ScalarType dtype, std::vector<Tensor>* out) {
   const auto first = firsts(counts);
-  TORCH_CHECK(x.Cp() == w.Cp(), "linear8: columns do not match");
+  TORCH_CHECK(M < (int64_t)1 << 30 && first.back() < (int64_t)1 << 30,
+              "linear8: too many rows");
+  TORCH_CHECK(w.Cp() <= (int64_t)1 << 22, "linear8: too many columns");
   b8::GemmArgs a{};
-  a.x = x.c();
-  a.xs = x.s();
-  a.ldx = x.Cp();
-  a.xsp = x.Rp();
   a.w = w.c();
   a.ws = w.s();
   a.ldw = w.Cp();
   a.wsp = w.Rp();
-  TORCH_CHECK(M < (int64_t)1 << 30 && first.back() < (int64_t)1 << 30,
-              "linear8: too many rows");
   a.M = (int)M;
   a.N = (int)std::min(first.back(), w.codes.size(0));
-  a.KT = (int)(x.Cp() / 128);
+  a.KT = (int)(w.Cp() / 128);
   a.parts = (int)counts.size();
   a.f32 = dtype == torch::kFloat32;
-  std::vector<Tensor> out;
   for (size_t i = 0; i < counts.size(); ++i) {
-    out.push_back(torch::empty({M, counts[i]}, x.codes.options().dtype(dtype)));
-    a.out[i] = out[i].data_ptr();
+    out->push_back(
+        torch::empty({M, counts[i]}, w.codes.options().dtype(dtype)));
+    a.out[i] = (*out)[i].data_ptr();
     a.first[i] = (int)first[i];
     a.count[i] = (int)counts[i];
   }
+  return a;
+}
+
+std::vector<Tensor> product(const Packed& x, const Packed& w, int64_t M,
+                            const std::vector<int64_t>& counts,
+                            torch::ScalarType dtype) {
+  TORCH_CHECK(x.Cp() == w.Cp(), "linear8: columns do not match");
+  std::vector<Tensor> out;
+  b8::GemmArgs a = gemm_args(w, M, counts, dtype, &out);
+  a.x = x.c();
+  a.xs = x.s();
+  a.ldx = x.Cp();
+  a.xsp = x.Rp();
   if (M) launch_b8_gemm(&a, stream_of(x.codes));
   return out;
 }
@@ -404,7 +415,14 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
               " columns, the weights ", K);
   same_device(x, wcodes, "weight");
   const CUDAGuard guard(x.device());
-  return product(pack_rows(x), w, x.size(0), counts, torch::kBFloat16);
+  const int64_t M = x.size(0);
+  if (M >= 1 && M <= 16 && vec8(x)) {
+    std::vector<Tensor> out;
+    const b8::GemmArgs a = gemm_args(w, M, counts, torch::kBFloat16, &out);
+    launch_b8_gemm_bf16(&a, x.data_ptr(), ld(x), (int)K, stream_of(x));
+    return out;
+  }
+  return product(pack_rows(x), w, M, counts, torch::kBFloat16);
 }
 
 // dx and one dw a weight; dx empty or no dw where they are not asked for

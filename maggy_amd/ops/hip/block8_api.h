@@ -84,4 +84,6 @@ void launch_b8_rms_bwd(int dtype, int vec, const void* dy, long long ldy,
                        long long R, int C, void* dx, float* partials,
                        float* dw, hipStream_t st);
 void launch_b8_gemm(const b8::GemmArgs* args, hipStream_t st);
+void launch_b8_gemm_bf16(const b8::GemmArgs* args, const void* x,
+                         long long ldx, int K, hipStream_t st);
 }
