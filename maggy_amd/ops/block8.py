@@ -94,7 +94,7 @@ def _pack_cpu(x):
     R = x.shape[0]
     b = _blocks(x)
     t = _scale_exponents(_tops(b, -1))
-    codes = _encode(b, t).view(torch.uint8).flatten(1)
+    codes = _encode(b, t).view(torch.uint8).transpose(0, 1).contiguous()
     E = (t + 127).to(torch.uint8).flatten(1)
     E = nn.functional.pad(E, (0, -E.shape[1] % 4), value=1)
     scales = torch.ones(E.shape[1] // 4, _up(R, 256), 4, dtype=torch.uint8)
@@ -103,9 +103,9 @@ def _pack_cpu(x):
 
 
 def _unpack_cpu(codes, scales, C, dtype):
-    R, Cp = codes.shape
-    E = scales[:, :R].transpose(0, 1).flatten(1)[:, :Cp // BLOCK]
-    v = codes.view(torch.float8_e4m3fn).float().unflatten(1, (-1, BLOCK))
+    n, R = codes.shape[:2]
+    E = scales[:, :R].transpose(0, 1).flatten(1)[:, :n]
+    v = codes.transpose(0, 1).view(torch.float8_e4m3fn).float()
     v = v * _power(E.int()[..., None] - 127)
     most = torch.finfo(dtype).max
     # a value next to the type's largest may have been rounded up past it
@@ -117,8 +117,8 @@ def _unpack_cpu(codes, scales, C, dtype):
 class Block8:
     """A tensor held in 8 bits a value (``pack8``), read by ``unpack8``.
 
-    ``codes`` [rows, C up to 128] and ``scales`` are uint8 tensors; leading
-    axes are flattened into rows.  ``shape`` and ``dtype`` are those of the
+    ``codes`` [C / 128 rounded up, rows, 128] and ``scales`` are uint8
+    tensors; leading axes are flattened into rows.  ``shape`` and ``dtype`` are those of the
     tensor that was packed."""
 
     __slots__ = ("codes", "scales", "shape", "dtype")

@@ -59,29 +59,30 @@ void same_device(const Tensor& a, const Tensor& b, const char* name) {
 }
 
 struct Packed {
-  Tensor codes, scales;  // [rows][Cp], [Q][Rp][4]
+  Tensor codes, scales;  // [Cp / 128][rows][128], [Q][Rp][4]
   uint8_t* c() const { return codes.data_ptr<uint8_t>(); }
   uint32_t* s() const { return (uint32_t*)scales.data_ptr<uint8_t>(); }
-  int64_t Cp() const { return codes.size(1); }
+  int64_t rows() const { return codes.size(1); }
+  int64_t Cp() const { return codes.size(0) * 128; }
   int64_t Rp() const { return scales.size(1); }
 };
 
 Packed new_packed(int64_t rows, int64_t C, const Tensor& like) {
   const auto o = like.options().dtype(torch::kUInt8).requires_grad(false);
   const int64_t Cp = up(C, 128);
-  return {torch::empty({rows, Cp}, o),
+  return {torch::empty({Cp / 128, rows, 128}, o),
           torch::empty({(Cp + 511) / 512, up(rows, 256), 4}, o)};
 }
 
 Packed packed(const Tensor& codes, const Tensor& scales, const char* name) {
   TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == torch::kUInt8 &&
-                  codes.dim() == 2 && codes.is_contiguous() &&
-                  codes.size(1) % 128 == 0,
-              name, ": codes must be contiguous uint8 [rows][128 n]");
+                  codes.dim() == 3 && codes.is_contiguous() &&
+                  codes.size(0) >= 1 && codes.size(2) == 128,
+              name, ": codes must be contiguous uint8 [n][rows][128]");
   TORCH_CHECK(scales.scalar_type() == torch::kUInt8 && scales.dim() == 3 &&
                   scales.is_contiguous() &&
-                  scales.size(0) == (codes.size(1) + 511) / 512 &&
-                  scales.size(1) == up(codes.size(0), 256) &&
+                  scales.size(0) == (codes.size(0) + 3) / 4 &&
+                  scales.size(1) == up(codes.size(1), 256) &&
                   scales.size(2) == 4,
               name, ": scales do not fit the codes");
   same_device(codes, scales, name);
@@ -110,7 +111,7 @@ Tensor unpack8(Tensor codes, Tensor scales, int64_t C,
   TORCH_CHECK(C >= 1 && up(C, 128) == p.Cp(), "unpack8: ", C,
               " columns do not fit the codes");
   const CUDAGuard guard(codes.device());
-  const int64_t R = codes.size(0);
+  const int64_t R = p.rows();
   Tensor out = torch::empty({R, C}, codes.options().dtype(dtype));
   if (R)
     launch_b8_unpack(type_of(out, "out"), C % 8 == 0, p.c(), (int)p.Cp(),
@@ -147,8 +148,8 @@ std::vector<Tensor> swiglu8_bwd(Tensor dh, Tensor gc, Tensor gs, Tensor uc,
   dh = matrix(dh, "dh");
   const Packed g = packed(gc, gs, "swiglu8"), u = packed(uc, us, "swiglu8");
   const int64_t R = dh.size(0), C = dh.size(1);
-  TORCH_CHECK(gc.sizes() == uc.sizes() && gc.size(0) == R &&
-                  gc.size(1) == up(C, 128),
+  TORCH_CHECK(gc.sizes() == uc.sizes() && g.rows() == R &&
+                  g.Cp() == up(C, 128),
               "swiglu8: the gradient does not fit what was kept");
   same_device(dh, gc, "g");
   same_device(dh, uc, "u");
@@ -208,8 +209,7 @@ std::vector<c10::optional<Tensor>> rms8_bwd(Tensor dy, Tensor codes,
   dy = matrix(dy, "dy");
   const Packed p = packed(codes, scales, "rms_norm8");
   const int64_t R = dy.size(0), C = dy.size(1);
-  TORCH_CHECK(C <= kRmsMost && codes.size(0) == R &&
-                  codes.size(1) == up(C, 128),
+  TORCH_CHECK(C <= kRmsMost && p.rows() == R && p.Cp() == up(C, 128),
               "rms_norm8: the gradient does not fit what was kept");
   TORCH_CHECK(inv.numel() == R && inv.is_contiguous() &&
                   inv.scalar_type() == torch::kFloat32,
@@ -283,7 +283,7 @@ void run_tiles(Tiles what, const Tensor& t, Packed* rows, int64_t row_r0,
   if (rows) {
     a.row_codes = rows->c();
     a.row_scales = (uint8_t*)rows->s();
-    a.row_ld = rows->Cp();
+    a.row_n = rows->rows();
     a.row_sp = rows->Rp();
     a.row_r0 = row_r0;
     a.row_c0 = row_c0;
@@ -291,7 +291,7 @@ void run_tiles(Tiles what, const Tensor& t, Packed* rows, int64_t row_r0,
   if (cols) {
     a.col_codes = cols->c();
     a.col_scales = (uint8_t*)cols->s();
-    a.col_ld = cols->Cp();
+    a.col_n = cols->rows();
     a.col_sp = cols->Rp();
     a.col_r0 = col_r0;
     a.col_c0 = col_c0;
@@ -335,14 +335,17 @@ b8::GemmArgs gemm_args(const Packed& w, int64_t M,
   const auto first = firsts(counts);
   TORCH_CHECK(M < (int64_t)1 << 30 && first.back() < (int64_t)1 << 30,
               "linear8: too many rows");
-  TORCH_CHECK(w.Cp() <= (int64_t)1 << 22, "linear8: too many columns");
+  // the kernel reaches a matrix's scales by 32-bit offsets
+  TORCH_CHECK(w.scales.numel() < (int64_t)1 << 31 &&
+                  w.scales.size(0) * up(M, 256) * 4 < (int64_t)1 << 31,
+              "linear8: matrix is too large");
   b8::GemmArgs a{};
   a.w = w.c();
   a.ws = w.s();
-  a.ldw = w.Cp();
+  a.wn = w.rows();
   a.wsp = w.Rp();
   a.M = (int)M;
-  a.N = (int)std::min(first.back(), w.codes.size(0));
+  a.N = (int)std::min(first.back(), w.rows());
   a.KT = (int)(w.Cp() / 128);
   a.parts = (int)counts.size();
   a.f32 = dtype == torch::kFloat32;
@@ -364,9 +367,15 @@ std::vector<Tensor> product(const Packed& x, const Packed& w, int64_t M,
   b8::GemmArgs a = gemm_args(w, M, counts, dtype, &out);
   a.x = x.c();
   a.xs = x.s();
-  a.ldx = x.Cp();
+  a.xn = x.rows();
   a.xsp = x.Rp();
-  if (M) launch_b8_gemm(&a, stream_of(x.codes));
+  if (M) {
+    const long long bytes = b8_gemm_workspace(&a);
+    Tensor space;
+    if (bytes) space = torch::empty({bytes}, x.codes.options());
+    launch_b8_gemm(&a, bytes ? (float*)space.data_ptr() : nullptr,
+                   stream_of(x.codes));
+  }
   return out;
 }
 
@@ -408,7 +417,7 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
   x = matrix(x, "x");
   check_counts(counts);
   const Packed w = packed(wcodes, wscales, "linear8");
-  TORCH_CHECK(firsts(counts).back() == w.codes.size(0) &&
+  TORCH_CHECK(firsts(counts).back() == w.rows() &&
                   up(K, 128) == w.Cp(),
               "linear8: the packed weights do not have these shapes");
   TORCH_CHECK(x.size(1) == K, "linear8: x has ", x.size(1),
@@ -470,20 +479,20 @@ std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys,
   if (need_dw) {
     TORCH_CHECK(codes && scales, "linear8: nothing was kept of x");
     const Packed x = packed(*codes, *scales, "linear8");
-    TORCH_CHECK(x.codes.size(0) == M && x.Cp() == up(K, 128),
+    TORCH_CHECK(x.rows() == M && x.Cp() == up(K, 128),
                 "linear8: the gradient does not fit what was kept");
     same_device(ws[0], x.codes, "x");
     Packed xt = new_packed(x.Cp(), M, x.codes);
     b8::TileArgs a{};
     a.x = x.c();
     a.xs = x.s();
-    a.ldx = x.Cp();
+    a.ldx = x.rows();
     a.xsp = x.Rp();
     a.R = M;
     a.C = (int)x.Cp();
     a.col_codes = xt.c();
     a.col_scales = (uint8_t*)xt.s();
-    a.col_ld = xt.Cp();
+    a.col_n = xt.rows();
     a.col_sp = xt.Rp();
     launch_b8_tiles(kFrom8, 2, 0, &a, stream_of(x.codes));
     // dW [N][K], all weights' rows in one product; the weights' own rows of

@@ -1,8 +1,12 @@
 // The 8-bit block format and the device helpers that its kernels share.
 //
 // A Block8 of R rows and C columns holds
-//   codes   [R][Cp] bytes, Cp = C up to a multiple of 128: OCP e4m3, the
-//           padding columns zero
+//   codes   [Cp / 128][R][128] bytes, Cp = C up to a multiple of 128: OCP
+//           e4m3, the padding columns zero.  A panel of 128 columns is one
+//           piece of memory, because products walk along the columns: the
+//           128 bytes that they want of each of 256 rows are 32 KB in a row
+//           here, and 256 far apart lines in a row-major matrix, which cost
+//           them up to a fifth of their rate
 //   scales  [ceil(Cp / 512)][Rp][4] bytes, Rp = R up to a multiple of 256:
 //           byte j of dword (q, r) is the e8m0 scale E of row r's block
 //           4q + j, worth 2^(E - 127)
@@ -172,13 +176,24 @@ __device__ __forceinline__ uint32_t block_top(const float (&v)[8]) {
   return max16(m);
 }
 
+// where the codes of columns c .. of a row are
+__device__ __forceinline__ uint8_t* code_at(uint8_t* codes, long long R,
+                                            long long row, int c) {
+  return codes + ((c >> 7) * R + row) * 128 + (c & 127);
+}
+__device__ __forceinline__ const uint8_t* code_at(const uint8_t* codes,
+                                                  long long R, long long row,
+                                                  int c) {
+  return codes + ((c >> 7) * R + row) * 128 + (c & 127);
+}
+
 // packs a wave's 512 columns of one row and stores them
 __device__ __forceinline__ void pack512(const float (&v)[8], int lane, int c,
-                                        int Cp, uint8_t* code_row,
-                                        uint32_t* scale_at) {
+                                        int Cp, uint8_t* codes, long long R,
+                                        long long row, uint32_t* scale_at) {
   const uint32_t E = scale_of(block_top(v));
   const u32x2 code = encode8(v, scale_inverse(E));
-  if (c < Cp) *(u32x2*)(code_row + c) = code;
+  if (c < Cp) *(u32x2*)code_at(codes, R, row, c) = code;
   const uint32_t four = gather_scales(E);
   if (lane == 0) *scale_at = four;
 }

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kThreads) void pack_rows(
     const int c = at.q * 512 + lane * 8;
     float v[8];
     load8<T, VEC>(x + at.row * ldx, c, C, v);
-    pack512(v, lane, c, Cp, codes + at.row * Cp,
+    pack512(v, lane, c, Cp, codes, R, at.row,
             scales + at.q * Rp + at.row);
   }
 }
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kThreads) void unpack_rows(
     const uint32_t E =
         scales[at.q * Rp + at.row] >> (8 * (lane >> 4)) & 255u;
     float v[8];
-    decode8(*(const u32x2*)(codes + at.row * Cp + c), scale_value(E), v);
+    decode8(*(const u32x2*)code_at(codes, R, at.row, c), scale_value(E), v);
     // a value next to the type's largest may have been rounded up past it
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
       if constexpr (FROM8) {
         const uint32_t E = ((const uint8_t*)a.xs)
             [4 * ((tc >> 2) * a.xsp + r) + (tc & 3)];
-        decode8(*(const u32x2*)((const uint8_t*)a.x + r * a.ldx + c0),
+        decode8(*(const u32x2*)code_at((const uint8_t*)a.x, a.ldx, r, c0),
                 scale_value(E), v[i]);
       } else {
         load8<T, VEC>((const typename T::raw*)a.x + r * a.ldx, c0, a.C,
@@ -131,9 +131,9 @@ __global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
       const uint32_t E = ONE_SCALE ? tile_E : scale_of(block_top(v[i]));
       const u32x2 code = encode8(v[i], scale_inverse(E));
       if (r < a.R) {
-        *(u32x2*)(a.row_codes + (a.row_r0 + r) * a.row_ld + a.row_c0 + c0) =
-            code;
         const long long b = a.row_c0 / 128 + tc;
+        *(u32x2*)(a.row_codes + (b * a.row_n + a.row_r0 + r) * 128 + cg * 8) =
+            code;
         if (cg == 0)
           a.row_scales[4 * ((b >> 2) * a.row_sp + a.row_r0 + r) + (b & 3)] =
               (uint8_t)E;
@@ -187,8 +187,9 @@ __global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
     for (int h = 0; h < 2; ++h) {
       const int c = h * 64 + (t >> 3), k = (t & 7) * 4;
       const uint32_t* s = turned + c * kPitch + k;
-      *(u32x4*)(a.col_codes + (a.col_r0 + tc * 128 + c) * a.col_ld +
-                b * 128 + k * 4) = u32x4{s[0], s[1], s[2], s[3]};
+      *(u32x4*)(a.col_codes +
+                (b * a.col_n + a.col_r0 + tc * 128 + c) * 128 + k * 4) =
+          u32x4{s[0], s[1], s[2], s[3]};
     }
   }
 }
@@ -227,8 +228,8 @@ __global__ __launch_bounds__(kThreads) void swiglu_fwd(
     store8<T, VEC>(h + at.row * C, c, C, o);
     if (gc) {
       const long long s = at.q * Rp + at.row;
-      pack512(a, lane, c, Cp, gc + at.row * Cp, gs + s);
-      pack512(b, lane, c, Cp, uc + at.row * Cp, us + s);
+      pack512(a, lane, c, Cp, gc, R, at.row, gs + s);
+      pack512(b, lane, c, Cp, uc, R, at.row, us + s);
     }
   }
 }
@@ -253,9 +254,9 @@ __global__ __launch_bounds__(kThreads) void swiglu_bwd(
     const int shift = 8 * (lane >> 4);
     float a[8], b[8], d[8];
     load8<T, VEC>(dh + at.row * ldh, c, C, d);
-    decode8(*(const u32x2*)(gc + at.row * Cp + c),
+    decode8(*(const u32x2*)code_at(gc, R, at.row, c),
             scale_value(gs[s] >> shift & 255u), a);
-    decode8(*(const u32x2*)(uc + at.row * Cp + c),
+    decode8(*(const u32x2*)code_at(uc, R, at.row, c),
             scale_value(us[s] >> shift & 255u), b);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(kThreads) void rms_fwd(
       const int q = q0 + i * WPR, c = q * 512 + lane * 8;
       if (q * 512 >= Cp) continue;  // the same for the whole wave
       if (codes)
-        pack512(v[i], lane, c, Cp, codes + r * Cp, scales + q * Rp + r);
+        pack512(v[i], lane, c, Cp, codes, R, r, scales + q * Rp + r);
       float g[8];
       load8<Fp32, VEC>(w, c, C, g);
 #pragma unroll
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(kThreads) void rms_bwd(
       u32x2 code = {0, 0};
       uint32_t E = 1;
       if (c < Cp) {
-        code = *(const u32x2*)(codes + r * Cp + c);
+        code = *(const u32x2*)code_at(codes, R, r, c);
         E = scales[q * Rp + r] >> (8 * (lane >> 4)) & 255u;
       }
       decode8(code, scale_value(E), n[i]);

@@ -10,16 +10,17 @@ namespace b8 {
 struct TileArgs {
   const void* x;        // plain numbers, or codes
   const uint32_t* xs;   // codes: their scales
-  long long ldx;        // elements a row (codes: bytes)
+  long long ldx;        // elements a row (codes: rows of the packed matrix)
   long long xsp;        // codes: padded rows of xs
   long long R;
   int C;
-  uint8_t* row_codes;   // [..][row_ld]; row 0, column 0 of this matrix lie
-  uint8_t* row_scales;  // at (row_r0, row_c0), both multiples of 128
-  long long row_ld, row_sp, row_c0, row_r0;
-  uint8_t* col_codes;   // transposed: value (r, c) is at row col_r0 + c,
-  uint8_t* col_scales;  // column col_c0 + r
-  long long col_ld, col_sp, col_r0, col_c0;
+  // outputs are packed matrices of row_n, col_n rows (scales row_sp, col_sp)
+  uint8_t* row_codes;   // value (r, c) is at row row_r0 + r, column
+  uint8_t* row_scales;  // row_c0 + c; the offsets are multiples of 128
+  long long row_n, row_sp, row_c0, row_r0;
+  uint8_t* col_codes;   // transposed: at row col_r0 + c, column col_c0 + r
+  uint8_t* col_scales;
+  long long col_n, col_sp, col_r0, col_c0;
 };
 
 // Y[m][n] = sum_k X[m][k] W[n][k], X and W packed along k (gemm8.hip).
@@ -29,11 +30,11 @@ constexpr int kMaxParts = 4;
 struct GemmArgs {
   const uint8_t* x;
   const uint32_t* xs;
-  long long ldx, xsp;
+  long long xn, xsp;  // rows of the codes, padded rows of the scales
   const uint8_t* w;
   const uint32_t* ws;
-  long long ldw, wsp;
-  int M, N;  // rows of x and of w
+  long long wn, wsp;
+  int M, N;  // rows of x and of w that take part
   int KT;    // K steps of 128
   void* out[kMaxParts];
   int first[kMaxParts];  // first row of w
@@ -83,7 +84,10 @@ void launch_b8_rms_bwd(int dtype, int vec, const void* dy, long long ldy,
                        long long Rp, const float* w, const float* inv,
                        long long R, int C, void* dx, float* partials,
                        float* dw, hipStream_t st);
-void launch_b8_gemm(const b8::GemmArgs* args, hipStream_t st);
+// bytes of workspace that the product wants, and the product
+long long b8_gemm_workspace(const b8::GemmArgs* args);
+void launch_b8_gemm(const b8::GemmArgs* args, float* workspace,
+                    hipStream_t st);
 void launch_b8_gemm_bf16(const b8::GemmArgs* args, const void* x,
                          long long ldx, int K, hipStream_t st);
 }

@@ -30,12 +30,6 @@ __device__ __forceinline__ int swizzled(int row, int chunk) {
   return row * 128 + ((chunk ^ (row >> 1 & 7)) << 4);
 }
 
-__device__ __forceinline__ i32x8 fragment(const char* tile, int row, int g) {
-  const i32x4 lo = *(const i32x4*)(tile + swizzled(row, 2 * g));
-  const i32x4 hi = *(const i32x4*)(tile + swizzled(row, 2 * g + 1));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
 // where a wave's columns go: they lie inside one of the outputs, as both
 // start at multiples of 128 rows of w
 struct Out {
@@ -74,129 +68,42 @@ __device__ __forceinline__ void store4(const Out& o, int m, int c, f32x4 v) {
   }
 }
 
-// BM rows of x by BN rows of w; WM x WN waves.  Both tiles of a K step and,
-// every fourth step, the scale dwords of all rows go straight to LDS
-// (global_load_lds); two buffers, the next step's loads issued before this
-// step's products and drained by the barrier after them.
-template <int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64) void gemm_tile(GemmArgs a,
-                                                         int tiles_n) {
-  constexpr int kWaves = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int kTile = (BM + BN) * 128;
-  __shared__ __align__(16) char lds[2 * kTile + 2 * (BM + BN) * 4];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  const int m0 = blockIdx.x / tiles_n * BM, n0 = blockIdx.x % tiles_n * BN;
-  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-
-  // a wave's load covers 8 rows; rows past the end read the last one, their
-  // products are never stored
-  constexpr int kLoads = (BM + BN) / 8 / kWaves;
-  const uint8_t* src[kLoads];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int row = (i * kWaves + wave) * 8 + (lane >> 3);
-    const int chunk = (lane & 7) ^ (row >> 1 & 7);
-    if (row < BM) {
-      const int m = min(m0 + row, a.M - 1);
-      src[i] = a.x + m * a.ldx + chunk * 16;
-    } else {
-      const int n = min(n0 + row - BM, a.N - 1);
-      src[i] = a.w + n * a.ldw + chunk * 16;
-    }
-  }
-  auto stage = [&](int kt) {
-    char* buf = lds + (kt & 1) * kTile;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      __builtin_amdgcn_global_load_lds(
-          B8_GLOBAL(src[i] + (long long)kt * 128),
-          B8_LDS(buf + (i * kWaves + wave) * 1024), 16, 0, 0);
-    if ((kt & 3) == 0) {
-      char* sc = lds + 2 * kTile + (kt >> 2 & 1) * (BM + BN) * 4;
-#pragma unroll
-      for (int i = 0; i < (BM + BN) / 64; i += kWaves) {
-        if (i + wave < (BM + BN) / 64) {
-          const int row = (i + wave) * 64;
-          const uint32_t* s =
-              row < BM ? a.xs + (kt >> 2) * a.xsp + m0 + row
-                       : a.ws + (kt >> 2) * a.wsp + n0 + row - BM;
-          __builtin_amdgcn_global_load_lds(B8_GLOBAL(s + lane),
-                                           B8_LDS(sc + row * 4), 4, 0, 0);
-        }
-      }
-    }
-  };
-
-  f32x4 acc[FM * FN];
-#pragma unroll
-  for (int i = 0; i < FM * FN; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  stage(0);
-  __syncthreads();
-  for (int kt = 0; kt < a.KT; ++kt) {
-    if (kt + 1 < a.KT) stage(kt + 1);
-    const char* xt = lds + (kt & 1) * kTile;
-    const char* wt = xt + BM * 128;
-    const uint32_t* sc =
-        (const uint32_t*)(lds + 2 * kTile + (kt >> 2 & 1) * (BM + BN) * 4);
-    const int shift = 8 * (kt & 3);
-    i32x8 wf[FN];
-    int wsc[FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      wf[j] = fragment(wt, wn + j * 16 + r, g);
-      wsc[j] = (int)(sc[BM + wn + j * 16 + r] >> shift);
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const i32x8 xf = fragment(xt, wm + i * 16 + r, g);
-      const int xsc = (int)(sc[wm + i * 16 + r] >> shift);
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-        acc[i * FN + j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            wf[j], xf, acc[i * FN + j], 0, 0, 0, wsc[j], 0, xsc);
-    }
-    __syncthreads();
-  }
-
-  const Out o = out_of(a, n0 + wn);
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = m0 + wm + i * 16 + r;
-    if (m < a.M) {
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-        store4(o, m, o.c0 + j * 16 + 4 * g, acc[i * FN + j]);
-    }
-  }
-}
-
-// ------------------------------------------------------------ large tiles
-// 256 x 256 by four waves, each 128 x 128 as 4 x 4 of 32x32x64.  A wave
-// reads (128 + 128) bytes of LDS a unit of K for 128 x 128 products; eight
-// waves of 128 x 64 would read 1.5 times as much, which with the writes is
-// all that LDS can do.  One wave a SIMD, so the overlap is inside the wave:
-// the fragments of the next half step are read while this half's products
-// run, and one barrier a K step serves both uses of a buffer:
+// ------------------------------------------------------------ tiles in LDS
+// Four waves, 2 x 2, each FX x FW products of 32x32x64 (one is half a block
+// of K; both halves take the same scale).  One workgroup a CU, so the
+// overlap is inside the wave: the fragments of the next half step are read
+// while this half's products run, and one barrier a K step serves both uses
+// of a buffer:
 //
 //   half 0: products of (kt, 0)    reads (kt, 1) from buffer kt
 //   barrier: buffer kt is read by all, the loads of kt + 1 have landed
 //   half 1: products of (kt, 1)    reads (kt + 1, 0) from buffer kt + 1
-//                                  loads kt + 2 into buffer kt
+//                                  loads kt + NBUF into buffer kt
 //
-// so a load has two half steps (2048 cycles of matrix work) to land.
+// Every wave issues the same number of loads a step, so that the barrier
+// waits for the oldest step's only and leaves NBUF - 2 steps in flight.
+//
+// 4 x 4 is for large products: a wave reads 128 + 128 bytes of LDS a unit of
+// K for 128 x 128 products; eight waves of 128 x 64 would read 1.5 times as
+// much, which with the writes is all that LDS can do.  2 x 2 has more
+// workgroups and more steps in flight, for products too small to fill the
+// card with 256 x 256.
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 
-struct Half {
-  i32x8 x[4], w[4];
-};
-
-__global__ __launch_bounds__(256, 1) void gemm_large(GemmArgs a, int tiles_m,
-                                                     int tiles_n, int group) {
-  constexpr int kTile = 512 * 128, kScales = 512 * 4;
-  __shared__ __align__(16) char lds[2 * kTile + 2 * kScales];
+template <int FX, int FW, int NBUF>
+__global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a, int tiles_m,
+                                                    int tiles_n, int group,
+                                                    int splits,
+                                                    float* partials) {
+  constexpr int BM = 64 * FX, BN = 64 * FW, kRows = BM + BN;
+  constexpr int kTile = kRows * 128, kScales = kRows * 4;
+  constexpr int kRing = NBUF <= 2 ? 2 : 4;     // quads of scales
+  constexpr int kProducts = FX * FW;           // a half step
+  constexpr int kReads = 2 * (FX + FW);        // 16 bytes a lane
+  constexpr int kLoads = kRows / 32;           // tile loads a step and wave
+  constexpr int kInFlight = (NBUF - 2) * (kLoads + 2);
+  static_assert(kInFlight < 64 && 4 * kRing >= NBUF + 6);
+  __shared__ __align__(16) char lds[NBUF * kTile + kRing * kScales];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -204,7 +111,8 @@ __global__ __launch_bounds__(256, 1) void gemm_large(GemmArgs a, int tiles_m,
   // the 8 XCDs takes a contiguous run of that order, so that the tiles in
   // its L2 at one time are a compact block
   const int tiles = tiles_m * tiles_n;
-  int t = blockIdx.x;
+  int t = blockIdx.x % tiles;
+  const int split = blockIdx.x / tiles;
   {
     const int q = tiles / 8, r = tiles % 8, xcd = t % 8, idx = t / 8;
     t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
@@ -213,82 +121,109 @@ __global__ __launch_bounds__(256, 1) void gemm_large(GemmArgs a, int tiles_m,
   const int rows = min(group, tiles_m - band * group);
   // divisions are done in vector registers; buffer descriptors need scalars
   const int m0 = __builtin_amdgcn_readfirstlane(
-      (band * group + in_band % rows) * 256);
-  const int n0 = __builtin_amdgcn_readfirstlane(in_band / rows * 256);
-  const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;
+      (band * group + in_band % rows) * BM);
+  const int n0 = __builtin_amdgcn_readfirstlane(in_band / rows * BN);
+  const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
 
-  // loads by buffer descriptors: rows past the end read as zero
-  const auto rx = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(a.x + (long long)m0 * a.ldx), 0,
-      (int)(min(256, a.M - m0) * a.ldx), 0x00020000);
-  const auto rw = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(a.w + (long long)n0 * a.ldw), 0,
-      (int)(min(256, a.N - n0) * a.ldw), 0x00020000);
+  // this split's K steps: whole quads, so that scale dwords stay whole, and
+  // at least one, as there are no more splits than quads
+  const int quads = (a.KT + 3) >> 2;
+  const int q0 = __builtin_amdgcn_readfirstlane(
+      (int)((long long)quads * split / splits));
+  const int q1 = __builtin_amdgcn_readfirstlane(
+      (int)((long long)quads * (split + 1) / splits));
+  const int KT = min(4 * q1, a.KT) - 4 * q0;
+
+  // Loads by buffer descriptors: rows past the end read as zero, and all
+  // that changes from step to step is a base address a matrix.  Scalar
+  // arithmetic between the products would hold them up: a lone wave issues
+  // one instruction in about four cycles.
+  const uint8_t* px = a.x + (4 * q0 * a.xn + m0) * 128;
+  const uint8_t* pw = a.w + (4 * q0 * a.wn + n0) * 128;
+  const long long x_step = a.xn * 128, w_step = a.wn * 128;
+  const int x_bytes = min(BM, a.M - m0) * 128;
+  const int w_bytes = min(BN, a.N - n0) * 128;
+  const auto rxs = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(a.xs + q0 * a.xsp + m0), 0,
+      (int)((quads - q0) * a.xsp - m0) * 4, 0x00020000);
+  const auto rws = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(a.ws + q0 * a.wsp + n0), 0,
+      (int)((quads - q0) * a.wsp - n0) * 4, 0x00020000);
   const int lrow = wave * 8 + (lane >> 3);
-  const int lchunk = ((lane & 7) ^ (lrow >> 1 & 7)) * 16;
-  const int vx = lrow * (int)a.ldx + lchunk;
-  const int vw = lrow * (int)a.ldw + lchunk;
-
-  // scales of quad q: piece 0 those of x, 1 those of w
-  const int Q = (a.KT + 3) >> 2;
-  auto load_scales = [&](int q, int piece) {
-    char* sc = lds + 2 * kTile + (q & 1) * kScales + piece * 1024;
-    const int at = min(q, Q - 1);
-    const uint32_t* src = piece ? a.ws + at * a.wsp + n0
-                                : a.xs + at * a.xsp + m0;
-    __builtin_amdgcn_global_load_lds(B8_GLOBAL(src + wave * 64 + lane),
-                                     B8_LDS(sc + wave * 256), 4, 0, 0);
-  };
-  // the n-th of a step's 16 loads a wave: 8 rows of x, then of w
+  const int at = lrow * 128 + ((lane & 7) ^ (lrow >> 1 & 7)) * 16;
+  // the n-th of a step's loads: 32 rows of x, then of w
   auto load = [&](int step, int n) {
-    char* to = lds + (step & 1) * kTile + (n * 32 + wave * 8) * 128;
-    const int kt = min(step, a.KT - 1), row = n % 8 * 32;
-    if (n < 8)
+    char* to = lds + step % NBUF * kTile + (n * 32 + wave * 8) * 128;
+    if (n < BM / 32)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rx, B8_LDS(to), 16, vx, row * (int)a.ldx + kt * 128, 0, 0);
+          __builtin_amdgcn_make_buffer_rsrc((void*)px, 0, x_bytes,
+                                            0x00020000),
+          B8_LDS(to), 16, at, n * 4096, 0, 0);
     else
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rw, B8_LDS(to), 16, vw, row * (int)a.ldw + kt * 128, 0, 0);
+          __builtin_amdgcn_make_buffer_rsrc((void*)pw, 0, w_bytes,
+                                            0x00020000),
+          B8_LDS(to), 16, at, (n - BM / 32) * 4096, 0, 0);
+  };
+  auto advance = [&](int step) {
+    px += step + 1 < KT ? x_step : 0;
+    pw += step + 1 < KT ? w_step : 0;
+  };
+  // two loads of scales a step and wave, those of quad (step + 3) / 4: its
+  // four steps bring it four times, all before the first of them is read
+  const int sx_at = wave % (BM / 64) * 64, sw_at = wave % (BN / 64) * 64;
+  auto load_scales = [&](int q) {
+    char* to = lds + NBUF * kTile + q % kRing * kScales;
+    const int at = min(q, q1 - q0 - 1);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rxs, B8_LDS(to + sx_at * 4), 4, (sx_at + lane) * 4,
+        at * (int)a.xsp * 4, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rws, B8_LDS(to + (BM + sw_at) * 4), 4, (sw_at + lane) * 4,
+        at * (int)a.wsp * 4, 0, 0);
   };
 
   // fragment (row = lane % 32, 32 bytes at half * 64 + lane / 32 * 32), in
-  // the order that the products want them
+  // the order that the products want them: x0 w0 .. x1 ..
+  struct Half {
+    i32x8 x[FX], w[FW];
+  };
   const int frow = lane & 31, fg = lane >> 5;
   auto read = [&](Half& f, int kt, int half, int n) {
-    // n / 2: x0 w0 w1 w2 w3 x1 x2 x3
     const int k = n / 2, c = 4 * half + 2 * fg + n % 2;
-    const bool of_w = k >= 1 && k < 5;
-    const int row = of_w ? 256 + wn + (k - 1) * 32
-                         : wm + (k ? k - 4 : 0) * 32;
-    const i32x4 v = *(const i32x4*)(lds + (kt & 1) * kTile +
+    const bool of_w = k >= 1 && k <= FW;
+    const int row = of_w ? BM + wn + (k - 1) * 32
+                         : wm + (k ? k - FW : 0) * 32;
+    const i32x4 v = *(const i32x4*)(lds + kt % NBUF * kTile +
                                     swizzled(row + frow, c));
-    i32x8& to = of_w ? f.w[k - 1] : f.x[k ? k - 4 : 0];
+    i32x8& to = of_w ? f.w[k - 1] : f.x[k ? k - FW : 0];
 #pragma unroll
     for (int i = 0; i < 4; ++i) to[n % 2 * 4 + i] = v[i];
   };
-  uint32_t quad_x[4], quad_w[4];  // the scales of four K steps
+  uint32_t quad_x[FX], quad_w[FW];  // the scales of four K steps
   auto read_scales = [&](int kt) {
-    const uint32_t* sc =
-        (const uint32_t*)(lds + 2 * kTile + (kt >> 2 & 1) * kScales);
+    const uint32_t* sc = (const uint32_t*)(lds + NBUF * kTile +
+                                           (kt >> 2) % kRing * kScales);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      quad_x[i] = sc[wm + i * 32 + frow];
-      quad_w[i] = sc[256 + wn + i * 32 + frow];
-    }
+    for (int i = 0; i < FX; ++i) quad_x[i] = sc[wm + i * 32 + frow];
+#pragma unroll
+    for (int j = 0; j < FW; ++j) quad_w[j] = sc[BM + wn + j * 32 + frow];
   };
 
-  f32x16 acc[16];
+  f32x16 acc[kProducts];
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int i = 0; i < kProducts; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
-  auto product = [&](const Half& f, const int (&sx)[4], const int (&sw)[4],
+  auto product = [&](const Half& f, const int (&sx)[FX], const int (&sw)[FW],
                      int n) {
     acc[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-        f.w[n % 4], f.x[n / 4], acc[n], 0, 0, 0, sw[n % 4], 0, sx[n / 4]);
+        f.w[n % FW], f.x[n / FW], acc[n], 0, 0, 0, sw[n % FW], 0,
+        sx[n / FW]);
   };
   auto meet = [&] {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight)
+                 : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
@@ -296,59 +231,77 @@ __global__ __launch_bounds__(256, 1) void gemm_large(GemmArgs a, int tiles_m,
   // Past the last step the loads repeat it and the reads find what is
   // there; nothing uses either.  The alternative, a peeled tail, made the
   // compiler copy all accumulators.
-  load_scales(0, 0);
-  load_scales(0, 1);
 #pragma unroll
-  for (int n = 0; n < 16; ++n) load(0, n);
+  for (int step = 0; step < NBUF; ++step) {
+    load_scales(step + 3 >> 2);
 #pragma unroll
-  for (int n = 0; n < 16; ++n) load(1, n);
-  meet();
+    for (int n = 0; n < kLoads; ++n) load(step, n);
+    advance(step);
+  }
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NBUF - 1) * (kLoads + 2))
+               : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
   Half f0, f1;
 #pragma unroll
-  for (int n = 0; n < 16; ++n) read(f0, 0, 0, n);
+  for (int n = 0; n < kReads; ++n) read(f0, 0, 0, n);
   read_scales(0);
-  // the fence after each product keeps the order written here
-  for (int kt = 0; kt < a.KT; ++kt) {
-    int sx[4], sw[4];
+  // the reads are done early in the half, the loads spread over it
+  constexpr int kReadsEach =
+      kProducts >= 4 ? 2 : (kReads + kProducts - 1) / kProducts;
+  constexpr int kLoadsEach = (kLoads + kProducts - 1) / kProducts;
+  static_assert(kReadsEach * kProducts >= kReads);
+  // the fence after each product keeps the order written here: loads in a
+  // burst would fill the memory unit's queue and hold up the products
+  for (int kt = 0; kt < KT; ++kt) {
+    int sx[FX], sw[FW];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sx[i] = (int)(quad_x[i] >> (8 * (kt & 3)));
-      sw[i] = (int)(quad_w[i] >> (8 * (kt & 3)));
-    }
+    for (int i = 0; i < FX; ++i) sx[i] = (int)(quad_x[i] >> (8 * (kt & 3)));
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
+    for (int j = 0; j < FW; ++j) sw[j] = (int)(quad_w[j] >> (8 * (kt & 3)));
+#pragma unroll
+    for (int n = 0; n < kProducts; ++n) {
       product(f0, sx, sw, n);
-      if (n < 8) read(f1, kt, 1, 2 * n), read(f1, kt, 1, 2 * n + 1);
+#pragma unroll
+      for (int k = n * kReadsEach; k < (n + 1) * kReadsEach; ++k)
+        if (k < kReads) read(f1, kt, 1, k);
       __builtin_amdgcn_sched_barrier(0);
     }
     meet();
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
+    for (int n = 0; n < kProducts; ++n) {
       product(f1, sx, sw, n);
-      load(kt + 2, n);
-      if (n < 8) read(f0, kt + 1, 0, 2 * n), read(f0, kt + 1, 0, 2 * n + 1);
-      if (n == 8) read_scales(kt + 1);
-      // one piece of the next quad a step (each comes twice); its buffer
-      // was last read before this step's barrier
-      if (n == 15) load_scales((kt + 1 >> 2) + 1, kt + 1 & 1);
+      if (n == 0) load_scales(kt + NBUF + 3 >> 2);
+#pragma unroll
+      for (int k = n * kLoadsEach; k < (n + 1) * kLoadsEach; ++k)
+        if (k < kLoads) load(kt + NBUF, k);
+#pragma unroll
+      for (int k = n * kReadsEach; k < (n + 1) * kReadsEach; ++k)
+        if (k < kReads) read(f0, kt + 1, 0, k);
+      if (n == kProducts / 2) read_scales(kt + 1);
+      if (n == kProducts - 1) advance(kt + NBUF);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  meet();
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 
   // lane: row m = lane % 32 of its fragment, columns (r / 4) * 8 +
   // lane / 32 * 4 + r % 4
-  const Out o = out_of(a, n0 + wn);
+  Out o = out_of(a, n0 + wn);
+  if (splits > 1)
+    o = Out{partials + (long long)split * a.M * a.N, n0 + wn, a.N, 1};
   if (o.f32 || (o.count & 7)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < FX; ++i) {
       const int m = m0 + wm + i * 32 + frow;
       if (m < a.M) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < FW; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const f32x16& v = acc[i * 4 + j];
+            const f32x16& v = acc[i * FW + j];
             store4(o, m, o.c0 + j * 32 + r * 8 + fg * 4,
                    f32x4{v[4 * r], v[4 * r + 1], v[4 * r + 2],
                          v[4 * r + 3]});
@@ -357,19 +310,21 @@ __global__ __launch_bounds__(256, 1) void gemm_large(GemmArgs a, int tiles_m,
     }
     return;
   }
-  // through LDS, 32 KB a wave, so that 16 lanes store 256 bytes of one row:
-  // straight from the accumulators a store would touch 16 bytes of 32 rows.
-  // 16-byte chunk c of row m lies at c ^ (m % 16)
-  char* mine = lds + wave * 32768;
+  // through LDS, so that a row's lanes store whole lines: straight from the
+  // accumulators a store would touch 16 bytes of 32 rows.  16-byte chunk c
+  // of row m lies at c ^ m % kChunks
+  constexpr int kChunks = FW * 4, kRowBytes = FW * 64;
+  char* mine = lds + wave * (FX * 32 * kRowBytes);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < FX; ++i) {
     const int m = i * 32 + frow;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < FW; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const f32x16& v = acc[i * 4 + j];
-        *(u32x2*)(mine + m * 256 + ((j * 4 + r ^ m & 15) << 4) + fg * 8) =
+        const f32x16& v = acc[i * FW + j];
+        *(u32x2*)(mine + m * kRowBytes +
+                  ((j * 4 + r ^ m % kChunks) << 4) + fg * 8) =
             u32x2{Bf16::from_f(v[4 * r]) |
                       (uint32_t)Bf16::from_f(v[4 * r + 1]) << 16,
                   Bf16::from_f(v[4 * r + 2]) |
@@ -377,30 +332,51 @@ __global__ __launch_bounds__(256, 1) void gemm_large(GemmArgs a, int tiles_m,
       }
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  const int c = lane & 15;
+  const int c = lane % kChunks;
   if (o.c0 + c * 8 >= o.count) return;
   uint16_t* out = (uint16_t*)o.p + o.c0 + c * 8;
+  constexpr int kRowsEach = 64 / kChunks;
 #pragma unroll 8
-  for (int k = 0; k < 32; ++k) {
-    const int row = k * 4 + (lane >> 4), m = m0 + wm + row;
-    const u32x4 v = *(const u32x4*)(mine + row * 256 + ((c ^ row & 15) << 4));
+  for (int k = 0; k < FX * 32 / kRowsEach; ++k) {
+    const int row = k * kRowsEach + lane / kChunks, m = m0 + wm + row;
+    const u32x4 v = *(const u32x4*)(mine + row * kRowBytes +
+                                    ((c ^ row % kChunks) << 4));
     if (m < a.M) *(u32x4*)(out + (long long)m * o.count) = v;
   }
 }
 
-// -------------------------------------------------------------- few rows
-// Up to 64 rows of x: the time is that of reading w once.  A workgroup takes
-// 16 rows of w; its waves share K by quads of four K steps (512 bytes of a
-// row, read by every lane's 16-byte loads straight into the operand), and
-// their sums meet in LDS, added in the order of the waves.  With FUSED, for
-// up to 16 rows of bf16, x is packed on the way: each lane needs 32
-// neighbouring values a step, which four lanes share a scale for, so the
-// codes are those of pack_rows and a launch is saved.
-struct RowsArgs {
+// the sums of the splits, in order, to the outputs; 4 columns a thread
+__global__ __launch_bounds__(256) void join_splits(GemmArgs a, int splits,
+                                                   const float* partials) {
+  const int groups = a.N / 4;  // N is a multiple of 128 where K is split
+  const long long all = (long long)a.M * groups;
+  const long long step = (long long)gridDim.x * 256;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += step) {
+    const int m = (int)(i / groups), n = (int)(i - (long long)m * groups) * 4;
+    const float* p = partials + (long long)m * a.N + n;
+    f32x4 v = *(const f32x4*)p;
+    for (int s = 1; s < splits; ++s)
+      v += *(const f32x4*)(p + (long long)s * a.M * a.N);
+    const Out o = out_of(a, n);
+    store4(o, m, o.c0, v);
+  }
+}
+
+// ------------------------------------------------------- K over the waves
+// Small products, few rows among them: what counts is how soon all of w and
+// x is under way.  A workgroup takes 16 FM rows of x by 16 FN rows of w; its
+// waves share K, U steps at a time, and load their operands straight from
+// global memory: within a workgroup nothing is read twice, so LDS would save
+// nothing, and there is no barrier before the sums meet in LDS, added in the
+// order of the waves.  With FUSED, for up to 16 rows of bf16, x is packed on
+// the way: each lane needs 32 neighbouring values a step, which four lanes
+// share a scale for, so the codes are those of pack_rows and a launch is
+// saved.
+struct SplitArgs {
   GemmArgs g;
   const uint16_t* x;  // FUSED: bf16, rows of ldx elements, K columns
   long long ldx;
-  int K;
+  int K, tiles_n;
 };
 
 using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
@@ -448,140 +424,249 @@ __device__ __forceinline__ i32x8 pack_step(const u32x4 (&v)[4], int* scale) {
   return code;
 }
 
-template <int FM, int WAVES, bool FUSED>
-__global__ __launch_bounds__(WAVES * 64) void gemm_rows(RowsArgs ra) {
-  const GemmArgs& a = ra.g;
-  __shared__ f32x4 sums[WAVES][FM][64];
+template <int FM, int FN, int U, int WAVES, bool FUSED>
+__global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
+  const GemmArgs& a = sa.g;
+  extern __shared__ f32x4 sums[];  // [WAVES][FM * FN][64]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int n = min(n0 + r, a.N - 1);
-  const uint8_t* w = a.w + n * a.ldw + g * 32;
-  const uint32_t* ws = a.ws + n;
+  const int m0 = (int)(blockIdx.x / sa.tiles_n) * 16 * FM;
+  const int n0 = (int)(blockIdx.x % sa.tiles_n) * 16 * FN;
+  // rows past the end repeat the last one and are not stored
+  const uint8_t* w[FN];
+  const uint32_t* ws[FN];
+#pragma unroll
+  for (int j = 0; j < FN; ++j) {
+    const int n = min(n0 + j * 16 + r, a.N - 1);
+    w[j] = a.w + n * 128ll + g * 32;
+    ws[j] = a.ws + n;
+  }
+  const uint8_t* x[FM];
+  const uint32_t* xs[FM];
+  if constexpr (!FUSED) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int m = min(m0 + i * 16 + r, a.M - 1);
+      x[i] = a.x + m * 128ll + g * 32;
+      xs[i] = a.xs + m;
+    }
+  }
 
-  f32x4 acc[FM];
+  f32x4 acc[FM * FN];
 #pragma unroll
-  for (int i = 0; i < FM; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int Q = (a.KT + 3) >> 2;
-  for (int q = wave; q < Q; q += WAVES) {
-    i32x4 wv[4][2];
-    i32x8 xv[4][FM];
-    u32x4 raw[FUSED ? 4 : 1][4];
-    uint32_t xs[FM];
-    const uint32_t wsc = ws[q * a.wsp];
+  for (int i = 0; i < FM * FN; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  static_assert(4 % U == 0);  // so that U steps have one scale dword a row
+  for (int k0 = wave * U; k0 < a.KT; k0 += WAVES * U) {
+    i32x4 wv[U][FN][2], xv[U][FUSED ? 1 : FM][2];
+    u32x4 raw[FUSED ? U : 1][4];
+    uint32_t wq[FN], xq[FM];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int kt = min(4 * q + j, a.KT - 1);
-      const i32x4* p = (const i32x4*)(w + (long long)kt * 128);
-      wv[j][0] = p[0];
-      wv[j][1] = p[1];
+    for (int j = 0; j < FN; ++j) {
+      wq[j] = ws[j][(k0 >> 2) * a.wsp];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const i32x4* p =
+            (const i32x4*)(w[j] + min(k0 + u, a.KT - 1) * a.wn * 128);
+        wv[u][j][0] = p[0];
+        wv[u][j][1] = p[1];
+      }
     }
     if constexpr (FUSED) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int k = (4 * q + j) * 128 + g * 32 + c * 8;
-          raw[j][c] = r < a.M && k < ra.K
-                          ? *(const u32x4*)(ra.x + r * ra.ldx + k)
+          const int k = (k0 + u) * 128 + g * 32 + c * 8;
+          raw[u][c] = r < a.M && k < sa.K
+                          ? *(const u32x4*)(sa.x + r * sa.ldx + k)
                           : u32x4{0, 0, 0, 0};
         }
     } else {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const int m = min(i * 16 + r, a.M - 1);
-        xs[i] = a.xs[q * a.xsp + m];
+        xq[i] = xs[i][(k0 >> 2) * a.xsp];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int kt = min(4 * q + j, a.KT - 1);
+        for (int u = 0; u < U; ++u) {
           const i32x4* p =
-              (const i32x4*)(a.x + m * a.ldx + (long long)kt * 128 + g * 32);
-          // past the end w repeats its last block, against zeros; the
-          // scales there are not written, see below
-          const i32x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-          xv[j][i] = 4 * q + j < a.KT
-                         ? __builtin_shufflevector(p[0], p[1], 0, 1, 2, 3, 4,
-                                                   5, 6, 7)
-                         : zero;
+              (const i32x4*)(x[i] + min(k0 + u, a.KT - 1) * a.xn * 128);
+          xv[u][i][0] = p[0];
+          xv[u][i][1] = p[1];
         }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool inside = 4 * q + j < a.KT;
-      const int sw = inside ? (int)(wsc >> (8 * j)) : 1;
-      const i32x8 wf =
-          __builtin_shufflevector(wv[j][0], wv[j][1], 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int u = 0; u < U; ++u) {
+      // past the end w repeats its last block, against zeros; scales there
+      // may never have been written
+      const bool inside = k0 + u < a.KT;
+      const int shift = 8 * (k0 + u & 3);
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         int sx;
         i32x8 xf;
         if constexpr (FUSED) {
-          xf = pack_step(raw[j], &sx);
+          xf = pack_step(raw[u], &sx);
         } else {
-          xf = xv[j][i];
-          sx = inside ? (int)(xs[i] >> (8 * j)) : 1;
+          const i32x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+          xf = inside ? __builtin_shufflevector(xv[u][i][0], xv[u][i][1], 0,
+                                                1, 2, 3, 4, 5, 6, 7)
+                      : zero;
+          sx = inside ? (int)(xq[i] >> shift) : 1;
         }
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            wf, xf, acc[i], 0, 0, 0, sw, 0, sx);
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i * FN + j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              __builtin_shufflevector(wv[u][j][0], wv[u][j][1], 0, 1, 2, 3, 4,
+                                      5, 6, 7),
+              xf, acc[i * FN + j], 0, 0, 0,
+              inside ? (int)(wq[j] >> shift) : 1, 0, sx);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < FM; ++i) sums[wave][i][lane] = acc[i];
+  for (int i = 0; i < FM * FN; ++i)
+    sums[(wave * FM * FN + i) * 64 + lane] = acc[i];
   __syncthreads();
-  if (wave >= FM) return;
-  f32x4 v = sums[0][wave][lane];
 #pragma unroll
-  for (int k = 1; k < WAVES; ++k) v += sums[k][wave][lane];
-  const int m = wave * 16 + r;
-  if (m < a.M) {
-    const Out o = out_of(a, n0);
-    store4(o, m, o.c0 + 4 * g, v);
+  for (int f = 0; f < FM * FN; f += WAVES) {
+    if (f + wave >= FM * FN) return;
+    const int i = (f + wave) / FN, j = (f + wave) % FN;
+    f32x4 v = sums[(f + wave) * 64 + lane];
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k)
+      v += sums[(k * FM * FN + f + wave) * 64 + lane];
+    const int m = m0 + i * 16 + r;
+    if (m < a.M) {
+      const Out o = out_of(a, n0 + j * 16);
+      store4(o, m, o.c0 + 4 * g, v);
+    }
   }
 }
 
-template <int FM, bool FUSED>
-static void rows_run(const RowsArgs& ra, hipStream_t st) {
-  const int blocks = (ra.g.N + 15) / 16, Q = (ra.g.KT + 3) / 4;
-  if (Q <= 4)
-    launch(gemm_rows<FM, 4, FUSED>, blocks, 256, st, ra);
-  else if (Q <= 8 || FM == 4)  // 16 waves have no registers for four
-    launch(gemm_rows<FM, 8, FUSED>, blocks, 512, st, ra);
-  else if constexpr (FM < 4)
-    launch(gemm_rows<FM, 16, FUSED>, blocks, 1024, st, ra);
+template <int FM, int FN, int U, int WAVES, bool FUSED>
+static void split_run(SplitArgs sa, hipStream_t st) {
+  constexpr int kLds = WAVES * FM * FN * 64 * 16;
+  const auto kernel = gemm_split<FM, FN, U, WAVES, FUSED>;
+  sa.tiles_n = (sa.g.N + 16 * FN - 1) / (16 * FN);
+  const long long tiles_m = (sa.g.M + 16 * FM - 1) / (16 * FM);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * sa.tiles_n)),
+                     dim3(WAVES * 64), kLds, st, sa);
+}
+
+// --------------------------------------------------------------- the choice
+// Which kernel, and K split how often: the one with the least predicted
+// time.  A workgroup of gemm_tile takes fixed + steps * step us, where a
+// step is slower when the whole card computes (its power limit); one fits a
+// CU, so more than 256 go in rounds.  Measured in us (gfx950, K steps of
+// 128, one workgroup .. 256):
+//
+//   tile       fixed   step alone   step on a full card
+//   256 x 256   11.7      0.93          1.37
+//   128 x 256    7.9      0.62          0.85
+//   128 x 128    5.7      0.36          0.48
+//    64 x  64    4.0      0.29          0.33
+//
+// Joining the splits costs a launch, about 4 us, and their traffic at about
+// 4 TB/s.  Measured either way, in us: 24576x4096x14336 1004 by 256 x 256
+// and 1500 by 128 x 128; 2048x2048x2048 25 and 14; 1001x777x1111 18, 8.2 and
+// 6.6 by 64 x 64; 128x4096x14336 by 128 x 128 48, and 21 in four splits.
+struct Plan {
+  int kind;  // 0 256 x 256, 1 128 x 256, 2 128 x 128, 3 64 x 64, 4 gemm_split
+  int tiles_m, tiles_n, splits;
+};
+
+static Plan plan_of(const GemmArgs& a) {
+  static const struct {
+    int bm, bn;
+    float fixed, alone, full;
+  } kinds[] = {{256, 256, 11.7f, 0.93f, 1.37f},
+               {128, 256, 7.9f, 0.62f, 0.85f},
+               {128, 128, 5.7f, 0.36f, 0.48f},
+               {64, 64, 4.0f, 0.29f, 0.33f}};
+  const int quads = (a.KT + 3) / 4;
+  Plan best{};
+  float least = 0.f;
+  for (int k = 0; k < 4; ++k) {
+    const int tm = (a.M + kinds[k].bm - 1) / kinds[k].bm;
+    const int tn = (a.N + kinds[k].bn - 1) / kinds[k].bn;
+    for (int splits = 1; splits <= 8; splits *= 2) {
+      if (splits > 1 && quads < 2 * splits) break;
+      const long long groups = (long long)tm * tn * splits;
+      const float steps = 4.f * ((quads + splits - 1) / splits);
+      const auto round = [&](float busy) {
+        return kinds[k].fixed +
+               (splits > 1 ? steps : a.KT) *
+                   (kinds[k].alone +
+                    (kinds[k].full - kinds[k].alone) * busy);
+      };
+      float us = groups / 256 * round(1.f);
+      if (groups % 256) us += round((groups % 256) / 256.f);
+      if (splits > 1)
+        us += 4.f + (4.f * splits + 2.f) * a.M * a.N / 4e6f;
+      if (least == 0.f || us < least) {
+        least = us;
+        best = Plan{k, tm, tn, splits};
+      }
+    }
+  }
+  // 32 rows of x by 16 of w a workgroup, a K step a wave at a time
+  const long long groups = (a.M + 31) / 32 * ((a.N + 15) / 16);
+  const float us =
+      2.3f + 2.8f * ((a.KT + 15) / 16) * (groups < 256 ? 1.f : groups / 256.f);
+  if (us < least) best = Plan{4, 0, 0, 1};
+  return best;
+}
+
+template <int FX, int FW, int NBUF>
+static void tile_run(const GemmArgs& a, const Plan& p, float* partials,
+                     hipStream_t st) {
+  launch(gemm_tile<FX, FW, NBUF>, (long long)p.tiles_m * p.tiles_n * p.splits,
+         256, st, a, p.tiles_m, p.tiles_n, 4, p.splits, partials);
 }
 
 }  // namespace b8
 
 using namespace b8;
 
-extern "C" void launch_b8_gemm(const GemmArgs* args, hipStream_t st) {
+extern "C" long long b8_gemm_workspace(const GemmArgs* args) {
+  const Plan p = plan_of(*args);
+  return p.splits > 1 ? 4ll * p.splits * args->M * args->N : 0;
+}
+
+extern "C" void launch_b8_gemm(const GemmArgs* args, float* workspace,
+                               hipStream_t st) {
   const GemmArgs a = *args;
-  if (a.M <= 64) {
-    const RowsArgs ra{a, nullptr, 0, 0};
-    if (a.M <= 16)
-      rows_run<1, false>(ra, st);
-    else if (a.M <= 32)
-      rows_run<2, false>(ra, st);
-    else
-      rows_run<4, false>(ra, st);
-    return;
+  const Plan p = plan_of(a);
+  if (p.kind == 0)
+    tile_run<4, 4, 2>(a, p, workspace, st);
+  else if (p.kind == 1)
+    tile_run<2, 4, 3>(a, p, workspace, st);
+  else if (p.kind == 2)
+    tile_run<2, 2, 4>(a, p, workspace, st);
+  else if (p.kind == 3)
+    tile_run<1, 1, 8>(a, p, workspace, st);
+  else
+    split_run<2, 1, 1, 16, false>(SplitArgs{a}, st);
+  if (p.splits > 1) {
+    const long long blocks = ((long long)a.M * a.N / 4 + 255) / 256;
+    launch(join_splits, blocks < 4096 ? blocks : 4096, 256, st, a, p.splits,
+           workspace);
   }
-  const int tm = (a.M + 255) / 256, tn = (a.N + 255) / 256;
-  if ((long long)tm * tn >= 192) {
-    launch(gemm_large, (long long)tm * tn, 256, st, a, tm, tn, 4);
-    return;
-  }
-  const int t128 = (a.N + 127) / 128;
-  launch(gemm_tile<128, 128, 2, 2>, (long long)((a.M + 127) / 128) * t128,
-         256, st, a, t128);
 }
 
 // x in bf16, at most 16 rows of K columns, K and ldx multiples of 8, packed
-// on the way; the codes of x in args are not read
+// on the way; the codes of x in args are not read.  A workgroup takes 16
+// columns of y for each FN: more share the packing of x, fewer are more
+// workgroups.  Measured with 1, 2 and 4: 1x2048x2048 4.4, 5.1 and 7.2 us;
+// 16x8192x2048 11.7, 8.7 and 10.3; 8x14336x4096 31, 23.7 and 22.2.
 extern "C" void launch_b8_gemm_bf16(const GemmArgs* args, const void* x,
                                     long long ldx, int K, hipStream_t st) {
-  rows_run<1, true>(RowsArgs{*args, (const uint16_t*)x, ldx, K}, st);
+  const SplitArgs sa{*args, (const uint16_t*)x, ldx, K};
+  if (args->N <= 6144)
+    split_run<1, 1, 1, 16, true>(sa, st);
+  else if (args->N <= 12288)
+    split_run<1, 2, 1, 16, true>(sa, st);
+  else
+    split_run<1, 4, 1, 16, true>(sa, st);
 }
