@@ -194,31 +194,22 @@ def _swiglu_cpu(g, u):
     return (gf * torch.sigmoid(gf) * u.float()).to(g.dtype)
 
 
-class _SwiGLU8Function(torch.autograd.Function):
+class _SwiGLU8Cpu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, g, u):
-        if g.is_cuda:
-            h, *kept = ops.require_ext().swiglu8_fwd(g, u, True)
-        else:
-            h = _swiglu_cpu(g, u)
-            kept = (*_pack_cpu(g), *_pack_cpu(u))
-        ctx.save_for_backward(*kept)
-        return h
+        ctx.save_for_backward(*_pack_cpu(g), *_pack_cpu(u))
+        return _swiglu_cpu(g, u)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        if dh.is_cuda:
-            dg, du = ops.require_ext().swiglu8_bwd(dh, *ctx.saved_tensors)
-        else:
-            gc, gs, uc, us = ctx.saved_tensors
-            C, d = dh.shape[1], dh.float()
-            g = _unpack_cpu(gc, gs, C, torch.float32)
-            u = _unpack_cpu(uc, us, C, torch.float32)
-            s = torch.sigmoid(g)
-            dg = (d * u * s * (1 + g * (1 - s))).to(dh.dtype)
-            du = (d * g * s).to(dh.dtype)
-        return dg, du
+        gc, gs, uc, us = ctx.saved_tensors
+        C, d = dh.shape[1], dh.float()
+        g = _unpack_cpu(gc, gs, C, torch.float32)
+        u = _unpack_cpu(uc, us, C, torch.float32)
+        s = torch.sigmoid(g)
+        return ((d * u * s * (1 + g * (1 - s))).to(dh.dtype),
+                (d * g * s).to(dh.dtype))
 
 
 def swiglu8(g, u):
@@ -231,14 +222,9 @@ def swiglu8(g, u):
                          "{} {} {}, {} {} {}".format(
                              tuple(g.shape), g.dtype, g.device,
                              tuple(u.shape), u.dtype, u.device))
-    shape, g, u = g.shape, _rows(g), _rows(u)
-    if torch.is_grad_enabled() and (g.requires_grad or u.requires_grad):
-        h = _SwiGLU8Function.apply(g, u)
-    elif g.is_cuda:
-        h, = ops.require_ext().swiglu8_fwd(g, u, False)
-    else:
-        h = _swiglu_cpu(g, u)
-    return h.view(shape)
+    if g.is_cuda:
+        return ops.require_ext().swiglu8(g, u)
+    return _SwiGLU8Cpu.apply(_rows(g), _rows(u)).view(g.shape)
 
 
 # ------------------------------------------------------------------- RMSNorm
@@ -247,34 +233,22 @@ def _inv_rms(x, eps):
     return torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps)
 
 
-class _RMSNorm8Function(torch.autograd.Function):
+class _RMSNorm8Cpu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps):
-        if x.is_cuda:
-            y, codes, scales, inv = ops.require_ext().rms8_fwd(
-                x, weight, eps, True)
-        else:
-            inv = _inv_rms(x, eps)
-            y = (x.float() * inv * weight).to(x.dtype)
-            codes, scales = _pack_cpu(x)
-        ctx.save_for_backward(codes, scales, inv, weight)
-        return y
+        inv = _inv_rms(x, eps)
+        ctx.save_for_backward(*_pack_cpu(x), inv, weight)
+        return (x.float() * inv * weight).to(x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         codes, scales, inv, weight = ctx.saved_tensors
-        need_dx, need_dw = ctx.needs_input_grad[:2]
-        if dy.is_cuda:
-            dx, dw = ops.require_ext().rms8_bwd(
-                dy, codes, scales, weight, inv, need_dx, need_dw)
-        else:
-            d = dy.float()
-            n = _unpack_cpu(codes, scales, d.shape[1], torch.float32) * inv
-            a = d * weight
-            dx = inv * (a - n * (a * n).mean(-1, keepdim=True))
-            dx, dw = dx.to(dy.dtype), (d * n).sum(0)
-        return dx if need_dx else None, dw if need_dw else None, None
+        d = dy.float()
+        n = _unpack_cpu(codes, scales, d.shape[1], torch.float32) * inv
+        a = d * weight
+        dx = inv * (a - n * (a * n).mean(-1, keepdim=True))
+        return dx.to(dy.dtype), (d * n).sum(0), None
 
 
 def rms_norm8(x, weight, eps=1e-5):
@@ -287,14 +261,9 @@ def rms_norm8(x, weight, eps=1e-5):
             x.shape[-1], x.device, tuple(weight.shape), weight.device))
     # the kernels take a float32 weight; .float() is differentiable
     weight = weight.float().contiguous()
-    shape, x = x.shape, _rows(x)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        y = _RMSNorm8Function.apply(x, weight, eps)
-    elif x.is_cuda:
-        y, = ops.require_ext().rms8_fwd(x, weight, eps, False)
-    else:
-        y = (x.float() * _inv_rms(x, eps) * weight).to(x.dtype)
-    return y.view(shape)
+    if x.is_cuda:
+        return ops.require_ext().rms_norm8(x, weight, eps)
+    return _RMSNorm8Cpu.apply(_rows(x), weight, eps).view(x.shape)
 
 
 # -------------------------------------------------------------------- linear
@@ -357,52 +326,24 @@ def pack_weight8(*weights):
     return Weight8(codes, scales, counts, K)
 
 
-class _Linear8Function(torch.autograd.Function):
+class _Linear8Cpu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, *weights):
-        if x.is_cuda:
-            *ys, codes, scales = ops.require_ext().linear8_fwd(
-                x, list(weights))
-        else:
-            held = _held(x)
-            ys = [(held @ _held_weight(w).t()).to(x.dtype) for w in weights]
-            codes, scales = _pack_cpu(x)
-        if any(ctx.needs_input_grad[1:]):
-            ctx.save_for_backward(codes, scales, *weights)
-        else:  # dX does not read x
-            ctx.save_for_backward(None, None, *weights)
-        return tuple(ys)
+        held = _held(x)
+        ctx.save_for_backward(*_pack_cpu(x), *weights)
+        return tuple((held @ _held_weight(w).t()).to(x.dtype)
+                     for w in weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *dys):
         codes, scales, *weights = ctx.saved_tensors
-        need_dx, need_dw = ctx.needs_input_grad[0], \
-            any(ctx.needs_input_grad[1:])
-        if dys[0].is_cuda:
-            dx, *dws = ops.require_ext().linear8_bwd(
-                list(dys), codes, scales, weights, need_dx, need_dw)
-        else:
-            dx, dws = _linear8_backward_cpu(dys, codes, scales, weights,
-                                            need_dx, need_dw)
-        if not need_dw:
-            dws = [None] * len(weights)
-        return (dx if need_dx else None,
-                *(d if need else None
-                  for d, need in zip(dws, ctx.needs_input_grad[1:])))
-
-
-def _linear8_backward_cpu(dys, codes, scales, weights, need_dx, need_dw):
-    dx, dws = None, []
-    if need_dx:
-        dx = sum(_held(d) @ _held_weight(w) for d, w in zip(dys, weights))
-        dx = dx.to(dys[0].dtype)
-    if need_dw:
         x = _unpack_cpu(codes, scales, weights[0].shape[1], torch.float32)
         xt = _held(x.t())
-        dws = [(_held(d.t()) @ xt.t()).to(w.dtype)
-               for d, w in zip(dys, weights)]
-    return dx, dws
+        dx = sum(_held(d) @ _held_weight(w) for d, w in zip(dys, weights))
+        return (dx.to(dys[0].dtype),
+                *((_held(d.t()) @ xt.t()).to(w.dtype)
+                  for d, w in zip(dys, weights)))
 
 
 def linear8(x, *weights):
@@ -425,17 +366,15 @@ def linear8(x, *weights):
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("packed weights have no backward pass: call "
                                "linear8 with the weights, or under no_grad")
-        ys = _linear8_packed(_rows(x), weights[0])
+        ys = _linear8_packed(x, weights[0])
     else:
         _check_weights(weights)
         _check_input(x, weights[0].shape[1], weights[0].device)
-        if torch.is_grad_enabled() and (
-                x.requires_grad or any(w.requires_grad for w in weights)):
-            ys = _Linear8Function.apply(_rows(x), *weights)
+        if x.is_cuda:
+            ys = ops.require_ext().linear8(x, list(weights))
         else:
-            ys = _linear8_packed(_rows(x), pack_weight8(*weights))
-    if x.dim() != 2:
-        ys = tuple(y.view(*x.shape[:-1], y.shape[-1]) for y in ys)
+            ys = [y.view(*x.shape[:-1], y.shape[-1])
+                  for y in _Linear8Cpu.apply(_rows(x), *weights)]
     return tuple(ys) if len(ys) > 1 else ys[0]
 
 
@@ -454,9 +393,10 @@ def _linear8_packed(x, w):
         return ops.require_ext().linear8_packed(x, w.codes, w.scales,
                                                 w.counts, w.columns)
     values = _unpack_cpu(w.codes, w.scales, w.columns, torch.float32)
-    held, ys, at = _held(x), [], 0
+    held, ys, at = _held(_rows(x)), [], 0
     for n in w.counts:
-        ys.append((held @ values[at:at + n].t()).to(x.dtype))
+        y = (held @ values[at:at + n].t()).to(x.dtype)
+        ys.append(y.view(*x.shape[:-1], n))
         at += _up(n, BLOCK)
     return ys
 

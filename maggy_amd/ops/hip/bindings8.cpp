@@ -510,17 +510,164 @@ std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys,
   return out;
 }
 
+// ---------------------------------------------------------------- autograd
+// The graph's nodes are C++ too: a Python node costs tens of microseconds a
+// pass, more than the kernels of a small batch.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// [..., C] as a matrix, and back
+Tensor as_rows(const Tensor& t) {
+  return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+}
+Tensor as_shape(const Tensor& rows, at::IntArrayRef lead) {
+  if (lead.size() == 1) return rows;
+  auto shape = lead.vec();
+  shape.push_back(rows.size(1));
+  return rows.view(shape);
+}
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+void no_second_derivative(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name,
+              " has no second derivative: backward cannot create a graph");
+}
+
+struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
+  static Tensor forward(AutogradContext* ctx, Tensor g, Tensor u) {
+    auto out = swiglu8_fwd(g, u, true);
+    ctx->save_for_backward({out[1], out[2], out[3], out[4]});
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dh) {
+    no_second_derivative("swiglu8");
+    const auto k = ctx->get_saved_variables();
+    return swiglu8_bwd(dh[0], k[0], k[1], k[2], k[3]);
+  }
+};
+
+Tensor swiglu8(Tensor g, Tensor u) {
+  const auto lead = g.sizes().slice(0, g.dim() - 1).vec();
+  g = as_rows(g);
+  u = as_rows(u);
+  return as_shape(wants_grad({&g, &u}) ? SwiGLU8::apply(g, u)
+                                       : swiglu8_fwd(g, u, false)[0],
+                  lead);
+}
+
+struct RMSNorm8 : torch::autograd::Function<RMSNorm8> {
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w,
+                        double eps) {
+    auto out = rms8_fwd(x, w, eps, true);
+    ctx->save_for_backward({out[1], out[2], out[3], w});
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    no_second_derivative("rms_norm8");
+    const auto k = ctx->get_saved_variables();
+    auto d = rms8_bwd(dy[0], k[0], k[1], k[3], k[2],
+                      ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    return {d[0].value_or(Tensor()), d[1].value_or(Tensor()), Tensor()};
+  }
+};
+
+Tensor rms_norm8(Tensor x, Tensor w, double eps) {
+  const auto lead = x.sizes().slice(0, x.dim() - 1).vec();
+  x = as_rows(x);
+  return as_shape(wants_grad({&x, &w}) ? RMSNorm8::apply(x, w, eps)
+                                       : rms8_fwd(x, w, eps, false)[0],
+                  lead);
+}
+
+static_assert(b8::kMaxParts == 4);
+struct Linear8 : torch::autograd::Function<Linear8> {
+  using Maybe = c10::optional<Tensor>;
+  static variable_list forward(AutogradContext* ctx, Tensor x, Tensor w0,
+                               Maybe w1, Maybe w2, Maybe w3) {
+    variable_list weights{w0};
+    for (const Maybe& w : {w1, w2, w3})
+      if (w) weights.push_back(*w);
+    auto out = linear8_fwd(x, weights);
+    bool dw = false;
+    for (const Tensor& w : weights) dw = dw || w.requires_grad();
+    variable_list kept(weights);
+    // dX does not read x
+    kept.push_back(dw ? out[weights.size()] : Tensor());
+    kept.push_back(dw ? out[weights.size() + 1] : Tensor());
+    ctx->save_for_backward(kept);
+    out.resize(weights.size());
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dys) {
+    no_second_derivative("linear8");
+    auto kept = ctx->get_saved_variables();
+    const size_t n = kept.size() - 2;
+    c10::optional<Tensor> codes, scales;
+    if (kept[n].defined()) codes = kept[n], scales = kept[n + 1];
+    kept.resize(n);
+    bool need_dw = false;
+    for (size_t i = 0; i < n; ++i)
+      need_dw = need_dw || ctx->needs_input_grad(1 + i);
+    auto d = linear8_bwd(dys, codes, scales, kept, ctx->needs_input_grad(0),
+                         need_dw);
+    d.resize(1 + b8::kMaxParts);
+    for (size_t i = 0; i < n; ++i)
+      if (!ctx->needs_input_grad(1 + i)) d[1 + i] = Tensor();
+    return d;
+  }
+};
+
+std::vector<Tensor> linear8(Tensor x, std::vector<Tensor> weights) {
+  const auto lead = x.sizes().slice(0, x.dim() - 1).vec();
+  x = as_rows(x);
+  bool grad = wants_grad({&x});
+  for (const Tensor& w : weights) grad = grad || wants_grad({&w});
+  std::vector<Tensor> out;
+  if (grad) {
+    check_counts(std::vector<int64_t>(weights.size()));
+    const auto at = [&](size_t i) {
+      return i < weights.size() ? Linear8::Maybe(weights[i]) : c10::nullopt;
+    };
+    out = Linear8::apply(x, weights[0], at(1), at(2), at(3));
+  } else {
+    out = linear8_fwd(x, weights);
+    out.resize(weights.size());
+  }
+  for (Tensor& y : out) y = as_shape(y, lead);
+  return out;
+}
+
+std::vector<Tensor> linear8_on_packed(Tensor x, Tensor codes, Tensor scales,
+                                      std::vector<int64_t> counts,
+                                      int64_t K) {
+  const auto lead = x.sizes().slice(0, x.dim() - 1).vec();
+  auto out = linear8_packed(as_rows(x), codes, scales, counts, K);
+  for (Tensor& y : out) y = as_shape(y, lead);
+  return out;
+}
+
 }  // namespace
 
 void bind_block8(pybind11::module_& m) {
-  m.def("pack8", &pack8, "matrix -> 8-bit block codes and scales");
-  m.def("unpack8", &unpack8, "8-bit block codes and scales -> matrix");
-  m.def("swiglu8_fwd", &swiglu8_fwd, "silu(g)*u, g and u kept in 8 bits");
-  m.def("swiglu8_bwd", &swiglu8_bwd, "gradients of swiglu8");
-  m.def("rms8_fwd", &rms8_fwd, "RMSNorm, x kept in 8 bits");
-  m.def("rms8_bwd", &rms8_bwd, "gradients of rms_norm8");
-  m.def("pack8_weights", &pack8_weights, "stacked weights in 8 bits");
-  m.def("linear8_fwd", &linear8_fwd, "x @ W^T of 8-bit operands");
-  m.def("linear8_packed", &linear8_packed, "x @ W^T on packed weights");
-  m.def("linear8_bwd", &linear8_bwd, "gradients of linear8");
+  using release = pybind11::call_guard<pybind11::gil_scoped_release>;
+  m.def("pack8", &pack8, "matrix -> 8-bit block codes and scales",
+        release());
+  m.def("unpack8", &unpack8, "8-bit block codes and scales -> matrix",
+        release());
+  m.def("swiglu8", &swiglu8, "silu(g)*u, differentiable, g and u kept in 8 "
+        "bits", release());
+  m.def("rms_norm8", &rms_norm8, "RMSNorm, differentiable, x kept in 8 bits",
+        release());
+  m.def("pack8_weights", &pack8_weights, "stacked weights in 8 bits",
+        release());
+  m.def("linear8", &linear8, "x @ W^T of 8-bit operands, differentiable",
+        release());
+  m.def("linear8_packed", &linear8_on_packed, "x @ W^T on packed weights",
+        release());
 }

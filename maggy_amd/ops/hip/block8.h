@@ -56,31 +56,51 @@ struct Fp32 {
 // Loads columns [c, c + 8) of a row; columns from C on read as zero.  VEC:
 // the host has checked that C, the row stride and the base allow 16-byte
 // loads, so a group of 8 lies inside the row or outside as a whole.
+struct Eight {
+  u32x4 a, b;  // 16-bit types use a only
+};
+
 template <class T, bool VEC>
-__device__ __forceinline__ void load8(const typename T::raw* row, int c,
-                                      int C, float (&v)[8]) {
+__device__ __forceinline__ Eight load8_raw(const typename T::raw* row, int c,
+                                           int C) {
+  Eight e{{0, 0, 0, 0}, {0, 0, 0, 0}};
   if constexpr (VEC) {
     if (c < C) {
-      if constexpr (sizeof(typename T::raw) == 2) {
-        const u32x4 d = *(const u32x4*)(row + c);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i] = T::to_f((uint16_t)(d[i >> 1] >> (16 * (i & 1))));
-      } else {
-        const f32x4 a = *(const f32x4*)(row + c);
-        const f32x4 b = *(const f32x4*)(row + c + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      e.a = *(const u32x4*)(row + c);
+      if constexpr (sizeof(typename T::raw) == 4)
+        e.b = *(const u32x4*)(row + c + 4);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = c + i < C ? T::to_f(row[c + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      if (c + i >= C) continue;
+      if constexpr (sizeof(typename T::raw) == 2)
+        e.a[i >> 1] |= (uint32_t)row[c + i] << (16 * (i & 1));
+      else
+        (i < 4 ? e.a : e.b)[i & 3] =
+            __builtin_bit_cast(uint32_t, (float)row[c + i]);
+    }
   }
+  return e;
+}
+
+template <class T>
+__device__ __forceinline__ void widen(const Eight& e, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(typename T::raw) == 2) {
+      v[i] = T::to_f((uint16_t)(e.a[i >> 1] >> (16 * (i & 1))));
+    } else {
+      const uint32_t bits = i < 4 ? e.a[i & 3] : e.b[i & 3];
+      v[i] = __builtin_bit_cast(float, bits);
+    }
+  }
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const typename T::raw* row, int c,
+                                      int C, float (&v)[8]) {
+  widen<T>(load8_raw<T, VEC>(row, c, C), v);
 }
 
 template <class T, bool VEC>

@@ -337,7 +337,8 @@ __global__ __launch_bounds__(kThreads) void rms_fwd(
 // dw: every wave adds up its rows in registers and writes one row of
 // partials; the fold sums them in a fixed order, so results repeat.
 template <class T, bool VEC, int WPR, int NI>
-__global__ __launch_bounds__(kThreads) void rms_bwd(
+__global__ __launch_bounds__(kThreads, NI <= 2 ? 4 : NI <= 4 ? 2 : 1) void
+rms_bwd(
     const typename T::raw* __restrict__ dy, long long ldy,
     const uint8_t* __restrict__ codes, int Cp,
     const uint32_t* __restrict__ scales, long long Rp,
@@ -357,22 +358,42 @@ __global__ __launch_bounds__(kThreads) void rms_bwd(
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
   }
-  int parity = 0;
-  for (long long r = first; r < R; r += step, parity ^= 1) {
-    float n[NI][8], d[NI][8], sum = 0.f;
-    const float inv = inv_rms[r];
+  // the next row's loads are under way while this row is summed; 8 * 8
+  // values a lane leave no registers for that
+  constexpr bool kAhead = NI <= 4;
+  struct Row {
+    Eight d[NI];
+    u32x2 code[NI];
+    uint32_t E[NI];
+    float inv;
+  };
+  auto load_row = [&](long long r, Row& row) {
+    row.inv = inv_rms[r];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int q = q0 + i * WPR, c = q * 512 + lane * 8;
-      load8<T, VEC>(dy + r * ldy, c, C, d[i]);
-      u32x2 code = {0, 0};
-      uint32_t E = 1;
+      row.d[i] = load8_raw<T, VEC>(dy + r * ldy, c, C);
+      row.code[i] = u32x2{0, 0};
+      row.E[i] = 1;
       if (c < Cp) {
-        code = *(const u32x2*)code_at(codes, R, r, c);
-        E = scales[q * Rp + r] >> (8 * (lane >> 4)) & 255u;
+        row.code[i] = *(const u32x2*)code_at(codes, R, r, c);
+        row.E[i] = scales[q * Rp + r] >> (8 * (lane >> 4)) & 255u;
       }
-      decode8(code, scale_value(E), n[i]);
     }
+  };
+  Row ahead;
+  if (kAhead && first < R) load_row(first, ahead);
+  int parity = 0;
+  for (long long r = first; r < R; r += step, parity ^= 1) {
+    float n[NI][8], d[NI][8], sum = 0.f;
+    if (!kAhead) load_row(r, ahead);
+    const float inv = ahead.inv;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      widen<T>(ahead.d[i], d[i]);
+      decode8(ahead.code[i], scale_value(ahead.E[i]), n[i]);
+    }
+    if (kAhead) load_row(r + step < R ? r + step : r, ahead);
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -410,8 +431,10 @@ __global__ __launch_bounds__(1024) void fold_rows(
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + lane;
   float s = 0.f;
-  if (c < C)
+  if (c < C) {
+#pragma unroll 8
     for (int p = wave; p < P; p += 16) s += partials[(long long)p * C + c];
+  }
   part[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && c < C) {
@@ -577,7 +600,12 @@ extern "C" void launch_b8_rms_fwd(int dtype, int vec, const void* x,
 // the workgroups of the backward pass, and the rows of partials they write
 extern "C" int b8_rms_bwd_blocks(long long R, int C) {
   const long long groups = C <= 2048 ? (R + 3) / 4 : R;
-  return (int)(groups < 512 ? groups : 512);
+#ifdef RB
+  const int most = RB;
+#else
+  const int most = C <= 1024 || (C > 2048 && C <= 4096) ? 1024 : 512;
+#endif
+  return (int)(groups < most ? groups : most);
 }
 extern "C" int b8_rms_bwd_partials(long long R, int C) {
   return b8_rms_bwd_blocks(R, C) * (C <= 2048 ? 4 : 1);

@@ -498,3 +498,50 @@ def test_gpu_refusals():
     wide = torch.zeros(1, 16385, device="cuda")
     with pytest.raises(RuntimeError):
         ops.rms_norm8(wide, torch.ones(16385, device="cuda"))
+
+
+def test_second_derivatives_are_refused():
+    x = _normal((4, 32), 1).requires_grad_(True)
+    w = _normal((8, 32), 2).requires_grad_(True)
+    n = torch.ones(32, device="cuda", requires_grad=True)
+    for y in (ops.linear8(x, w), ops.swiglu8(x, x), ops.rms_norm8(x, n)):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(y.float().sum(), x, create_graph=True)
+
+
+def test_gradients_of_shared_and_expanded_inputs():
+    """The same tensor twice, a broadcast input, the same weight twice."""
+    x = _normal((5, 200), 1).requires_grad_(True)
+    ops.swiglu8(x, x).backward(torch.ones_like(x))
+    (_, _), (dg, bg), (du, bu) = oracle.swiglu(
+        x.detach(), x.detach(), torch.ones_like(x))
+    # each part is rounded to bf16 before autograd adds them
+    oracle.assert_within(x.grad, dg + du,
+                         bg + bu + (dg.abs() + du.abs()) * 2.0 ** -8)
+    row = _normal((1, 200), 2).requires_grad_(True)
+    w = _normal((60, 200), 3, 0.1).requires_grad_(True)
+    dy = _normal((7, 60), 4)
+    wide = row.expand(7, 200)
+    wide.retain_grad()
+    y = ops.linear8(wide, w)
+    y.backward(dy)
+    want_y, want_dx, want_dw = oracle.linear(
+        row.detach().expand(7, 200), [w.detach()], [dy])
+    oracle.assert_within(y, *want_y[0])
+    oracle.assert_within(wide.grad, *want_dx)
+    oracle.assert_within(w.grad, *want_dw[0])
+    # the same weight twice: both outputs are equal, the gradients add
+    a, b = ops.linear8(row, w, w)
+    assert torch.equal(a, b)
+    ga, = torch.autograd.grad(a, w, dy[:1], retain_graph=False)
+    assert ga.shape == w.shape
+
+
+def test_weights_changed_before_backward_are_noticed():
+    x = _normal((4, 32), 1).requires_grad_(True)
+    w = _normal((8, 32), 2).requires_grad_(True)
+    y = ops.linear8(x, w)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
