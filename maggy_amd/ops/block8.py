@@ -296,6 +296,9 @@ def _check_weights(weights):
             MAX_WEIGHTS, len(weights)))
     first = weights[0]
     for w in weights:
+        if isinstance(w, Weight8):
+            raise TypeError("pack weights that share an input together: "
+                            "pack_weight8(w1, w2, ...)")
         _check_float(w, "weight")
         if w.dim() != 2 or w.shape[0] == 0:
             raise ValueError("a weight must be [N, K], got {}".format(
@@ -358,15 +361,17 @@ def linear8(x, *weights):
     _check_float(x, "x")
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         x = x.to(torch.get_autocast_dtype("cuda"))
-    if any(isinstance(w, Weight8) for w in weights):
-        if len(weights) > 1:
-            raise TypeError("pack weights that share an input together: "
-                            "pack_weight8(w1, w2, ...)")
-        _check_input(x, weights[0].columns, weights[0].device)
-        if torch.is_grad_enabled() and x.requires_grad:
+    if len(weights) == 1 and isinstance(weights[0], Weight8):
+        w, = weights
+        _check_input(x, w.columns, w.device)
+        if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("packed weights have no backward pass: call "
                                "linear8 with the weights, or under no_grad")
-        ys = _linear8_packed(x, weights[0])
+        if x.is_cuda:
+            ys = ops.require_ext().linear8_packed(x, w.codes, w.scales,
+                                                  w.counts, w.columns)
+        else:
+            ys = _linear8_packed_cpu(x, w)
     else:
         _check_weights(weights)
         _check_input(x, weights[0].shape[1], weights[0].device)
@@ -387,11 +392,7 @@ def _check_input(x, K, device):
             x.dtype))
 
 
-@torch.no_grad()
-def _linear8_packed(x, w):
-    if x.is_cuda:
-        return ops.require_ext().linear8_packed(x, w.codes, w.scales,
-                                                w.counts, w.columns)
+def _linear8_packed_cpu(x, w):
     values = _unpack_cpu(w.codes, w.scales, w.columns, torch.float32)
     held, ys, at = _held(_rows(x)), [], 0
     for n in w.counts:

@@ -257,56 +257,105 @@ void check_counts(const std::vector<int64_t>& counts) {
               counts.size());
 }
 
-enum Tiles {
-  kBoth = 0,
-  kCols = 1,
-  kOneRows = 2,
-  kOneCols = 3,
-  kFrom8 = 4,
-  kRows = 5
+// A packed matrix in memory that a tensor somewhere owns
+struct Mat8 {
+  uint8_t* c = nullptr;
+  uint32_t* s = nullptr;
+  int64_t rows = 0, Cp = 0, Rp = 0;
+  int64_t code_bytes() const { return up(rows * Cp, 256); }
+  int64_t scale_bytes() const { return up((Cp + 511) / 512 * Rp * 4, 256); }
 };
-
-// packs t by 128 x 128 tiles into rows and/or into the transposed cols, its
-// first value landing at row r0 and column c0 of each
-void run_tiles(Tiles what, const Tensor& t, Packed* rows, int64_t row_r0,
-               int64_t row_c0, Packed* cols, int64_t col_r0,
-               int64_t col_c0) {
-  const bool by_rows = what == kBoth || what == kOneRows || what == kRows;
-  const bool by_cols = what == kBoth || what == kOneCols || what == kCols;
-  TORCH_CHECK(by_rows == (rows != nullptr) && by_cols == (cols != nullptr),
-              "run_tiles: outputs do not match the kernel");
-  b8::TileArgs a{};
-  a.x = t.data_ptr();
-  a.ldx = ld(t);
-  a.R = t.size(0);
-  a.C = (int)t.size(1);
-  if (rows) {
-    a.row_codes = rows->c();
-    a.row_scales = (uint8_t*)rows->s();
-    a.row_n = rows->rows();
-    a.row_sp = rows->Rp();
-    a.row_r0 = row_r0;
-    a.row_c0 = row_c0;
-  }
-  if (cols) {
-    a.col_codes = cols->c();
-    a.col_scales = (uint8_t*)cols->s();
-    a.col_n = cols->rows();
-    a.col_sp = cols->Rp();
-    a.col_r0 = col_r0;
-    a.col_c0 = col_c0;
-  }
-  TORCH_CHECK((a.R + 127) / 128 * ((a.C + 127) / 128) < (int64_t)1 << 31,
-              "matrix is too large");
-  launch_b8_tiles(what, type_of(t, "matrix"), vec8(t), &a, stream_of(t));
+Mat8 mat8(const Packed& p) {
+  return {p.c(), p.s(), p.rows(), p.Cp(), p.Rp()};
 }
 
-Packed pack_stacked(const std::vector<Tensor>& ws,
-                    const std::vector<int64_t>& first) {
-  Packed p = new_packed(first.back(), ws[0].size(1), ws[0]);
+// temporaries of one call, in one allocation
+struct Arena {
+  std::vector<Mat8*> mats;
+  void want(Mat8* m, int64_t rows, int64_t C) {
+    *m = Mat8{nullptr, nullptr, rows, up(C, 128), up(rows, 256)};
+    mats.push_back(m);
+  }
+  Tensor take(const Tensor& like) {
+    int64_t bytes = 0;
+    for (Mat8* m : mats) bytes += m->code_bytes() + m->scale_bytes();
+    Tensor space = torch::empty(
+        {bytes}, like.options().dtype(torch::kUInt8).requires_grad(false));
+    uint8_t* at = space.data_ptr<uint8_t>();
+    for (Mat8* m : mats) {
+      m->c = at;
+      m->s = (uint32_t*)(at + m->code_bytes());
+      at += m->code_bytes() + m->scale_bytes();
+    }
+    return space;
+  }
+};
+
+// The packing that a call needs, in one launch.  A job's outputs start at
+// (row_r0, row_c0) of rows and at (col_r0, col_c0) of cols.
+struct Jobs {
+  b8::TileJobs jobs{};
+
+  b8::TileJob& add(b8::TileKind kind, const Mat8* rows, int64_t row_r0,
+                   int64_t row_c0, const Mat8* cols, int64_t col_r0,
+                   int64_t col_c0) {
+    const bool by_rows = kind == b8::kTileBoth || kind == b8::kTileRows ||
+                         kind == b8::kTileOneRows;
+    TORCH_CHECK(by_rows == (rows != nullptr) &&
+                    (kind == b8::kTileBoth || !by_rows) == (cols != nullptr),
+                "linear8: outputs do not match the job");
+    TORCH_CHECK(jobs.count < b8::kMaxJobs, "linear8: too many matrices");
+    b8::TileJob& a = jobs.job[jobs.count++];
+    a.kind = kind;
+    if (rows) {
+      a.row_codes = rows->c;
+      a.row_scales = (uint8_t*)rows->s;
+      a.row_n = rows->rows;
+      a.row_sp = rows->Rp;
+      a.row_r0 = row_r0;
+      a.row_c0 = row_c0;
+    }
+    if (cols) {
+      a.col_codes = cols->c;
+      a.col_scales = (uint8_t*)cols->s;
+      a.col_n = cols->rows;
+      a.col_sp = cols->Rp;
+      a.col_r0 = col_r0;
+      a.col_c0 = col_c0;
+    }
+    return a;
+  }
+  void plain(const Tensor& t, b8::TileJob& a) {
+    a.x = t.data_ptr();
+    a.ldx = ld(t);
+    a.R = (int)t.size(0);
+    a.C = (int)t.size(1);
+    a.dtype = type_of(t, "matrix");
+    a.vec = vec8(t);
+    const bool weight =
+        a.kind == b8::kTileOneRows || a.kind == b8::kTileOneCols;
+    TORCH_CHECK(a.dtype == 0 || (weight && a.dtype == 2),
+                "linear8: no packing of ", t.scalar_type());
+  }
+  void packed(const Mat8& m, b8::TileJob& a) {
+    a.x = m.c;
+    a.xs = m.s;
+    a.ldx = m.rows;
+    a.xsp = m.Rp;
+    a.R = (int)m.rows;
+    a.C = (int)m.Cp;
+  }
+  void run(hipStream_t st) {
+    TORCH_CHECK(launch_b8_tiles(&jobs, st), "linear8: matrix is too large");
+  }
+};
+
+// the weights' rows one below the other
+void stack_weights(Jobs& jobs, const std::vector<Tensor>& ws,
+                   const std::vector<int64_t>& first, const Mat8& to) {
   for (size_t i = 0; i < ws.size(); ++i)
-    run_tiles(kOneRows, ws[i], &p, first[i], 0, nullptr, 0, 0);
-  return p;
+    jobs.plain(ws[i], jobs.add(b8::kTileOneRows, &to, first[i], 0, nullptr, 0,
+                               0));
 }
 
 std::vector<Tensor> weights_of(const std::vector<Tensor>& weights,
@@ -328,30 +377,32 @@ std::vector<Tensor> weights_of(const std::vector<Tensor>& weights,
 }
 
 // the product of packed w with x, packed (M rows) or, for a few rows, plain
-// bf16 that the kernel packs on the way
-b8::GemmArgs gemm_args(const Packed& w, int64_t M,
+// bf16 that the kernel packs on the way; like: a tensor of their device
+b8::GemmArgs gemm_args(const Mat8& w, int64_t M,
                        const std::vector<int64_t>& counts,
-                       torch::ScalarType dtype, std::vector<Tensor>* out) {
+                       torch::ScalarType dtype, const Tensor& like,
+                       std::vector<Tensor>* out) {
   const auto first = firsts(counts);
   TORCH_CHECK(M < (int64_t)1 << 30 && first.back() < (int64_t)1 << 30,
               "linear8: too many rows");
   // the kernel reaches a matrix's scales by 32-bit offsets
-  TORCH_CHECK(w.scales.numel() < (int64_t)1 << 31 &&
-                  w.scales.size(0) * up(M, 256) * 4 < (int64_t)1 << 31,
+  const int64_t quads = (w.Cp + 511) / 512;
+  TORCH_CHECK(quads * w.Rp * 4 < (int64_t)1 << 31 &&
+                  quads * up(M, 256) * 4 < (int64_t)1 << 31,
               "linear8: matrix is too large");
   b8::GemmArgs a{};
-  a.w = w.c();
-  a.ws = w.s();
-  a.wn = w.rows();
-  a.wsp = w.Rp();
+  a.w = w.c;
+  a.ws = w.s;
+  a.wn = w.rows;
+  a.wsp = w.Rp;
   a.M = (int)M;
-  a.N = (int)std::min(first.back(), w.rows());
-  a.KT = (int)(w.Cp() / 128);
+  a.N = (int)std::min(first.back(), w.rows);
+  a.KT = (int)(w.Cp / 128);
   a.parts = (int)counts.size();
   a.f32 = dtype == torch::kFloat32;
+  const auto o = like.options().dtype(dtype).requires_grad(false);
   for (size_t i = 0; i < counts.size(); ++i) {
-    out->push_back(
-        torch::empty({M, counts[i]}, w.codes.options().dtype(dtype)));
+    out->push_back(torch::empty({M, counts[i]}, o));
     a.out[i] = (*out)[i].data_ptr();
     a.first[i] = (int)first[i];
     a.count[i] = (int)counts[i];
@@ -359,22 +410,25 @@ b8::GemmArgs gemm_args(const Packed& w, int64_t M,
   return a;
 }
 
-std::vector<Tensor> product(const Packed& x, const Packed& w, int64_t M,
+std::vector<Tensor> product(const Mat8& x, const Mat8& w, int64_t M,
                             const std::vector<int64_t>& counts,
-                            torch::ScalarType dtype) {
-  TORCH_CHECK(x.Cp() == w.Cp(), "linear8: columns do not match");
+                            torch::ScalarType dtype, const Tensor& like) {
+  TORCH_CHECK(x.Cp == w.Cp && M <= x.rows, "linear8: columns do not match");
   std::vector<Tensor> out;
-  b8::GemmArgs a = gemm_args(w, M, counts, dtype, &out);
-  a.x = x.c();
-  a.xs = x.s();
-  a.xn = x.rows();
-  a.xsp = x.Rp();
+  b8::GemmArgs a = gemm_args(w, M, counts, dtype, like, &out);
+  a.x = x.c;
+  a.xs = x.s;
+  a.xn = x.rows;
+  a.xsp = x.Rp;
   if (M) {
     const long long bytes = b8_gemm_workspace(&a);
     Tensor space;
-    if (bytes) space = torch::empty({bytes}, x.codes.options());
+    if (bytes)
+      space = torch::empty({bytes}, like.options()
+                                        .dtype(torch::kUInt8)
+                                        .requires_grad(false));
     launch_b8_gemm(&a, bytes ? (float*)space.data_ptr() : nullptr,
-                   stream_of(x.codes));
+                   stream_of(like));
   }
   return out;
 }
@@ -389,7 +443,11 @@ std::vector<Tensor> pack8_weights(std::vector<Tensor> weights) {
   std::vector<int64_t> counts;
   const auto ws = weights_of(weights, &counts);
   const CUDAGuard guard(ws[0].device());
-  const Packed p = pack_stacked(ws, firsts(counts));
+  const auto first = firsts(counts);
+  const Packed p = new_packed(first.back(), ws[0].size(1), ws[0]);
+  Jobs jobs;
+  stack_weights(jobs, ws, first, mat8(p));
+  jobs.run(stream_of(ws[0]));
   return {p.codes, p.scales};
 }
 
@@ -403,9 +461,19 @@ std::vector<Tensor> linear8_fwd(Tensor x, std::vector<Tensor> weights) {
               " columns, the weights ", ws[0].size(1));
   same_device(x, ws[0], "weight");
   const CUDAGuard guard(x.device());
-  const Packed p = pack_rows(x);
-  auto out = product(p, pack_stacked(ws, firsts(counts)), x.size(0), counts,
-                     torch::kBFloat16);
+  const auto first = firsts(counts);
+  const Packed p = new_packed(x.size(0), x.size(1), x);
+  const Mat8 held = mat8(p);
+  Mat8 w;
+  Arena arena;
+  arena.want(&w, first.back(), x.size(1));
+  const Tensor space = arena.take(x);
+  Jobs jobs;
+  if (x.size(0))
+    jobs.plain(x, jobs.add(b8::kTileRows, &held, 0, 0, nullptr, 0, 0));
+  stack_weights(jobs, ws, first, w);
+  jobs.run(stream_of(x));
+  auto out = product(held, w, x.size(0), counts, torch::kBFloat16, x);
   out.push_back(p.codes);
   out.push_back(p.scales);
   return out;
@@ -427,11 +495,12 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
   const int64_t M = x.size(0);
   if (M >= 1 && M <= 16 && vec8(x)) {
     std::vector<Tensor> out;
-    const b8::GemmArgs a = gemm_args(w, M, counts, torch::kBFloat16, &out);
+    const b8::GemmArgs a =
+        gemm_args(mat8(w), M, counts, torch::kBFloat16, x, &out);
     launch_b8_gemm_bf16(&a, x.data_ptr(), ld(x), (int)K, stream_of(x));
     return out;
   }
-  return product(pack_rows(x), w, M, counts, torch::kBFloat16);
+  return product(mat8(pack_rows(x)), mat8(w), M, counts, torch::kBFloat16, x);
 }
 
 // dx and one dw a weight; dx empty or no dw where they are not asked for
@@ -461,45 +530,49 @@ std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys,
       for (int64_t n : counts) out.push_back(torch::zeros({n, K}, o));
     return out;
   }
-  Packed rows, cols;
-  if (need_dx) rows = new_packed(M, N, dys[0]);
-  if (need_dw) cols = new_packed(N, M, dys[0]);
-  if (need_dx || need_dw)
-    for (size_t i = 0; i < dys.size(); ++i)
-      run_tiles(need_dx && need_dw ? kBoth : need_dx ? kRows : kCols, dys[i],
-                need_dx ? &rows : nullptr, 0, first[i],
-                need_dw ? &cols : nullptr, first[i], 0);
+  // dY by rows for dX and by columns for dW; W^T [K][N], each weight's
+  // columns side by side; x^T from the codes that were kept
+  Mat8 rows, cols, wt, xt, x;
+  Arena arena;
   if (need_dx) {
-    // W^T, [K][N]: each weight's columns side by side
-    Packed wt = new_packed(up(K, 128), N, ws[0]);
-    for (size_t i = 0; i < ws.size(); ++i)
-      run_tiles(kOneCols, ws[i], nullptr, 0, 0, &wt, 0, first[i]);
-    out[0] = product(rows, wt, M, {K}, torch::kBFloat16)[0];
+    arena.want(&rows, M, N);
+    arena.want(&wt, up(K, 128), N);
   }
   if (need_dw) {
     TORCH_CHECK(codes && scales, "linear8: nothing was kept of x");
-    const Packed x = packed(*codes, *scales, "linear8");
-    TORCH_CHECK(x.rows() == M && x.Cp() == up(K, 128),
+    const Packed kept = packed(*codes, *scales, "linear8");
+    TORCH_CHECK(kept.rows() == M && kept.Cp() == up(K, 128),
                 "linear8: the gradient does not fit what was kept");
-    same_device(ws[0], x.codes, "x");
-    Packed xt = new_packed(x.Cp(), M, x.codes);
-    b8::TileArgs a{};
-    a.x = x.c();
-    a.xs = x.s();
-    a.ldx = x.rows();
-    a.xsp = x.Rp();
-    a.R = M;
-    a.C = (int)x.Cp();
-    a.col_codes = xt.c();
-    a.col_scales = (uint8_t*)xt.s();
-    a.col_n = xt.rows();
-    a.col_sp = xt.Rp();
-    launch_b8_tiles(kFrom8, 2, 0, &a, stream_of(x.codes));
-    // dW [N][K], all weights' rows in one product; the weights' own rows of
-    // it are contiguous
+    same_device(ws[0], kept.codes, "x");
+    x = mat8(kept);
+    arena.want(&cols, N, M);
+    arena.want(&xt, x.Cp, M);
+  }
+  if (!need_dx && !need_dw) return out;
+  const Tensor space = arena.take(ws[0]);
+  Jobs jobs;
+  for (size_t i = 0; i < dys.size(); ++i)
+    jobs.plain(dys[i],
+               jobs.add(need_dx && need_dw ? b8::kTileBoth
+                        : need_dx          ? b8::kTileRows
+                                           : b8::kTileCols,
+                        need_dx ? &rows : nullptr, 0, first[i],
+                        need_dw ? &cols : nullptr, first[i], 0));
+  if (need_dx)
+    for (size_t i = 0; i < ws.size(); ++i)
+      jobs.plain(ws[i], jobs.add(b8::kTileOneCols, nullptr, 0, 0, &wt, 0,
+                                 first[i]));
+  if (need_dw)
+    jobs.packed(x, jobs.add(b8::kTileFrom8, nullptr, 0, 0, &xt, 0, 0));
+  jobs.run(stream_of(ws[0]));
+  if (need_dx)
+    out[0] = product(rows, wt, M, {K}, torch::kBFloat16, ws[0])[0];
+  if (need_dw) {
+    // dW [N][K], all weights' rows in one product; a weight's own rows of it
+    // are contiguous
     const Tensor all = product(cols, xt, first[counts.size() - 1] +
                                              counts.back(),
-                               {K}, ws[0].scalar_type())[0];
+                               {K}, ws[0].scalar_type(), ws[0])[0];
     for (size_t i = 0; i < counts.size(); ++i)
       out.push_back(counts.size() == 1
                         ? all

@@ -180,6 +180,14 @@ __device__ __forceinline__ uint32_t max16(uint32_t x) {
   return max(x, ror<1>(x));
 }
 
+// the maximum over lanes l, l ^ 16, l ^ 32 and l ^ 48, in all of them
+__device__ __forceinline__ uint32_t max_rows(uint32_t x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max(b[0], b[1]);
+}
+
 // A wave holds 512 columns of one row, 8 a lane, so 16 lanes hold a block:
 // their scales, gathered into the dword (q, row) of the format.
 __device__ __forceinline__ uint32_t gather_scales(uint32_t E) {

@@ -69,21 +69,30 @@ __global__ __launch_bounds__(kThreads) void unpack_rows(
 
 // --------------------------------------------- 128 x 128 tiles, transposed
 // Reads a 128 x 128 tile once and writes its codes by rows (blocks along the
-// columns), by columns ([C][Rp] codes, blocks along the rows) or both.  With
+// columns), by columns (the transpose, blocks along the rows) or both.  With
 // ONE_SCALE the whole tile shares one scale, so that both orders stand for
 // the same values.  FROM8 reads a packed matrix instead of plain numbers.
 //
 // 512 threads: thread (cg, rg) = (t % 16, t / 16) holds 8 columns of 4
 // neighbouring rows, so that four rows of one column make one dword of the
 // transposed codes, and 16 lanes (one DPP row) hold a whole row of the tile.
-template <class T, bool VEC, bool FROM8, bool ONE_SCALE, bool ROWS, bool COLS>
-__global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
-  constexpr int kPitch = 33;  // dwords a transposed row of 128 codes
-  __shared__ uint32_t turned[COLS ? 128 * kPitch : 1];
-  __shared__ uint32_t tops[8][128];
+struct TileSpace {
+  static constexpr int kPitch = 33;  // dwords a transposed row of 128 codes
+  uint32_t turned[128 * kPitch];
+  uint32_t tops[8][128];
+  uint32_t scales[128];
+};
+
+template <class T, bool FROM8, bool ONE_SCALE, bool ROWS, bool COLS>
+__device__ __forceinline__ void pack_tile(const TileJob& a, TileSpace& space,
+                                          int tile) {
+  constexpr int kPitch = TileSpace::kPitch;
+  uint32_t(&tops)[8][128] = space.tops;
+  uint32_t* turned = space.turned;
   const int t = threadIdx.x, cg = t & 15, rg = t >> 4, wave = t >> 6;
-  const long long tr = blockIdx.x / tiles_c;
-  const int tc = blockIdx.x % tiles_c;
+  const int tiles_c = (a.C + 127) / 128;
+  const long long tr = tile / tiles_c;
+  const int tc = tile % tiles_c;
   const long long r0 = tr * 128 + rg * 4;
   const int c0 = tc * 128 + cg * 8;
 
@@ -98,8 +107,11 @@ __global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
         decode8(*(const u32x2*)code_at((const uint8_t*)a.x, a.ldx, r, c0),
                 scale_value(E), v[i]);
       } else {
-        load8<T, VEC>((const typename T::raw*)a.x + r * a.ldx, c0, a.C,
-                      v[i]);
+        const auto* row = (const typename T::raw*)a.x + r * a.ldx;
+        if (a.vec)
+          load8<T, true>(row, c0, a.C, v[i]);
+        else
+          load8<T, false>(row, c0, a.C, v[i]);
       }
     } else {
 #pragma unroll
@@ -114,9 +126,7 @@ __global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = max(m, finite_bits(v[i][j]));
-    m = max16(m);
-    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+    m = max_rows(max16(m));
     if ((t & 63) == 0) tops[wave][0] = m;
     __syncthreads();
 #pragma unroll
@@ -142,45 +152,43 @@ __global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
   }
 
   if constexpr (COLS) {
+    const long long b = a.col_c0 / 128 + tr;
     uint32_t E[8];
     if constexpr (ONE_SCALE) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) E[j] = tile_E;
     } else {
-      uint32_t m[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        m[j] = 0;
+        uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m[j] = max(m[j], finite_bits(v[i][j]));
-        m[j] = max(m[j], (uint32_t)__shfl_xor((int)m[j], 16));
-        m[j] = max(m[j], (uint32_t)__shfl_xor((int)m[j], 32));
-      }
-      if ((t & 63) < 16) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) tops[wave][cg * 8 + j] = m[j];
+        for (int i = 0; i < 4; ++i) m = max(m, finite_bits(v[i][j]));
+        m = max_rows(m);
+        if ((t & 63) < 16) tops[wave][cg * 8 + j] = m;
       }
       __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
+    }
+    if (t < 128) {
+      uint32_t mine = tile_E;
+      if constexpr (!ONE_SCALE) {
         uint32_t top = 0;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) top = max(top, tops[w][cg * 8 + j]);
-        E[j] = scale_of(top);
+        for (int w = 0; w < 8; ++w) top = max(top, tops[w][t]);
+        space.scales[t] = mine = scale_of(top);
       }
+      a.col_scales[4 * ((b >> 2) * a.col_sp + a.col_r0 + tc * 128 + t) +
+                   (b & 3)] = (uint8_t)mine;
+    }
+    if constexpr (!ONE_SCALE) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) E[j] = space.scales[cg * 8 + j];
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float s = scale_inverse(E[j]);
       turned[(cg * 8 + j) * kPitch + rg] =
           encode4(v[0][j] * s, v[1][j] * s, v[2][j] * s, v[3][j] * s);
-    }
-    const long long b = a.col_c0 / 128 + tr;
-    if (rg == 0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        a.col_scales[4 * ((b >> 2) * a.col_sp + a.col_r0 + c0 + j) +
-                     (b & 3)] = (uint8_t)E[j];
     }
     __syncthreads();
 #pragma unroll
@@ -191,6 +199,33 @@ __global__ __launch_bounds__(512) void pack_tile(TileArgs a, int tiles_c) {
                 (b * a.col_n + a.col_r0 + tc * 128 + c) * 128 + k * 4) =
           u32x4{s[0], s[1], s[2], s[3]};
     }
+  }
+}
+
+__global__ __launch_bounds__(512) void pack_tiles(TileJobs jobs) {
+  __shared__ TileSpace space;
+  int j = 0;
+  while (j + 1 < jobs.count && (int)blockIdx.x >= jobs.job[j + 1].first_block)
+    ++j;
+  const TileJob& a = jobs.job[j];
+  const int tile = (int)blockIdx.x - a.first_block;
+  switch (a.kind) {
+    case kTileBoth:
+      return pack_tile<Bf16, false, false, true, true>(a, space, tile);
+    case kTileCols:
+      return pack_tile<Bf16, false, false, false, true>(a, space, tile);
+    case kTileRows:
+      return pack_tile<Bf16, false, false, true, false>(a, space, tile);
+    case kTileOneRows:
+      if (a.dtype)
+        return pack_tile<Fp32, false, true, true, false>(a, space, tile);
+      return pack_tile<Bf16, false, true, true, false>(a, space, tile);
+    case kTileOneCols:
+      if (a.dtype)
+        return pack_tile<Fp32, false, true, false, true>(a, space, tile);
+      return pack_tile<Bf16, false, true, false, true>(a, space, tile);
+    case kTileFrom8:
+      return pack_tile<Fp32, true, false, false, true>(a, space, tile);
   }
 }
 
@@ -527,36 +562,16 @@ extern "C" void launch_b8_unpack(int dtype, int vec, const uint8_t* codes,
                codes, Cp, scales, Rp, Q, R, C, (T::raw*)out, most)));
 }
 
-// what: 0 rows and columns by their own blocks, 1 columns only,
-//       2 one scale a tile by rows, 3 one scale a tile by columns,
-//       4 columns of a packed matrix, 5 rows only
-extern "C" void launch_b8_tiles(int what, int dtype, int vec,
-                                const TileArgs* args, hipStream_t st) {
-  const TileArgs a = *args;
-  const int tc = (a.C + 127) / 128;
-  const long long blocks = (a.R + 127) / 128 * tc;
-  if (what == 4) {
-    launch(pack_tile<Fp32, false, true, false, false, true>, blocks, 512, st, a,
-             tc);
-    return;
+extern "C" bool launch_b8_tiles(TileJobs* jobs, hipStream_t st) {
+  long long blocks = 0;
+  for (int j = 0; j < jobs->count; ++j) {
+    TileJob& a = jobs->job[j];
+    a.first_block = (int)blocks;
+    blocks += (a.R + 127ll) / 128 * ((a.C + 127ll) / 128);
+    if (blocks >= 1ll << 31) return false;
   }
-  B8_TYPED(dtype, vec, {
-    if (what == 0)
-      launch(pack_tile<T, V, false, false, true, true>, blocks, 512, st, a,
-             tc);
-    else if (what == 1)
-      launch(pack_tile<T, V, false, false, false, true>, blocks, 512, st, a,
-             tc);
-    else if (what == 2)
-      launch(pack_tile<T, V, false, true, true, false>, blocks, 512, st, a,
-             tc);
-    else if (what == 5)
-      launch(pack_tile<T, V, false, false, true, false>, blocks, 512, st, a,
-             tc);
-    else
-      launch(pack_tile<T, V, false, true, false, true>, blocks, 512, st, a,
-             tc);
-  });
+  if (blocks) launch(pack_tiles, blocks, 512, st, *jobs);
+  return true;
 }
 
 extern "C" void launch_b8_swiglu_fwd(int dtype, int vec, const void* g,

@@ -6,14 +6,26 @@
 
 namespace b8 {
 
-// one matrix through the 128 x 128 tiles (block8.hip)
-struct TileArgs {
+// What is packed of a matrix by 128 x 128 tiles (block8.hip): its rows, its
+// columns (the transpose) or both, by blocks of their own or by one scale a
+// tile, from plain numbers or from a packed matrix
+enum TileKind {
+  kTileBoth,
+  kTileCols,
+  kTileRows,
+  kTileOneRows,
+  kTileOneCols,
+  kTileFrom8,  // columns of a packed matrix
+};
+struct TileJob {
+  TileKind kind;
+  int dtype, vec;       // 0 bf16, 2 fp32; whether 16-byte loads may be used
+  int first_block;      // of the launch; a workgroup packs a tile
   const void* x;        // plain numbers, or codes
   const uint32_t* xs;   // codes: their scales
   long long ldx;        // elements a row (codes: rows of the packed matrix)
   long long xsp;        // codes: padded rows of xs
-  long long R;
-  int C;
+  int R, C;
   // outputs are packed matrices of row_n, col_n rows (scales row_sp, col_sp)
   uint8_t* row_codes;   // value (r, c) is at row row_r0 + r, column
   uint8_t* row_scales;  // row_c0 + c; the offsets are multiples of 128
@@ -27,6 +39,12 @@ struct TileArgs {
 // The rows of W are up to four matrices, each padded to a multiple of 128
 // rows; each has a contiguous output of its own.
 constexpr int kMaxParts = 4;
+// all packing that one call of linear8 needs is one launch
+constexpr int kMaxJobs = 2 * kMaxParts + 1;
+struct TileJobs {
+  TileJob job[kMaxJobs];
+  int count;
+};
 struct GemmArgs {
   const uint8_t* x;
   const uint32_t* xs;
@@ -62,8 +80,8 @@ void launch_b8_pack(int dtype, int vec, const void* x, long long ldx,
 void launch_b8_unpack(int dtype, int vec, const uint8_t* codes, int Cp,
                       const uint32_t* scales, long long Rp, long long R,
                       int C, void* out, hipStream_t st);
-void launch_b8_tiles(int what, int dtype, int vec, const b8::TileArgs* args,
-                     hipStream_t st);
+// sets the jobs' first blocks; false if there are too many tiles
+bool launch_b8_tiles(b8::TileJobs* jobs, hipStream_t st);
 void launch_b8_swiglu_fwd(int dtype, int vec, const void* g, long long ldg,
                           const void* u, long long ldu, long long R, int C,
                           void* h, uint8_t* gc, uint8_t* uc, int Cp,

@@ -402,8 +402,7 @@ __device__ __forceinline__ i32x8 pack_step(const u32x4 (&v)[4], int* scale) {
       if (a < 0x7f80u) top = max(top, a);
     }
   }
-  top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-  top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+  top = max_rows(top);
   const uint32_t E = scale_of(top << 16);
   *scale = (int)E;
   i32x8 code;
