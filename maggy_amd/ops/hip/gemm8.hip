@@ -90,11 +90,61 @@ __device__ __forceinline__ void store4(const Out& o, int m, int c, f32x4 v) {
 // card with 256 x 256.
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 
+// The work of one launch: `full` tiles as a whole, then each of the others
+// `splits` times with a share of K, whose sums go to partials.  Tiles come
+// in order of bands of four tile rows, column by column; each of the 8 XCDs
+// takes a contiguous run of that order, so that the tiles in its L2 at one
+// time are a compact block.
+struct TileWork {
+  int tiles_m, tiles_n, full, splits;
+  int items;  // full + (tiles - full) * splits
+  float* partials;
+};
+
+__device__ __forceinline__ int xcd_run(int i, int n) {
+  const int q = n / 8, r = n % 8, xcd = i % 8, idx = i / 8;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+}
+
+struct Item {
+  int m0, n0, q0, q1;  // q: quads of K steps; scale dwords stay whole
+  int partial;         // index of its partial sums, -1 for a whole tile
+};
+template <int BM, int BN>
+__device__ __forceinline__ Item item_of(const TileWork& work, int quads,
+                                        int i) {
+  constexpr int kBand = 4;
+  Item it{0, 0, 0, quads, -1};
+  int t;
+  if (i < work.full) {
+    t = xcd_run(i, work.full);
+  } else {
+    const int rest = work.tiles_m * work.tiles_n - work.full;
+    const int k = (i - work.full) % rest, split = (i - work.full) / rest;
+    t = work.full + xcd_run(k, rest);
+    if (work.splits > 1) {
+      it.q0 = (int)((long long)quads * split / work.splits);
+      it.q1 = (int)((long long)quads * (split + 1) / work.splits);
+      it.partial = (t - work.full) * work.splits + split;
+    }
+  }
+  const int band = t / (kBand * work.tiles_n);
+  const int in_band = t % (kBand * work.tiles_n);
+  const int rows = min(kBand, work.tiles_m - band * kBand);
+  it.m0 = (band * kBand + in_band % rows) * BM;
+  it.n0 = in_band / rows * BN;
+  // divisions are done in vector registers; buffer descriptors need scalars
+  it.m0 = __builtin_amdgcn_readfirstlane(it.m0);
+  it.n0 = __builtin_amdgcn_readfirstlane(it.n0);
+  it.q0 = __builtin_amdgcn_readfirstlane(it.q0);
+  it.q1 = __builtin_amdgcn_readfirstlane(it.q1);
+  it.partial = __builtin_amdgcn_readfirstlane(it.partial);
+  return it;
+}
+
 template <int FX, int FW, int NBUF>
-__global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a, int tiles_m,
-                                                    int tiles_n, int group,
-                                                    int splits,
-                                                    float* partials) {
+__global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
+                                                    TileWork work) {
   constexpr int BM = 64 * FX, BN = 64 * FW, kRows = BM + BN;
   constexpr int kTile = kRows * 128, kScales = kRows * 4;
   constexpr int kRing = NBUF <= 2 ? 2 : 4;     // quads of scales
@@ -107,31 +157,11 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a, int tiles_m,
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  // tiles in order of a band of `group` tile rows, column by column; each of
-  // the 8 XCDs takes a contiguous run of that order, so that the tiles in
-  // its L2 at one time are a compact block
-  const int tiles = tiles_m * tiles_n;
-  int t = blockIdx.x % tiles;
-  const int split = blockIdx.x / tiles;
-  {
-    const int q = tiles / 8, r = tiles % 8, xcd = t % 8, idx = t / 8;
-    t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
-  }
-  const int band = t / (group * tiles_n), in_band = t % (group * tiles_n);
-  const int rows = min(group, tiles_m - band * group);
-  // divisions are done in vector registers; buffer descriptors need scalars
-  const int m0 = __builtin_amdgcn_readfirstlane(
-      (band * group + in_band % rows) * BM);
-  const int n0 = __builtin_amdgcn_readfirstlane(in_band / rows * BN);
+  const int quads = (a.KT + 3) >> 2;
+  const Item it = item_of<BM, BN>(work, quads, blockIdx.x);
+  const int m0 = it.m0, n0 = it.n0, q0 = it.q0, q1 = it.q1;
   const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
 
-  // this split's K steps: whole quads, so that scale dwords stay whole, and
-  // at least one, as there are no more splits than quads
-  const int quads = (a.KT + 3) >> 2;
-  const int q0 = __builtin_amdgcn_readfirstlane(
-      (int)((long long)quads * split / splits));
-  const int q1 = __builtin_amdgcn_readfirstlane(
-      (int)((long long)quads * (split + 1) / splits));
   const int KT = min(4 * q1, a.KT) - 4 * q0;
 
   // Loads by buffer descriptors: rows past the end read as zero, and all
@@ -289,9 +319,19 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a, int tiles_m,
 
   // lane: row m = lane % 32 of its fragment, columns (r / 4) * 8 +
   // lane / 32 * 4 + r % 4
-  Out o = out_of(a, n0 + wn);
-  if (splits > 1)
-    o = Out{partials + (long long)split * a.M * a.N, n0 + wn, a.N, 1};
+  if (it.partial >= 0) {
+    // in the order of the registers; join_splits knows it
+    f32x4* p = (f32x4*)work.partials +
+               ((long long)it.partial * 4 + wave) * kProducts * 256 + lane;
+#pragma unroll
+    for (int i = 0; i < kProducts; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        p[(i * 4 + r) * 64] = f32x4{acc[i][4 * r], acc[i][4 * r + 1],
+                                    acc[i][4 * r + 2], acc[i][4 * r + 3]};
+    return;
+  }
+  const Out o = out_of(a, n0 + wn);
   if (o.f32 || (o.count & 7)) {
 #pragma unroll
     for (int i = 0; i < FX; ++i) {
@@ -345,20 +385,30 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a, int tiles_m,
   }
 }
 
-// the sums of the splits, in order, to the outputs; 4 columns a thread
-__global__ __launch_bounds__(256) void join_splits(GemmArgs a, int splits,
-                                                   const float* partials) {
-  const int groups = a.N / 4;  // N is a multiple of 128 where K is split
-  const long long all = (long long)a.M * groups;
-  const long long step = (long long)gridDim.x * 256;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += step) {
-    const int m = (int)(i / groups), n = (int)(i - (long long)m * groups) * 4;
-    const float* p = partials + (long long)m * a.N + n;
-    f32x4 v = *(const f32x4*)p;
-    for (int s = 1; s < splits; ++s)
-      v += *(const f32x4*)(p + (long long)s * a.M * a.N);
-    const Out o = out_of(a, n);
-    store4(o, m, o.c0, v);
+// the sums of a split tile, in the order of the splits, to the outputs: 4
+// values a thread, a wave's fragment and register group a workgroup
+template <int FX, int FW>
+__global__ __launch_bounds__(256) void join_splits(GemmArgs a,
+                                                   TileWork work) {
+  constexpr int BM = 64 * FX, BN = 64 * FW, kProducts = FX * FW;
+  const int lane = threadIdx.x & 63, r = threadIdx.x >> 6;
+  const int frag = blockIdx.x % kProducts;
+  const int wave = blockIdx.x / kProducts % 4;
+  const int rest = work.tiles_m * work.tiles_n - work.full;
+  const int k = blockIdx.x / (kProducts * 4);
+  const Item it = item_of<BM, BN>(work, (a.KT + 3) >> 2, work.full + k);
+  const f32x4* p = (const f32x4*)work.partials +
+                   (((long long)it.partial * 4 + wave) * kProducts + frag) *
+                       256 +
+                   r * 64 + lane;
+  f32x4 v = p[0];
+  for (int s = 1; s < work.splits; ++s)
+    v += p[(long long)s * 4 * kProducts * 256];
+  const int m = it.m0 + (wave >> 1) * (BM / 2) + frag / FW * 32 + (lane & 31);
+  const int wn = (wave & 1) * (BN / 2);
+  if (k < rest && m < a.M) {
+    const Out o = out_of(a, it.n0 + wn);
+    store4(o, m, o.c0 + frag % FW * 32 + r * 8 + (lane >> 5) * 4, v);
   }
 }
 
@@ -555,57 +605,68 @@ static void split_run(SplitArgs sa, hipStream_t st) {
 
 // --------------------------------------------------------------- the choice
 // Which kernel, and K split how often: the one with the least predicted
-// time.  A workgroup of gemm_tile takes fixed + steps * step us, where a
-// step is slower when the whole card computes (its power limit); one fits a
-// CU, so more than 256 go in rounds.  Measured in us (gfx950, K steps of
-// 128, one workgroup .. 256):
+// time.  A tile takes fixed + steps * step us, where a step is slower when
+// the whole card computes (its power limit); one workgroup fits a CU, so
+// more than 256 tiles go in rounds.  K is split for the tiles of the last,
+// partly filled round only.  Measured in us (gfx950, K steps of 128, one
+// workgroup .. 256; a launch's first round takes about 2 us more):
 //
 //   tile       fixed   step alone   step on a full card
-//   256 x 256   11.7      0.93          1.37
-//   128 x 256    7.9      0.62          0.85
-//   128 x 128    5.7      0.36          0.48
-//    64 x  64    4.0      0.29          0.33
+//   256 x 256    9.0      0.93          1.37
+//   128 x 256    6.5      0.62          0.85
+//   128 x 128    4.5      0.36          0.48
+//    64 x  64    3.0      0.29          0.33
 //
 // Joining the splits costs a launch, about 4 us, and their traffic at about
 // 4 TB/s.  Measured either way, in us: 24576x4096x14336 1004 by 256 x 256
 // and 1500 by 128 x 128; 2048x2048x2048 25 and 14; 1001x777x1111 18, 8.2 and
 // 6.6 by 64 x 64; 128x4096x14336 by 128 x 128 48, and 21 in four splits.
+constexpr int kCUs = 256;
+
 struct Plan {
   int kind;  // 0 256 x 256, 1 128 x 256, 2 128 x 128, 3 64 x 64, 4 gemm_split
-  int tiles_m, tiles_n, splits;
+  TileWork work;
+  long long workspace;
 };
 
 static Plan plan_of(const GemmArgs& a) {
   static const struct {
     int bm, bn;
     float fixed, alone, full;
-  } kinds[] = {{256, 256, 11.7f, 0.93f, 1.37f},
-               {128, 256, 7.9f, 0.62f, 0.85f},
-               {128, 128, 5.7f, 0.36f, 0.48f},
-               {64, 64, 4.0f, 0.29f, 0.33f}};
+  } kinds[] = {{256, 256, 9.0f, 0.93f, 1.37f},
+               {128, 256, 6.5f, 0.62f, 0.85f},
+               {128, 128, 4.5f, 0.36f, 0.48f},
+               {64, 64, 3.0f, 0.29f, 0.33f}};
   const int quads = (a.KT + 3) / 4;
   Plan best{};
   float least = 0.f;
   for (int k = 0; k < 4; ++k) {
-    const int tm = (a.M + kinds[k].bm - 1) / kinds[k].bm;
-    const int tn = (a.N + kinds[k].bn - 1) / kinds[k].bn;
+    const auto& kind = kinds[k];
+    const int tm = (a.M + kind.bm - 1) / kind.bm;
+    const int tn = (a.N + kind.bn - 1) / kind.bn;
+    const long long tiles = (long long)tm * tn;
+    const long long rest = tiles % kCUs;
+    const long long rounds = tiles / kCUs;
     for (int splits = 1; splits <= 8; splits *= 2) {
-      if (splits > 1 && quads < 2 * splits) break;
-      const long long groups = (long long)tm * tn * splits;
-      const float steps = 4.f * ((quads + splits - 1) / splits);
-      const auto round = [&](float busy) {
-        return kinds[k].fixed +
-               (splits > 1 ? steps : a.KT) *
-                   (kinds[k].alone +
-                    (kinds[k].full - kinds[k].alone) * busy);
-      };
-      float us = groups / 256 * round(1.f);
-      if (groups % 256) us += round((groups % 256) / 256.f);
+      if (splits > 1 && (quads < 2 * splits || rest == 0)) break;
+      const long long last = rest * splits;  // workgroups of the last round
+      const float steps =
+          splits > 1 ? 4.f * ((quads + splits - 1) / splits) : a.KT;
+      float us = 2.f + rounds * (kind.fixed + a.KT * kind.full);
+      us += last / kCUs * (kind.fixed + steps * kind.full);
+      if (last % kCUs)
+        us += kind.fixed + steps * (kind.alone + (kind.full - kind.alone) *
+                                               (last % kCUs) / kCUs);
       if (splits > 1)
-        us += 4.f + (4.f * splits + 2.f) * a.M * a.N / 4e6f;
+        us += 4.f + (4.f * splits + 2.f) * rest * kind.bm * kind.bn / 4e6f;
       if (least == 0.f || us < least) {
         least = us;
-        best = Plan{k, tm, tn, splits};
+        const long long full = splits > 1 ? tiles - rest : tiles;
+        const long long items = full + (tiles - full) * splits;
+        best.kind = k;
+        best.work = TileWork{tm, tn, (int)full, splits, (int)items, nullptr};
+        best.workspace =
+            splits > 1 ? 4ll * splits * rest * kind.bm * kind.bn : 0;
       }
     }
   }
@@ -613,15 +674,17 @@ static Plan plan_of(const GemmArgs& a) {
   const long long groups = (a.M + 31) / 32 * ((a.N + 15) / 16);
   const float us =
       2.3f + 2.8f * ((a.KT + 15) / 16) * (groups < 256 ? 1.f : groups / 256.f);
-  if (us < least) best = Plan{4, 0, 0, 1};
+  if (us < least) best = Plan{4};
   return best;
 }
 
 template <int FX, int FW, int NBUF>
-static void tile_run(const GemmArgs& a, const Plan& p, float* partials,
-                     hipStream_t st) {
-  launch(gemm_tile<FX, FW, NBUF>, (long long)p.tiles_m * p.tiles_n * p.splits,
-         256, st, a, p.tiles_m, p.tiles_n, 4, p.splits, partials);
+static void tile_run(const GemmArgs& a, const Plan& p, hipStream_t st) {
+  launch(gemm_tile<FX, FW, NBUF>, p.work.items, 256, st, a, p.work);
+  const long long rest =
+      (long long)p.work.tiles_m * p.work.tiles_n - p.work.full;
+  if (rest)
+    launch(join_splits<FX, FW>, rest * 4 * FX * FW, 256, st, a, p.work);
 }
 
 }  // namespace b8
@@ -629,29 +692,24 @@ static void tile_run(const GemmArgs& a, const Plan& p, float* partials,
 using namespace b8;
 
 extern "C" long long b8_gemm_workspace(const GemmArgs* args) {
-  const Plan p = plan_of(*args);
-  return p.splits > 1 ? 4ll * p.splits * args->M * args->N : 0;
+  return plan_of(*args).workspace;
 }
 
 extern "C" void launch_b8_gemm(const GemmArgs* args, float* workspace,
                                hipStream_t st) {
   const GemmArgs a = *args;
-  const Plan p = plan_of(a);
+  Plan p = plan_of(a);
+  p.work.partials = workspace;
   if (p.kind == 0)
-    tile_run<4, 4, 2>(a, p, workspace, st);
+    tile_run<4, 4, 2>(a, p, st);
   else if (p.kind == 1)
-    tile_run<2, 4, 3>(a, p, workspace, st);
+    tile_run<2, 4, 3>(a, p, st);
   else if (p.kind == 2)
-    tile_run<2, 2, 4>(a, p, workspace, st);
+    tile_run<2, 2, 4>(a, p, st);
   else if (p.kind == 3)
-    tile_run<1, 1, 8>(a, p, workspace, st);
+    tile_run<1, 1, 8>(a, p, st);
   else
     split_run<2, 1, 1, 16, false>(SplitArgs{a}, st);
-  if (p.splits > 1) {
-    const long long blocks = ((long long)a.M * a.N / 4 + 255) / 256;
-    launch(join_splits, blocks < 4096 ? blocks : 4096, 256, st, a, p.splits,
-           workspace);
-  }
 }
 
 // x in bf16, at most 16 rows of K columns, K and ldx multiples of 8, packed
