@@ -12,6 +12,7 @@ backward + fused HIP Adam step, DDP over RCCL/xGMI for N>1.
 Other modes:
     --mode asha     completed ASHA trials/hr on the trial pool (1 proc)
     --model llama8b Llama-3-8B bf16 DP step (tokens/sec)
+    --eight-bit     the Llama layers on the 8-bit block operators
 
 Rank 0 prints ONE JSON line with the whole-job aggregate.
 """
@@ -36,6 +37,8 @@ def parse_args():
     p.add_argument("--workers", type=int, default=0,
                    help="ASHA pool size (0 = one per GPU; >gpus time-slices)")
     p.add_argument("--seq-len", type=int, default=4096)
+    p.add_argument("--eight-bit", action="store_true",
+                   help="llama: the layers on the 8-bit block operators")
     p.add_argument("--graphs", action="store_true",
                    help="capture the whole train step in a hipGraph "
                         "(single-GPU)")
@@ -99,6 +102,7 @@ def make_llama_step(args, device, world, size):
 
     cfg_model = (LlamaConfig.llama3_8b() if size == "8b"
                  else LlamaConfig.small_1b())
+    cfg_model.eight_bit = args.eight_bit
     batch = args.batch or (6 if size == "8b" else 8)
     seq = args.seq_len
     # construct directly on the GPU (init kernels run on-device; 8B fp32
@@ -127,6 +131,10 @@ def make_llama_step(args, device, world, size):
 
     cfg = {"model": "llama3-{}".format(size), "global_batch": batch * world,
            "seq_len": seq, "parallelism": "dp{}".format(world)}
+    if args.eight_bit:
+        cfg["layers"] = "8-bit blocks (e4m3)"
+        return (step, batch * seq,
+                "tokens/sec (Llama-3 8-bit layers synthetic)", cfg)
     return step, batch * seq, "tokens/sec (Llama-3 bf16 synthetic)", cfg
 
 
@@ -193,7 +201,7 @@ def run_train(args):
             "higher_is_better": True,
             "scaling": "weak",
             "vs_baseline": None,
-            "dtype": "bf16",
+            "dtype": "e4m3+bf16" if args.eight_bit else "bf16",
             "data": "synthetic",
             "config": cfg,
         }))

@@ -406,24 +406,37 @@ def _linear8_packed_cpu(x, w):
 class Linear8Group:
     """Bias-free linear modules that read the same input, run as one
     ``linear8``.  ``pack`` keeps their weights packed for calls without
-    gradients, until ``drop``; it belongs after the last weight update."""
+    gradients, until ``drop``, a call with gradients (training is about to
+    change them) or a change of the weights themselves."""
 
     def __init__(self, *linears):
         for m in linears:
             if m.bias is not None:
                 raise ValueError("linear8 has no bias")
         self.linears = linears
-        self.packed = None
+        self.drop()
+
+    def _state(self):
+        return [(m.weight, m.weight._version) for m in self.linears]
 
     def pack(self):
         self.packed = pack_weight8(*(m.weight for m in self.linears))
+        self._packed_of = self._state()
 
     def drop(self):
-        self.packed = None
+        self.packed = self._packed_of = None
+
+    def _is_packed(self):
+        if torch.is_grad_enabled():
+            return False
+        return all(m.weight is w and w._version == v
+                   for m, (w, v) in zip(self.linears, self._packed_of))
 
     def __call__(self, x):
-        if self.packed is not None and not torch.is_grad_enabled():
-            return linear8(x, self.packed)
+        if self.packed is not None:
+            if self._is_packed():
+                return linear8(x, self.packed)
+            self.drop()
         return linear8(x, *(m.weight for m in self.linears))
 
 
@@ -466,8 +479,10 @@ def groups8(module):
 
 
 def pack8_model(module):
-    """Pack the weights of every 8-bit linear of a model for serving; after
-    a weight update call it again, or ``drop8_model``."""
+    """Pack the weights of every 8-bit linear of a model for serving.  A call
+    with gradients or a change of a weight drops that layer's; code that
+    writes weights behind torch's back calls this again, or
+    ``drop8_model``."""
     for g in groups8(module):
         g.pack()
 

@@ -12,6 +12,7 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 from maggy_amd.models import LlamaConfig, LlamaModel  # noqa: E402
+from maggy_amd.ops import pack8_model  # noqa: E402
 
 
 def main():
@@ -23,9 +24,12 @@ def main():
     ap.add_argument("--iters", type=int, default=3)
     ap.add_argument("--captured", action="store_true",
                     help="hipGraph-captured decode step")
+    ap.add_argument("--eight-bit", action="store_true",
+                    help="the layers on 8-bit weights, packed once")
     args = ap.parse_args()
     cfg = (LlamaConfig.llama3_8b() if args.size == "8b"
            else LlamaConfig.small_1b())
+    cfg.eight_bit = args.eight_bit
     with torch.device("cuda"):
         model = LlamaModel(cfg)
     model = model.to(torch.bfloat16).eval()
@@ -33,6 +37,8 @@ def main():
     model.rope_sin = model.rope_sin.float()
     tokens = torch.randint(0, cfg.vocab_size, (args.batch, args.prompt),
                            device="cuda")
+    if args.eight_bit:
+        pack8_model(model)
     gen = (lambda t, n: model.generate_captured(t, n)) if args.captured \
         else (lambda t, n: model.generate(t, n))
     # warmup
@@ -44,9 +50,10 @@ def main():
     torch.cuda.synchronize()
     dt = (time.perf_counter() - t0) / args.iters
     new_tok = args.batch * args.new
-    print("llama-%s decode%s: batch %d, prompt %d, %d new tokens: "
+    print("llama-%s%s decode%s: batch %d, prompt %d, %d new tokens: "
           "%.3f s -> %.0f tokens/sec decode (%.2f ms/token/batch)"
-          % (args.size, " (captured)" if args.captured else "", args.batch, args.prompt, args.new, dt,
+          % (args.size, " 8-bit" if args.eight_bit else "",
+             " (captured)" if args.captured else "", args.batch, args.prompt, args.new, dt,
              new_tok / dt, dt / args.new * 1e3))
 
 

@@ -197,10 +197,19 @@ def test_module_packs_and_drops():
         before = lin(x)
         ops.pack8_model(lin)
         assert torch.equal(lin(x), before)
-        lin.weight.mul_(2)
-        assert torch.equal(lin(x), before)  # packed weights stay
+        assert lin.group.packed is not None
         ops.drop8_model(lin)
+        assert lin.group.packed is None
+        ops.pack8_model(lin)
+        lin.weight.mul_(2)  # a changed weight is noticed
         assert torch.equal(lin(x), before * 2)
+        assert lin.group.packed is None
+        ops.pack8_model(lin)
+        lin.weight = torch.nn.Parameter(lin.weight.detach() / 2)
+        assert torch.equal(lin(x), before)
+        ops.pack8_model(lin)
+    lin(x)  # with gradients: the weights are about to change
+    assert lin.group.packed is None
     with pytest.raises(ValueError):
         from maggy_amd.ops.block8 import Linear8Group
 
