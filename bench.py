@@ -42,7 +42,10 @@ def parse_args():
     p.add_argument("--graphs", action="store_true",
                    help="capture the whole train step in a hipGraph "
                         "(single-GPU)")
-    return p.parse_args()
+    args = p.parse_args()
+    if args.eight_bit and not args.model.startswith("llama"):
+        p.error("--eight-bit is for the llama models")
+    return args
 
 
 def dist_env():

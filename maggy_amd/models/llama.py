@@ -239,8 +239,6 @@ def _packed_while(generate):
     @functools.wraps(generate)
     def run(self, *args, **kw):
         fresh = [g for g in groups8(self) if g.packed is None]
-        if not fresh:
-            return generate(self, *args, **kw)
         try:
             for g in fresh:
                 g.pack()

@@ -118,8 +118,8 @@ class Block8:
     """A tensor held in 8 bits a value (``pack8``), read by ``unpack8``.
 
     ``codes`` [C / 128 rounded up, rows, 128] and ``scales`` are uint8
-    tensors; leading axes are flattened into rows.  ``shape`` and ``dtype`` are those of the
-    tensor that was packed."""
+    tensors; leading axes are flattened into rows.  ``shape`` and ``dtype``
+    are those of the tensor that was packed."""
 
     __slots__ = ("codes", "scales", "shape", "dtype")
 
@@ -407,35 +407,50 @@ class Linear8Group:
     """Bias-free linear modules that read the same input, run as one
     ``linear8``.  ``pack`` keeps their weights packed for calls without
     gradients, until ``drop``, a call with gradients (training is about to
-    change them) or a change of the weights themselves."""
+    change them) or a change of the weights themselves.  A HIP graph goes on
+    with the weights as they were packed when it was captured."""
 
     def __init__(self, *linears):
         for m in linears:
             if m.bias is not None:
                 raise ValueError("linear8 has no bias")
         self.linears = linears
-        self.drop()
+        self._held = None  # (Weight8, what it was packed from)
+        self._captured = []
+
+    def __getstate__(self):
+        # a copy packs its own: its weights count their versions anew
+        return {"linears": self.linears, "_held": None, "_captured": []}
+
+    @property
+    def packed(self):
+        held = self._held
+        return None if held is None else held[0]
 
     def _state(self):
-        return [(m.weight, m.weight._version) for m in self.linears]
+        # tensors made in inference mode count no versions
+        return [(m.weight, m.weight.device, m.weight.dtype,
+                 None if m.weight.is_inference() else m.weight._version)
+                for m in self.linears]
 
     def pack(self):
-        self.packed = pack_weight8(*(m.weight for m in self.linears))
-        self._packed_of = self._state()
+        self._held = (pack_weight8(*(m.weight for m in self.linears)),
+                      self._state())
 
     def drop(self):
-        self.packed = self._packed_of = None
-
-    def _is_packed(self):
-        if torch.is_grad_enabled():
-            return False
-        return all(m.weight is w and w._version == v
-                   for m, (w, v) in zip(self.linears, self._packed_of))
+        self._held = None
 
     def __call__(self, x):
-        if self.packed is not None:
-            if self._is_packed():
-                return linear8(x, self.packed)
+        held = self._held  # another thread may drop it meanwhile
+        if held is not None:
+            packed, of = held
+            if not torch.is_grad_enabled() and all(
+                    a[0] is b[0] and a[1:] == b[1:]
+                    for a, b in zip(self._state(), of)):
+                if x.is_cuda and torch.cuda.is_current_stream_capturing() \
+                        and not any(p is packed for p in self._captured):
+                    self._captured.append(packed)  # replays read it
+                return linear8(x, packed)
             self.drop()
         return linear8(x, *(m.weight for m in self.linears))
 

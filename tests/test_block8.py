@@ -270,3 +270,63 @@ def test_llama_in_8_bits_decodes():
     assert all(g.packed is not None for g in groups8(m))  # the caller's
     got = m.generate_captured(prompt, max_new_tokens=6, use_graph=False)
     assert torch.equal(got, out)
+
+
+def _group(N=48, K=96, dtype=torch.float32):
+    torch.manual_seed(0)
+    m = ops.MaggyLinear8(K, N).to(dtype)
+    return m, torch.randn(3, K, dtype=dtype)
+
+
+@torch.no_grad()
+def test_packed_weights_of_a_converted_module_are_dropped():
+    m, x = _group()
+    ops.pack8_model(m)
+    m.to(torch.bfloat16)
+    y = m(x.bfloat16())
+    assert m.group.packed is None
+    assert torch.equal(y, ops.linear8(x.bfloat16(), m.weight))
+
+
+@torch.no_grad()
+def test_packed_module_copies():
+    m, x = _group()
+    ops.pack8_model(m)
+    other = copy.deepcopy(m)
+    other.weight.mul_(2)
+    assert torch.equal(other(x), 2 * m(x))
+    assert m.group.packed is not None
+
+
+def test_weights_made_in_inference_mode_pack():
+    with torch.inference_mode():
+        m, x = _group()
+        want = m(x)
+        ops.pack8_model(m)
+        assert torch.equal(m(x), want)
+        assert m.group.packed is not None
+
+
+@torch.no_grad()
+def test_weights_dropped_by_another_thread_meanwhile(monkeypatch):
+    m, x = _group()
+    want = m(x)
+    ops.pack8_model(m)
+    state = m.group._state
+
+    def dropped_meanwhile():
+        m.group.drop()
+        return state()
+
+    monkeypatch.setattr(m.group, "_state", dropped_meanwhile)
+    assert torch.equal(m(x), want)
+
+
+def test_bench_refuses_8_bits_of_other_models(monkeypatch):
+    bench = pytest.importorskip("bench")
+    monkeypatch.setattr("sys.argv", ["bench.py", "--eight-bit"])
+    with pytest.raises(SystemExit):
+        bench.parse_args()
+    monkeypatch.setattr("sys.argv", ["bench.py", "--eight-bit", "--model",
+                                     "llama8b"])
+    assert bench.parse_args().eight_bit
