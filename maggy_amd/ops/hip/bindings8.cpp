@@ -8,6 +8,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 
 #include <limits>
 
@@ -422,6 +423,7 @@ std::vector<Tensor> product(const Mat8& x, const Mat8& w, int64_t M,
   a.xsp = x.Rp;
   if (M) {
     const long long bytes = b8_gemm_workspace(&a);
+    TORCH_CHECK(bytes >= 0, "linear8: matrix is too large");
     Tensor space;
     if (bytes)
       space = torch::empty({bytes}, like.options()
@@ -612,6 +614,25 @@ void no_second_derivative(const char* name) {
               " has no second derivative: backward cannot create a graph");
 }
 
+// A leaf whose eager graph lives accumulates on that graph's stream.  If that
+// is the default stream, capturing this pass would end in the runtime: no
+// capture can wait for it.
+void no_eager_leaves(const char* name) {
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() ==
+      c10::cuda::CaptureStatus::None)
+    return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()))
+      continue;
+    const auto stream = edge.function->stream();
+    TORCH_CHECK(!stream || stream->id() != 0, name,
+                ": a backward pass cannot be captured while an eager graph "
+                "of the same leaf, made on the default stream, lives");
+  }
+}
+
 struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
   static Tensor forward(AutogradContext* ctx, Tensor g, Tensor u) {
     auto out = swiglu8_fwd(g, u, true);
@@ -620,6 +641,7 @@ struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list dh) {
     no_second_derivative("swiglu8");
+    no_eager_leaves("swiglu8");
     const auto k = ctx->get_saved_variables();
     return swiglu8_bwd(dh[0], k[0], k[1], k[2], k[3]);
   }
@@ -643,6 +665,7 @@ struct RMSNorm8 : torch::autograd::Function<RMSNorm8> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
     no_second_derivative("rms_norm8");
+    no_eager_leaves("rms_norm8");
     const auto k = ctx->get_saved_variables();
     auto d = rms8_bwd(dy[0], k[0], k[1], k[3], k[2],
                       ctx->needs_input_grad(0), ctx->needs_input_grad(1));
@@ -679,6 +702,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list dys) {
     no_second_derivative("linear8");
+    no_eager_leaves("linear8");
     auto kept = ctx->get_saved_variables();
     const size_t n = kept.size() - 2;
     c10::optional<Tensor> codes, scales;

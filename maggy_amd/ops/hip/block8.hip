@@ -77,8 +77,13 @@ __global__ __launch_bounds__(kThreads) void unpack_rows(
 // neighbouring rows, so that four rows of one column make one dword of the
 // transposed codes, and 16 lanes (one DPP row) hold a whole row of the tile.
 struct TileSpace {
-  static constexpr int kPitch = 33;  // dwords a transposed row of 128 codes
-  uint32_t turned[128 * kPitch];
+  // the transposed codes: dword d of row c lies at d ^ (c / 8 % 8) * 4, so
+  // that 16-byte reads take 8 lanes a row without a bank conflict, and the
+  // columns that a wave writes at once, 8 apart, at most two by two
+  uint32_t turned[128 * 32];
+  static __device__ __forceinline__ int at(int c, int d) {
+    return c * 32 + (d ^ (c >> 3 & 7) << 2);
+  }
   uint32_t tops[8][128];
   uint32_t scales[128];
 };
@@ -86,7 +91,6 @@ struct TileSpace {
 template <class T, bool FROM8, bool ONE_SCALE, bool ROWS, bool COLS>
 __device__ __forceinline__ void pack_tile(const TileJob& a, TileSpace& space,
                                           int tile) {
-  constexpr int kPitch = TileSpace::kPitch;
   uint32_t(&tops)[8][128] = space.tops;
   uint32_t* turned = space.turned;
   const int t = threadIdx.x, cg = t & 15, rg = t >> 4, wave = t >> 6;
@@ -187,23 +191,22 @@ __device__ __forceinline__ void pack_tile(const TileJob& a, TileSpace& space,
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float s = scale_inverse(E[j]);
-      turned[(cg * 8 + j) * kPitch + rg] =
+      turned[TileSpace::at(cg * 8 + j, rg)] =
           encode4(v[0][j] * s, v[1][j] * s, v[2][j] * s, v[3][j] * s);
     }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = h * 64 + (t >> 3), k = (t & 7) * 4;
-      const uint32_t* s = turned + c * kPitch + k;
       *(u32x4*)(a.col_codes +
                 (b * a.col_n + a.col_r0 + tc * 128 + c) * 128 + k * 4) =
-          u32x4{s[0], s[1], s[2], s[3]};
+          *(const u32x4*)(turned + TileSpace::at(c, k));
     }
   }
 }
 
 __global__ __launch_bounds__(512) void pack_tiles(TileJobs jobs) {
-  __shared__ TileSpace space;
+  __shared__ __align__(16) TileSpace space;
   int j = 0;
   while (j + 1 < jobs.count && (int)blockIdx.x >= jobs.job[j + 1].first_block)
     ++j;
@@ -509,7 +512,7 @@ static void rms_fwd_run(int blocks, hipStream_t st, const void* x,
                         long long ldx, const float* w, long long R, int C,
                         float eps, void* y, float* inv, uint8_t* codes,
                         int Cp, uint32_t* scales, long long Rp) {
-  launch(rms_fwd<T, V, WPR, NI>, blocks, kThreads, st, 
+  launch(rms_fwd<T, V, WPR, NI>, blocks, kThreads, st,
       (const typename T::raw*)x, ldx, w, R, C, eps, (typename T::raw*)y, inv,
       codes, Cp, scales, Rp);
 }
@@ -520,7 +523,7 @@ static void rms_bwd_run(int blocks, hipStream_t st, const void* dy,
                         const uint32_t* scales, long long Rp, const float* w,
                         const float* inv, long long R, int C, void* dx,
                         float* partials) {
-  launch(rms_bwd<T, V, WPR, NI>, blocks, kThreads, st, 
+  launch(rms_bwd<T, V, WPR, NI>, blocks, kThreads, st,
       (const typename T::raw*)dy, ldy, codes, Cp, scales, Rp, w, inv, R, C,
       (typename T::raw*)dx, partials);
 }
@@ -546,7 +549,7 @@ extern "C" void launch_b8_pack(int dtype, int vec, const void* x,
                                long long Rp, hipStream_t st) {
   const int Q = (Cp + 511) / 512;
   B8_TYPED(dtype, vec,
-           (launch(pack_rows<T, V>, unit_blocks(R, Q), kThreads, st, 
+           (launch(pack_rows<T, V>, unit_blocks(R, Q), kThreads, st,
                (const T::raw*)x, ldx, R, C, codes, Cp, scales, Rp, Q)));
 }
 
@@ -558,7 +561,7 @@ extern "C" void launch_b8_unpack(int dtype, int vec, const uint8_t* codes,
   const float most =
       dtype == 0 ? 0x1.fep127f : dtype == 1 ? 65504.f : 0x1.fffffep127f;
   B8_TYPED(dtype, vec,
-           (launch(unpack_rows<T, V>, unit_blocks(R, Q), kThreads, st, 
+           (launch(unpack_rows<T, V>, unit_blocks(R, Q), kThreads, st,
                codes, Cp, scales, Rp, Q, R, C, (T::raw*)out, most)));
 }
 
@@ -568,7 +571,8 @@ extern "C" bool launch_b8_tiles(TileJobs* jobs, hipStream_t st) {
     TileJob& a = jobs->job[j];
     a.first_block = (int)blocks;
     blocks += (a.R + 127ll) / 128 * ((a.C + 127ll) / 128);
-    if (blocks >= 1ll << 31) return false;
+    // a launch has fewer than 2^32 threads
+    if (blocks >= 1ll << 23) return false;
   }
   if (blocks) launch(pack_tiles, blocks, 512, st, *jobs);
   return true;
@@ -582,7 +586,7 @@ extern "C" void launch_b8_swiglu_fwd(int dtype, int vec, const void* g,
                                      long long Rp, hipStream_t st) {
   const int Q = (Cp + 511) / 512;
   B8_TYPED(dtype, vec,
-           (launch(swiglu_fwd<T, V>, unit_blocks(R, Q), kThreads, st, 
+           (launch(swiglu_fwd<T, V>, unit_blocks(R, Q), kThreads, st,
                (const T::raw*)g, ldg, (const T::raw*)u, ldu, R, C,
                (T::raw*)h, gc, uc, Cp, gs, us, Rp, Q)));
 }
@@ -595,7 +599,7 @@ extern "C" void launch_b8_swiglu_bwd(int dtype, int vec, const void* dh,
                                      void* dg, void* du, hipStream_t st) {
   const int Q = (Cp + 511) / 512;
   B8_TYPED(dtype, vec,
-           (launch(swiglu_bwd<T, V>, unit_blocks(R, Q), kThreads, st, 
+           (launch(swiglu_bwd<T, V>, unit_blocks(R, Q), kThreads, st,
                (const T::raw*)dh, ldh, gc, uc, Cp, gs, us, Rp, Q, R, C,
                (T::raw*)dg, (T::raw*)du)));
 }
@@ -615,11 +619,9 @@ extern "C" void launch_b8_rms_fwd(int dtype, int vec, const void* x,
 // the workgroups of the backward pass, and the rows of partials they write
 extern "C" int b8_rms_bwd_blocks(long long R, int C) {
   const long long groups = C <= 2048 ? (R + 3) / 4 : R;
-#ifdef RB
-  const int most = RB;
-#else
+  // as many as the registers let run at once: 4 a CU where a lane holds up
+  // to 2 * 8 values, else 2
   const int most = C <= 1024 || (C > 2048 && C <= 4096) ? 1024 : 512;
-#endif
   return (int)(groups < most ? groups : most);
 }
 extern "C" int b8_rms_bwd_partials(long long R, int C) {
@@ -638,6 +640,6 @@ extern "C" void launch_b8_rms_bwd(int dtype, int vec, const void* dy,
            B8_ROWS(rms_bwd_run, C, blocks, st, dy, ldy, codes, Cp, scales,
                    Rp, w, inv, R, C, dx, partials));
   if (partials)
-    launch(fold_rows, (C + 63) / 64, 1024, st, 
+    launch(fold_rows, (C + 63) / 64, 1024, st,
         partials, b8_rms_bwd_partials(R, C), C, dw);
 }

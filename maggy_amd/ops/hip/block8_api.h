@@ -102,7 +102,8 @@ void launch_b8_rms_bwd(int dtype, int vec, const void* dy, long long ldy,
                        long long Rp, const float* w, const float* inv,
                        long long R, int C, void* dx, float* partials,
                        float* dw, hipStream_t st);
-// bytes of workspace that the product wants, and the product
+// bytes of workspace that the product wants (-1: too large a product for a
+// launch), and the product
 long long b8_gemm_workspace(const b8::GemmArgs* args);
 void launch_b8_gemm(const b8::GemmArgs* args, float* workspace,
                     hipStream_t st);

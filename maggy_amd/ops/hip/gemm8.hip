@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
   // compiler copy all accumulators.
 #pragma unroll
   for (int step = 0; step < NBUF; ++step) {
-    load_scales(step + 3 >> 2);
+    load_scales((step + 3) >> 2);
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) load(step, n);
     advance(step);
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
 #pragma unroll
     for (int n = 0; n < kProducts; ++n) {
       product(f1, sx, sw, n);
-      if (n == 0) load_scales(kt + NBUF + 3 >> 2);
+      if (n == 0) load_scales((kt + NBUF + 3) >> 2);
 #pragma unroll
       for (int k = n * kLoadsEach; k < (n + 1) * kLoadsEach; ++k)
         if (k < kLoads) load(kt + NBUF, k);
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
       for (int r = 0; r < 4; ++r) {
         const f32x16& v = acc[i * FW + j];
         *(u32x2*)(mine + m * kRowBytes +
-                  ((j * 4 + r ^ m % kChunks) << 4) + fg * 8) =
+                  (((j * 4 + r) ^ m % kChunks) << 4) + fg * 8) =
             u32x2{Bf16::from_f(v[4 * r]) |
                       (uint32_t)Bf16::from_f(v[4 * r + 1]) << 16,
                   Bf16::from_f(v[4 * r + 2]) |
@@ -394,7 +394,6 @@ __global__ __launch_bounds__(256) void join_splits(GemmArgs a,
   const int lane = threadIdx.x & 63, r = threadIdx.x >> 6;
   const int frag = blockIdx.x % kProducts;
   const int wave = blockIdx.x / kProducts % 4;
-  const int rest = work.tiles_m * work.tiles_n - work.full;
   const int k = blockIdx.x / (kProducts * 4);
   const Item it = item_of<BM, BN>(work, (a.KT + 3) >> 2, work.full + k);
   const f32x4* p = (const f32x4*)work.partials +
@@ -406,7 +405,7 @@ __global__ __launch_bounds__(256) void join_splits(GemmArgs a,
     v += p[(long long)s * 4 * kProducts * 256];
   const int m = it.m0 + (wave >> 1) * (BM / 2) + frag / FW * 32 + (lane & 31);
   const int wn = (wave & 1) * (BN / 2);
-  if (k < rest && m < a.M) {
+  if (m < a.M) {
     const Out o = out_of(a, it.n0 + wn);
     store4(o, m, o.c0 + frag % FW * 32 + r * 8 + (lane >> 5) * 4, v);
   }
@@ -549,7 +548,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
       // past the end w repeats its last block, against zeros; scales there
       // may never have been written
       const bool inside = k0 + u < a.KT;
-      const int shift = 8 * (k0 + u & 3);
+      const int shift = 8 * ((k0 + u) & 3);
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         int sx;
@@ -639,6 +638,7 @@ static Plan plan_of(const GemmArgs& a) {
                {64, 64, 3.0f, 0.29f, 0.33f}};
   const int quads = (a.KT + 3) / 4;
   Plan best{};
+  best.kind = -1;
   float least = 0.f;
   for (int k = 0; k < 4; ++k) {
     const auto& kind = kinds[k];
@@ -663,6 +663,7 @@ static Plan plan_of(const GemmArgs& a) {
         least = us;
         const long long full = splits > 1 ? tiles - rest : tiles;
         const long long items = full + (tiles - full) * splits;
+        if (items >= 1ll << 24) continue;  // a launch has < 2^32 threads
         best.kind = k;
         best.work = TileWork{tm, tn, (int)full, splits, (int)items, nullptr};
         best.workspace =
@@ -674,7 +675,7 @@ static Plan plan_of(const GemmArgs& a) {
   const long long groups = (a.M + 31) / 32 * ((a.N + 15) / 16);
   const float us =
       2.3f + 2.8f * ((a.KT + 15) / 16) * (groups < 256 ? 1.f : groups / 256.f);
-  if (us < least) best = Plan{4};
+  if (us < least) best = Plan{4};  // never for a grid that is too large
   return best;
 }
 
@@ -692,7 +693,8 @@ static void tile_run(const GemmArgs& a, const Plan& p, hipStream_t st) {
 using namespace b8;
 
 extern "C" long long b8_gemm_workspace(const GemmArgs* args) {
-  return plan_of(*args).workspace;
+  const Plan p = plan_of(*args);
+  return p.kind < 0 ? -1 : p.workspace;
 }
 
 extern "C" void launch_b8_gemm(const GemmArgs* args, float* workspace,

@@ -39,21 +39,27 @@ def block_value(b, dims):
     return torch.where(b.isfinite(), v, torch.full_like(b, float("nan")))
 
 
+def _padded(x):
+    return torch.nn.functional.pad(
+        x.double(), (0, -x.shape[1] % 128, 0, -x.shape[0] % 128))
+
+
 def held(x, axis=1):
     """[R, C] as held in blocks of 128 along ``axis``."""
     if axis == 0:
         return held(x.t(), 1).t()
-    if x.shape[0] == 0:
+    R, C = x.shape
+    if R == 0:
         return x.double()
-    return torch.cat([block_value(x[:, i:i + 128], (1,))
-                      for i in range(0, x.shape[1], 128)], 1)
+    b = _padded(x)[:R].unflatten(1, (-1, 128))
+    return block_value(b, (2,)).flatten(1)[:, :C]
 
 
 def held_weight(w):
-    return torch.cat([torch.cat([
-        block_value(w[i:i + 128, j:j + 128], (0, 1))
-        for j in range(0, w.shape[1], 128)], 1)
-        for i in range(0, w.shape[0], 128)], 0)
+    N, K = w.shape
+    p = _padded(w)
+    b = p.view(p.shape[0] // 128, 128, p.shape[1] // 128, 128)
+    return block_value(b, (1, 3)).reshape(p.shape)[:N, :K]
 
 
 def product_bound(a, b):

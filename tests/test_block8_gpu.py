@@ -545,3 +545,180 @@ def test_weights_changed_before_backward_are_noticed():
         w.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+# ------------------------------------------- every kernel, and large offsets
+# Sizes that reach each tile size, K split for all tiles and for the last
+# ones only, K shared by the waves, and few rows packed on the way; K short
+# of one block, ending inside a quad of blocks, and long.
+PLANS = [(1, 64, (48,)), (5, 700, (300, 20)), (16, 8, (16,)),
+         (16, 2048, (8192,)), (13, 1000, (14000,)), (17, 300, (40,)),
+         (32, 4096, (512,)), (48, 130, (1030,)), (64, 6000, (256,)),
+         (100, 128, (5000,)), (129, 640, (2049,)), (256, 16384, (128,)),
+         (700, 384, (700,)), (1025, 1024, (1025,)), (2048, 512, (2048, 700)),
+         (3000, 200, (3000,)), (4200, 1536, (2500,)), (4352, 4096, (4352,)),
+         (520, 12000, (390,))]
+
+
+@pytest.mark.parametrize("M,K,Ns", PLANS)
+def test_linear8_over_its_kernels(M, K, Ns):
+    x, ws, _ = _linear_inputs(M, K, Ns, seed=M + K)
+    xq = oracle.held(x)
+    with torch.no_grad():
+        packed = ops.pack_weight8(*ws)
+        for call in (ops.linear8(x, packed), ops.linear8(x, *ws)):
+            call = call if isinstance(call, tuple) else (call,)
+            for y, w in zip(call, ws):
+                wq = oracle.held_weight(w)
+                oracle.assert_within(y, xq @ wq.t(),
+                                     oracle.product_bound(xq, wq))
+
+
+def test_linear8_of_few_rows_holds_what_pack8_holds():
+    """Rows packed on the way are rows packed before: the same codes, so
+    results differ by the order of a sum only."""
+    x, ws, _ = _linear_inputs(16, 3000, (200,))
+    x[3, 100] = float("inf")
+    x[4, 2999] = float("nan")
+    x[5] = 0
+    x[6, :] = 1e-39
+    x[7, 5] = torch.finfo(torch.bfloat16).max
+    xq, wq = oracle.held(x), oracle.held_weight(ws[0])
+    with torch.no_grad():
+        y = ops.linear8(x, ops.pack_weight8(ws[0]))
+    bad = torch.zeros(16, dtype=torch.bool, device="cuda")
+    bad[[3, 4]] = True
+    assert y[bad].isnan().all()
+    oracle.assert_within(y[~bad], (xq[~bad] @ wq.t()),
+                         oracle.product_bound(xq[~bad], wq))
+
+
+def test_one_dimensional_input():
+    x, ws, _ = _linear_inputs(1, 200, (60, 50))
+    with torch.no_grad():
+        a, b = ops.linear8(x, *ws)
+        c, d = ops.linear8(x[0], *ws)
+        assert c.shape == (60,) and d.shape == (50,)
+        assert torch.equal(a[0], c) and torch.equal(b[0], d)
+        n = torch.ones(200, device="cuda")
+        assert torch.equal(ops.rms_norm8(x[0], n), ops.rms_norm8(x, n)[0])
+        assert torch.equal(ops.swiglu8(x[0], x[0]), ops.swiglu8(x, x)[0])
+        assert torch.equal(ops.unpack8(ops.pack8(x[0])),
+                           ops.unpack8(ops.pack8(x))[0])
+
+
+def test_offsets_past_32_bits():
+    R, C = 140001, 16384  # 2.3e9 values
+    x = torch.empty(R, C, device="cuda", dtype=torch.bfloat16)
+    x.normal_(generator=_gen(1))
+    last = slice(R - 40, R)
+    want = oracle.held(x[last])
+    held = ops.pack8(x)
+    assert torch.equal(ops.unpack8(held)[last].double(), want)
+    del held
+    # a product over all of it, and one with as large a result
+    w = _normal((64, C), 2, 0.02)
+    with torch.no_grad():
+        y = ops.linear8(x, ops.pack_weight8(w))
+    wq = oracle.held_weight(w)
+    oracle.assert_within(y[last], want @ wq.t(),
+                         oracle.product_bound(want, wq))
+    narrow = x[:, :40]
+    w = _normal((C, 40), 3, 0.1)
+    with torch.no_grad():
+        y = ops.linear8(narrow, ops.pack_weight8(w))
+    xq, wq = oracle.held(narrow[last]), oracle.held_weight(w)
+    oracle.assert_within(y[last], xq @ wq.t(), oracle.product_bound(xq, wq))
+    del y
+    # the norm and the gate, with their gradients
+    n = torch.ones(C, device="cuda", requires_grad=True)
+    x.requires_grad_(True)
+    y = ops.rms_norm8(x, n)
+    dx, _ = torch.autograd.grad(y, (x, n), x.detach())
+    d = x.detach()[last]
+    (wy, by), (wdx, bdx), _ = oracle.rms(d, n.detach(), d, 1e-5)
+    oracle.assert_within(y[last], wy, by)
+    oracle.assert_within(dx[last], wdx, bdx)
+    del y, dx
+    h = ops.swiglu8(x, x.detach())
+    dg, = torch.autograd.grad(h, x, x.detach())
+    (wh, bh), (wdg, bdg), _ = oracle.swiglu(d, d, d)
+    oracle.assert_within(h[last], wh, bh)
+    oracle.assert_within(dg[last], wdg, bdg)
+
+
+def test_a_batch_of_many_tokens_trains():
+    """dW over a long axis: more K steps than a tile has rows."""
+    x, ws, dys = _linear_inputs(40000, 130, (70,))
+    _check_linear(x, ws, dys)
+
+
+def test_a_graph_outlives_dropped_packed_weights():
+    """A captured module call reads the weights that it was captured with."""
+    m = ops.MaggyLinear8(512, 300).cuda().bfloat16()
+    x = _normal((4, 512), 1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        ops.pack8_model(m)
+        want = m(x)
+        with torch.cuda.graph(graph):
+            y = m(x)
+    ops.drop8_model(m)
+    junk = [torch.full((1 << 20,), 255, device="cuda", dtype=torch.uint8)
+            for _ in range(16)]  # would land in freed memory
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    del junk
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """A leaf whose eager graph lives belongs to the default stream."""
+    x = _normal((8, 256), 1)
+    w = _normal((64, 256), 2, 0.1).requires_grad_(True)
+    n = torch.ones(256, device="cuda", requires_grad=True)
+    g = _normal((8, 256), 3).requires_grad_(True)
+    for call, dy in ((lambda: ops.linear8(x, w), _normal((8, 64), 4)),
+                     (lambda: ops.rms_norm8(x, n), _normal((8, 256), 5)),
+                     (lambda: ops.swiglu8(g, x), _normal((8, 256), 6))):
+        eager = call()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            y = call()
+            with pytest.raises(RuntimeError, match="eager graph"):
+                y.backward(dy)
+        eager.backward(dy)  # not hurt by it
+        torch.cuda.synchronize()
+    assert all(t.grad.isfinite().all() for t in (w, n, g))
+
+
+def test_two_threads_at_once():
+    """Forward and backward passes of two threads, each on its own stream."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(seed):
+        x = _normal((300 + 50 * seed, 512), seed).requires_grad_(True)
+        w1, w3 = [_normal((384, 512), seed + s, 0.05).requires_grad_(True)
+                  for s in (10, 20)]
+        n = torch.ones(512, device="cuda", requires_grad=True)
+        h = ops.swiglu8(*ops.linear8(ops.rms_norm8(x, n), w1, w3))
+        return [h.detach(), *torch.autograd.grad(
+            h, [x, n, w1, w3], _normal(h.shape, seed + 30))]
+
+    def on_stream(seed):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            out = [work(seed) for _ in range(10)]
+        s.synchronize()
+        return out
+
+    want = [work(seed) for seed in (1, 2)]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(2) as pool:
+        got = list(pool.map(on_stream, (1, 2)))
+    for outs, exact in zip(got, want):
+        for out in outs:
+            for a, b in zip(out, exact):
+                assert torch.equal(a, b)
