@@ -70,15 +70,22 @@ __device__ __forceinline__ Eight load8_raw(const typename T::raw* row, int c,
       if constexpr (sizeof(typename T::raw) == 4)
         e.b = *(const u32x4*)(row + c + 4);
     }
-  } else {
+  } else if (c + 8 <= C) {  // by the same loads, aligned to a value only
+    __builtin_memcpy(&e.a, row + c, 16);
+    if constexpr (sizeof(typename T::raw) == 4)
+      __builtin_memcpy(&e.b, row + c + 4, 16);
+  } else if (c < C) {
+    // no branch a value: each would wait for its load alone
+    typename T::raw v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = row[c + i < C ? c + i : C - 1];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (c + i >= C) continue;
       if constexpr (sizeof(typename T::raw) == 2)
-        e.a[i >> 1] |= (uint32_t)row[c + i] << (16 * (i & 1));
+        e.a[i >> 1] |= (c + i < C ? (uint32_t)v[i] : 0u) << (16 * (i & 1));
       else
         (i < 4 ? e.a : e.b)[i & 3] =
-            __builtin_bit_cast(uint32_t, (float)row[c + i]);
+            c + i < C ? __builtin_bit_cast(uint32_t, (float)v[i]) : 0u;
     }
   }
   return e;
@@ -106,20 +113,28 @@ __device__ __forceinline__ void load8(const typename T::raw* row, int c,
 template <class T, bool VEC>
 __device__ __forceinline__ void store8(typename T::raw* row, int c, int C,
                                        const float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c >= C) return;
+  if (VEC ? c < C : c + 8 <= C) {
     if constexpr (sizeof(typename T::raw) == 2) {
       u32x4 d;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         d[i] = (uint32_t)T::from_f(v[2 * i]) |
                (uint32_t)T::from_f(v[2 * i + 1]) << 16;
-      *(u32x4*)(row + c) = d;
+      if constexpr (VEC)
+        *(u32x4*)(row + c) = d;
+      else
+        __builtin_memcpy(row + c, &d, 16);
     } else {
-      *(f32x4*)(row + c) = f32x4{v[0], v[1], v[2], v[3]};
-      *(f32x4*)(row + c + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      const f32x4 lo{v[0], v[1], v[2], v[3]}, hi{v[4], v[5], v[6], v[7]};
+      if constexpr (VEC) {
+        *(f32x4*)(row + c) = lo;
+        *(f32x4*)(row + c + 4) = hi;
+      } else {
+        __builtin_memcpy(row + c, &lo, 16);
+        __builtin_memcpy(row + c + 4, &hi, 16);
+      }
     }
-  } else {
+  } else if constexpr (!VEC) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (c + i < C) row[c + i] = T::from_f(v[i]);

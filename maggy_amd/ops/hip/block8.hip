@@ -100,26 +100,41 @@ __device__ __forceinline__ void pack_tile(const TileJob& a, TileSpace& space,
   const long long r0 = tr * 128 + rg * 4;
   const int c0 = tc * 128 + cg * 8;
 
+  // all four rows' loads under way at once; rows past the end repeat the
+  // last one and count as zeros
   float v[4][8];
+  if constexpr (FROM8) {
+    u32x2 code[4];
+    uint32_t E[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long r = r0 + i;
-    if (r < a.R) {
-      if constexpr (FROM8) {
-        const uint32_t E = ((const uint8_t*)a.xs)
-            [4 * ((tc >> 2) * a.xsp + r) + (tc & 3)];
-        decode8(*(const u32x2*)code_at((const uint8_t*)a.x, a.ldx, r, c0),
-                scale_value(E), v[i]);
-      } else {
-        const auto* row = (const typename T::raw*)a.x + r * a.ldx;
-        if (a.vec)
-          load8<T, true>(row, c0, a.C, v[i]);
-        else
-          load8<T, false>(row, c0, a.C, v[i]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const long long r = min(r0 + i, a.R - 1ll);
+      E[i] = ((const uint8_t*)a.xs)[4 * ((tc >> 2) * a.xsp + r) + (tc & 3)];
+      code[i] = *(const u32x2*)code_at((const uint8_t*)a.x, a.ldx, r, c0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (r0 + i >= a.R) code[i] = u32x2{0, 0};
+      decode8(code[i], scale_value(E[i]), v[i]);
+    }
+  } else {
+    Eight e[4];
+    const auto* x = (const typename T::raw*)a.x;
+    if (a.vec) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        e[i] = load8_raw<T, true>(x + min(r0 + i, a.R - 1ll) * a.ldx, c0,
+                                  a.C);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      for (int i = 0; i < 4; ++i)
+        e[i] = load8_raw<T, false>(x + min(r0 + i, a.R - 1ll) * a.ldx, c0,
+                                   a.C);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (r0 + i >= a.R) e[i] = Eight{{0, 0, 0, 0}, {0, 0, 0, 0}};
+      widen<T>(e[i], v[i]);
     }
   }
 

@@ -45,21 +45,22 @@ __device__ __forceinline__ Out out_of(const GemmArgs& a, int n) {
   return o;
 }
 
-// columns [c, c + 4) of row m
+// columns [c, c + 4) of row m; an odd row is aligned to a value only, which
+// these stores may be
 __device__ __forceinline__ void store4(const Out& o, int m, int c, f32x4 v) {
   const long long at = (long long)m * o.count + c;
-  if ((o.count & 3) == 0) {
-    if (c >= o.count) return;
-    if (o.f32)
-      *(f32x4*)((float*)o.p + at) = v;
-    else
-      *(u32x2*)((uint16_t*)o.p + at) =
-          u32x2{Bf16::from_f(v[0]) | (uint32_t)Bf16::from_f(v[1]) << 16,
-                Bf16::from_f(v[2]) | (uint32_t)Bf16::from_f(v[3]) << 16};
+  if (c + 4 <= o.count) {
+    if (o.f32) {
+      __builtin_memcpy((float*)o.p + at, &v, 16);
+    } else {
+      const u32x2 d{Bf16::from_f(v[0]) | (uint32_t)Bf16::from_f(v[1]) << 16,
+                    Bf16::from_f(v[2]) | (uint32_t)Bf16::from_f(v[3]) << 16};
+      __builtin_memcpy((uint16_t*)o.p + at, &d, 8);
+    }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 3; ++i) {
     if (c + i >= o.count) break;
     if (o.f32)
       ((float*)o.p)[at + i] = v[i];
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
     return;
   }
   const Out o = out_of(a, n0 + wn);
-  if (o.f32 || (o.count & 7)) {
+  if (o.f32) {
 #pragma unroll
     for (int i = 0; i < FX; ++i) {
       const int m = m0 + wm + i * 32 + frow;
@@ -373,7 +374,8 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   const int c = lane % kChunks;
-  if (o.c0 + c * 8 >= o.count) return;
+  const int left = o.count - (o.c0 + c * 8);
+  if (left <= 0) return;
   uint16_t* out = (uint16_t*)o.p + o.c0 + c * 8;
   constexpr int kRowsEach = 64 / kChunks;
 #pragma unroll 8
@@ -381,7 +383,15 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
     const int row = k * kRowsEach + lane / kChunks, m = m0 + wm + row;
     const u32x4 v = *(const u32x4*)(mine + row * kRowBytes +
                                     ((c ^ row % kChunks) << 4));
-    if (m < a.M) *(u32x4*)(out + (long long)m * o.count) = v;
+    if (m >= a.M) continue;
+    uint16_t* to = out + (long long)m * o.count;
+    if (left >= 8) {
+      __builtin_memcpy(to, &v, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (i < left) to[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+    }
   }
 }
 
