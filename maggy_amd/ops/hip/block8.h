@@ -55,7 +55,8 @@ struct Fp32 {
 
 // Loads columns [c, c + 8) of a row; columns from C on read as zero.  VEC:
 // the host has checked that C, the row stride and the base allow 16-byte
-// loads, so a group of 8 lies inside the row or outside as a whole.
+// loads, so a group of 8 lies inside the row or outside as a whole.  Without
+// VEC a group that reaches past the row's end goes value by value.
 struct Eight {
   u32x4 a, b;  // 16-bit types use a only
 };

