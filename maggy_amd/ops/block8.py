@@ -158,19 +158,17 @@ def _rows(x):
     return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
 
 
-@torch.no_grad()
 def pack8(x):
-    """Hold ``x`` [..., C] in 8 bits, blocks of 128 along the last axis."""
+    """Hold ``x`` [..., C] in 8 bits, blocks of 128 along the last axis.
+    Gradients do not pass."""
     _check_float(x, "x")
-    x2 = _rows(x)
     if x.is_cuda:
-        codes, scales = ops.require_ext().pack8(x2)
+        codes, scales = ops.require_ext().pack8(_rows(x))
     else:
-        codes, scales = _pack_cpu(x2)
+        codes, scales = _pack_cpu(_rows(x.detach()))
     return Block8(codes, scales, x.shape, x.dtype)
 
 
-@torch.no_grad()
 def unpack8(held, dtype=None):
     """The tensor that ``held`` (a ``Block8``) stands for."""
     if not isinstance(held, Block8):
