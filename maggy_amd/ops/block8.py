@@ -5,7 +5,7 @@ The format (``Block8``) is OCP e4m3 codes with one power-of-two scale for 128
 neighbouring values of a row: the scale is the smallest 2^t, t >= -126, with
 max|x| <= 448 * 2^t over the block's finite values, a code is x * 2^-t
 rounded to nearest even.  A value keeps 4 significant bits (an error of at
-most 1/16 of itself) down to 2^-14 of its block's largest.  Infinities and
+most 1/16 of itself) down to 2^-13 of its block's largest.  Infinities and
 NaN are held as NaN and leave their neighbours alone.
 
     pack8, unpack8   a tensor held in 8 bits, and read back
