@@ -10,6 +10,7 @@ without sharding, so plain DP is the natural parallelism.
 """
 import functools
 import math
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -238,11 +239,16 @@ def _packed_while(generate):
     has packed them (``pack8_model``)."""
     @functools.wraps(generate)
     def run(self, *args, **kw):
-        fresh = [g for g in groups8(self) if g.packed is None]
+        groups = groups8(self)
+        fresh = [g for g in groups if g.packed is None]
         try:
             for g in fresh:
-                g.pack()
-            return generate(self, *args, **kw)
+                g.pack(owner=threading.get_ident())
+            # a graph that generate captures reads these to its end
+            held = [g.packed for g in groups]
+            out = generate(self, *args, **kw)
+            del held
+            return out
         finally:
             for g in fresh:
                 g.drop()

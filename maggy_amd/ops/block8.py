@@ -24,6 +24,8 @@ is worth about 16 bits, well inside bfloat16 but not float32.
 All run as HIP kernels on GPU tensors and raise without the extension; on the
 CPU the same definitions run in torch.
 """
+import threading
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
@@ -406,14 +408,17 @@ class Linear8Group:
     ``linear8``.  ``pack`` keeps their weights packed for calls without
     gradients, until ``drop``, a call with gradients (training is about to
     change them) or a change of the weights themselves.  A HIP graph goes on
-    with the weights as they were packed when it was captured."""
+    with the weights as they were packed when it was captured; they are kept
+    for it until ``drop(captured=True)``."""
 
     def __init__(self, *linears):
         for m in linears:
             if m.bias is not None:
                 raise ValueError("linear8 has no bias")
         self.linears = linears
-        self._held = None  # (Weight8, what it was packed from)
+        # (Weight8, what it was packed from, the only thread that may
+        # capture it)
+        self._held = None
         self._captured = []
 
     def __getstate__(self):
@@ -431,26 +436,36 @@ class Linear8Group:
                  None if m.weight.is_inference() else m.weight._version)
                 for m in self.linears]
 
-    def pack(self):
+    def pack(self, owner=None):
+        """``owner``: the one thread whose graphs may read what is packed
+        (an ident); it sees to it that they do not outlive it."""
         self._held = (pack_weight8(*(m.weight for m in self.linears)),
-                      self._state())
+                      self._state(), owner)
 
-    def drop(self):
+    def drop(self, captured=False):
         self._held = None
+        if captured:
+            self._captured = []
 
     def __call__(self, x):
         held = self._held  # another thread may drop it meanwhile
         if held is not None:
-            packed, of = held
-            if not torch.is_grad_enabled() and all(
+            packed, of, owner = held
+            if torch.is_grad_enabled() or not all(
                     a[0] is b[0] and a[1:] == b[1:]
                     for a, b in zip(self._state(), of)):
-                if x.is_cuda and torch.cuda.is_current_stream_capturing() \
-                        and not any(p is packed for p in self._captured):
-                    self._captured.append(packed)  # replays read it
+                self.drop()
+            elif self._may_read(x, packed, owner):
                 return linear8(x, packed)
-            self.drop()
         return linear8(x, *(m.weight for m in self.linears))
+
+    def _may_read(self, x, packed, owner):
+        """A captured call reads what it was captured with at every replay."""
+        if not (x.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return True
+        if owner is None and not any(p is packed for p in self._captured):
+            self._captured.append(packed)
+        return owner in (None, threading.get_ident())
 
 
 class MaggyLinear8(MaggyLinear):
@@ -494,12 +509,14 @@ def groups8(module):
 def pack8_model(module):
     """Pack the weights of every 8-bit linear of a model for serving.  A call
     with gradients or a change of a weight drops that layer's; code that
-    writes weights behind torch's back calls this again, or
-    ``drop8_model``."""
+    writes weights behind torch's back, through ``.data`` or kernels of its
+    own, calls this again, or ``drop8_model``."""
     for g in groups8(module):
         g.pack()
 
 
-def drop8_model(module):
+def drop8_model(module, captured=False):
+    """Drop what is packed; with ``captured`` also what was kept for graphs,
+    none of which may be replayed afterwards."""
     for g in groups8(module):
-        g.drop()
+        g.drop(captured)

@@ -381,6 +381,32 @@ def test_llama_in_8_bits_trains_and_decodes():
         assert torch.equal(m(tokens), packed)
 
 
+def test_llama_in_8_bits_decodes_in_a_graph():
+    """Like the 16-bit one in a process of its own, since captures depend on
+    what else a process has run; the same step runs eagerly beside it."""
+    import os
+    import subprocess
+    import sys
+
+    code = (
+        "import torch\n"
+        "from tests.test_block8_gpu import _llama\n"
+        "from maggy_amd import ops\n"
+        "m = _llama().eval()\n"
+        "prompt = torch.randint(0, 97, (2, 8), device='cuda')\n"
+        "ref = m.generate_captured(prompt, 9, use_graph=False)\n"
+        "assert torch.equal(m.generate_captured(prompt, 9), ref)\n"
+        "ops.pack8_model(m)\n"
+        "assert torch.equal(m.generate_captured(prompt, 9), ref)\n"
+        "print('CAPTURED_OK')\n"
+    )
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", code], cwd=repo,
+                       capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0 and "CAPTURED_OK" in p.stdout, \
+        p.stdout[-1500:] + p.stderr[-1500:]
+
+
 def test_under_autocast_from_fp32():
     lin = ops.MaggyLinear8(200, 100).cuda()
     x = _normal((50, 200), 1, dtype=torch.float32).requires_grad_(True)
@@ -672,6 +698,28 @@ def test_a_graph_outlives_dropped_packed_weights():
         torch.cuda.synchronize()
         assert torch.equal(y, want)
     del junk
+    assert len(m.group._captured) == 1
+    ops.drop8_model(m, captured=True)
+    assert not m.group._captured
+
+
+def test_a_graph_takes_no_packed_weights_of_another_thread():
+    """What generate packs for its call another thread does not capture."""
+    import threading
+
+    m = ops.MaggyLinear8(512, 300).cuda().bfloat16()
+    x = _normal((4, 512), 1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        m.group.pack(owner=threading.get_ident() + 1)
+        want = m(x)
+        with torch.cuda.graph(graph):
+            y = m(x)
+        assert not m.group._captured and m.group.packed is not None
+        m.weight.mul_(2)
+        graph.replay()  # packs the weights as they are now
+        torch.cuda.synchronize()
+        assert torch.equal(y, 2 * want)
 
 
 def test_capture_beside_an_eager_graph_is_refused():
