@@ -495,7 +495,8 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
   same_device(x, wcodes, "weight");
   const CUDAGuard guard(x.device());
   const int64_t M = x.size(0);
-  if (M >= 1 && M <= 16 && vec8(x)) {
+  // a launch has fewer than 2^32 threads, 16 a row of w
+  if (M >= 1 && M <= 16 && vec8(x) && w.rows() < (int64_t)1 << 28) {
     std::vector<Tensor> out;
     const b8::GemmArgs a =
         gemm_args(mat8(w), M, counts, torch::kBFloat16, x, &out);

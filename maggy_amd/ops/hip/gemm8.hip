@@ -645,17 +645,21 @@ static void split_run(SplitArgs sa, hipStream_t st) {
 //
 //   tile       fixed   step alone   step on a full card
 //   256 x 256    9.0      0.93          1.37
-//   128 x 256    6.5      0.62          0.85
-//   128 x 128    4.5      0.36          0.48
-//    64 x  64    3.0      0.29          0.33
+//   128 x 256    5.5      0.62          0.85
+//   128 x 128    3.7      0.36          0.48
+//    64 x  64    2.0      0.29          0.33
 //
-// Joining the splits costs a launch, about 4 us, and their traffic at about
-// 4 TB/s.  Measured either way (M x N, K), in us: 24576 x 4096, 14336: 1014
-// by 256 x 256 and 1500 by 128 x 128; 4096 x 2048, 16384: 135 by 256 x 256,
-// 117 with K split in two, 116 by 128 x 256, 133 by 128 x 128;
-// 2048 x 2048, 2048: 25 by 256 x 256, 17, 12.5 by 128 x 128, 29 by 64 x 64;
-// 1001 x 777, 1111: 18.5, 12.5, 8.6 and 6.5; 128 x 4096, 14336 by 128 x 128:
-// 48, and 21 in four splits.
+// Joining the splits costs a launch, about 2.5 us, and their traffic at about
+// 5 TB/s.  gemm_split takes 0.6 + 0.16 steps us for each 256 workgroups.
+// Over 220 products of up to 24576 x 14336 the choice is within 1 % of the
+// best on average.  Measured either way (M x N, K), in us:
+//   24576 x 4096, 14336: 1014 by 256 x 256 and 1500 by 128 x 128
+//   4096 x 2048, 16384: 135 by 256 x 256, 117 with K split in two, 116 by
+//     128 x 256, 133 by 128 x 128
+//   2048 x 2048, 2048: 25, 17, 12.5 by 128 x 128, 29 by 64 x 64
+//   1001 x 777, 1111: 18.5, 12.5, 8.6, 6.5 by 64 x 64
+//   128 x 4096, 14336: 48 by 128 x 128, 20 in four splits
+//   710 x 229, 176: 4.3 by 64 x 64, 3.4 by gemm_split
 constexpr int kCUs = 256;
 
 struct Plan {
@@ -669,9 +673,9 @@ static Plan plan_of(const GemmArgs& a) {
     int bm, bn;
     float fixed, alone, full;
   } kinds[] = {{256, 256, 9.0f, 0.93f, 1.37f},
-               {128, 256, 6.5f, 0.62f, 0.85f},
-               {128, 128, 4.5f, 0.36f, 0.48f},
-               {64, 64, 3.0f, 0.29f, 0.33f}};
+               {128, 256, 5.5f, 0.62f, 0.85f},
+               {128, 128, 3.7f, 0.36f, 0.48f},
+               {64, 64, 2.0f, 0.29f, 0.33f}};
   const int quads = (a.KT + 3) / 4;
   Plan best{};
   best.kind = -1;
@@ -694,7 +698,7 @@ static Plan plan_of(const GemmArgs& a) {
         us += kind.fixed + steps * (kind.alone + (kind.full - kind.alone) *
                                                (last % kCUs) / kCUs);
       if (splits > 1)
-        us += 4.f + (4.f * splits + 2.f) * rest * kind.bm * kind.bn / 4e6f;
+        us += 2.5f + (4.f * splits + 2.f) * rest * kind.bm * kind.bn / 5e6f;
       if (least == 0.f || us < least) {
         least = us;
         const long long full = splits > 1 ? tiles - rest : tiles;
@@ -707,11 +711,10 @@ static Plan plan_of(const GemmArgs& a) {
       }
     }
   }
-  // 32 rows of x by 16 of w a workgroup, a K step a wave at a time
+  // 32 rows of x by 16 of w a workgroup, its waves sharing K
   const long long groups = (a.M + 31) / 32 * ((a.N + 15) / 16);
-  const float us =
-      2.3f + 2.8f * ((a.KT + 15) / 16) * (groups < 256 ? 1.f : groups / 256.f);
-  if (us < least) best = Plan{4};  // never for a grid that is too large
+  const float us = 2.f + (groups + kCUs - 1) / kCUs * (0.6f + 0.16f * a.KT);
+  if (groups < 1 << 22 && (us < least || best.kind < 0)) best = Plan{4};
   return best;
 }
 

@@ -583,7 +583,8 @@ PLANS = [(1, 64, (48,)), (5, 700, (300, 20)), (16, 8, (16,)),
          (100, 128, (5000,)), (129, 640, (2049,)), (256, 16384, (128,)),
          (700, 384, (700,)), (1025, 1024, (1025,)), (2048, 512, (2048, 700)),
          (3000, 200, (3000,)), (4200, 1536, (2500,)), (4352, 4096, (4352,)),
-         (520, 12000, (390,))]
+         (520, 12000, (390,)), (3001, 200, (2999,)), (2047, 512, (2701,)),
+         (4617, 1792, (3457,))]
 
 
 @pytest.mark.parametrize("M,K,Ns", PLANS)
