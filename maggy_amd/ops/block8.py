@@ -416,8 +416,7 @@ class Linear8Group:
             if m.bias is not None:
                 raise ValueError("linear8 has no bias")
         self.linears = linears
-        # (Weight8, what it was packed from, the only thread that may
-        # capture it)
+        # (Weight8, what it was packed from, the only thread that reads it)
         self._held = None
         self._captured = []
 
@@ -437,8 +436,9 @@ class Linear8Group:
                 for m in self.linears]
 
     def pack(self, owner=None):
-        """``owner``: the one thread whose graphs may read what is packed
-        (an ident); it sees to it that they do not outlive it."""
+        """``owner``: the ident of the one thread that reads what is packed.
+        It orders its streams after this one and keeps what its graphs
+        read."""
         self._held = (pack_weight8(*(m.weight for m in self.linears)),
                       self._state(), owner)
 
@@ -460,12 +460,13 @@ class Linear8Group:
         return linear8(x, *(m.weight for m in self.linears))
 
     def _may_read(self, x, packed, owner):
-        """A captured call reads what it was captured with at every replay."""
-        if not (x.is_cuda and torch.cuda.is_current_stream_capturing()):
-            return True
-        if owner is None and not any(p is packed for p in self._captured):
+        if owner is not None:
+            return owner == threading.get_ident()
+        # a captured call reads what it was captured with at every replay
+        if x.is_cuda and torch.cuda.is_current_stream_capturing() \
+                and not any(p is packed for p in self._captured):
             self._captured.append(packed)
-        return owner in (None, threading.get_ident())
+        return True
 
 
 class MaggyLinear8(MaggyLinear):
@@ -510,9 +511,16 @@ def pack8_model(module):
     """Pack the weights of every 8-bit linear of a model for serving.  A call
     with gradients or a change of a weight drops that layer's; code that
     writes weights behind torch's back, through ``.data`` or kernels of its
-    own, calls this again, or ``drop8_model``."""
+    own, calls this again, or ``drop8_model``.  All streams and threads may
+    use what is packed."""
+    devices = set()
     for g in groups8(module):
         g.pack()
+        devices.add(g.packed.device)
+    for device in devices:
+        if device.type == "cuda" and \
+                not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()
 
 
 def drop8_model(module, captured=False):

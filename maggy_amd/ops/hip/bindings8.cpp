@@ -495,6 +495,11 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
   same_device(x, wcodes, "weight");
   const CUDAGuard guard(x.device());
   const int64_t M = x.size(0);
+  // packed weights are shared between streams: their memory is not to be
+  // used again before this call's kernels have read it
+  for (const Tensor* t : {&wcodes, &wscales})
+    c10::cuda::CUDACachingAllocator::recordStream(
+        t->storage().data_ptr(), at::cuda::getCurrentCUDAStream());
   // a launch has fewer than 2^32 threads, 16 a row of w
   if (M >= 1 && M <= 16 && vec8(x) && w.rows() < (int64_t)1 << 28) {
     std::vector<Tensor> out;

@@ -704,8 +704,37 @@ def test_a_graph_outlives_dropped_packed_weights():
     assert not m.group._captured
 
 
+def test_packed_weights_on_another_stream():
+    """Packed behind long work on one stream, read at once on another; then
+    dropped, and their memory offered for use, before that read runs."""
+    m = ops.MaggyLinear8(2048, 2000).cuda().bfloat16()
+    x = _normal((40, 2048), 1)
+    big = torch.randn(4096, 4096, device="cuda")
+    side = torch.cuda.Stream()
+    with torch.no_grad():
+        want = m(x)
+        for _ in range(3):
+            torch.cuda.synchronize()
+            for _ in range(10):
+                big @ big
+            ops.pack8_model(m)
+            with torch.cuda.stream(side):
+                first = m(x)
+                for _ in range(10):
+                    big @ big
+                second = m(x)
+            sizes = [m.group.packed.codes.numel(),
+                     m.group.packed.scales.numel()]
+            ops.drop8_model(m)
+            junk = [torch.full((n,), 255, device="cuda", dtype=torch.uint8)
+                    for n in sizes for _ in range(4)]
+            torch.cuda.synchronize()
+            assert torch.equal(first, want) and torch.equal(second, want)
+            del junk
+
+
 def test_a_graph_takes_no_packed_weights_of_another_thread():
-    """What generate packs for its call another thread does not capture."""
+    """What generate packs for its call another thread does not read."""
     import threading
 
     m = ops.MaggyLinear8(512, 300).cuda().bfloat16()
