@@ -411,9 +411,11 @@ b8::GemmArgs gemm_args(const Mat8& w, int64_t M,
   return a;
 }
 
+// soon: the next kernels are going to read the outputs
 std::vector<Tensor> product(const Mat8& x, const Mat8& w, int64_t M,
                             const std::vector<int64_t>& counts,
-                            torch::ScalarType dtype, const Tensor& like) {
+                            torch::ScalarType dtype, const Tensor& like,
+                            bool soon = true) {
   TORCH_CHECK(x.Cp == w.Cp && M <= x.rows, "linear8: columns do not match");
   std::vector<Tensor> out;
   b8::GemmArgs a = gemm_args(w, M, counts, dtype, like, &out);
@@ -421,6 +423,7 @@ std::vector<Tensor> product(const Mat8& x, const Mat8& w, int64_t M,
   a.xs = x.s;
   a.xn = x.rows;
   a.xsp = x.Rp;
+  a.stream = 2 * M * a.N >= (soon ? b8::kStreamResult : b8::kStreamOnce);
   if (M) {
     const long long bytes = b8_gemm_workspace(&a);
     TORCH_CHECK(bytes >= 0, "linear8: matrix is too large");
@@ -580,7 +583,7 @@ std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys,
     // are contiguous
     const Tensor all = product(cols, xt, first[counts.size() - 1] +
                                              counts.back(),
-                               {K}, ws[0].scalar_type(), ws[0])[0];
+                               {K}, ws[0].scalar_type(), ws[0], false)[0];
     for (size_t i = 0; i < counts.size(); ++i)
       out.push_back(counts.size() == 1
                         ? all

@@ -53,29 +53,50 @@ struct Fp32 {
   static __device__ __forceinline__ raw from_f(float f) { return f; }
 };
 
-// Loads columns [c, c + 8) of a row; columns from C on read as zero.  VEC:
-// the host has checked that C, the row stride and the base allow 16-byte
-// loads, so a group of 8 lies inside the row or outside as a whole.  Without
-// VEC a group that reaches past the row's end goes value by value.
+// How a kernel reads and writes plain rows.  kVec: the host has checked that
+// the columns, the row strides and the bases allow 16-byte accesses, so a
+// group of 8 lies inside the row or outside as a whole.  kOdd: accesses are
+// aligned to a value only, and a group that reaches past the row's end goes
+// value by value.  kStream: kVec, and the caches do not keep the line.
+enum { kOdd, kVec, kStream };
+
+// Loads columns [c, c + 8) of a row; columns from C on read as zero.
 struct Eight {
   u32x4 a, b;  // 16-bit types use a only
 };
 
-template <class T, bool VEC>
+// 16 bytes from p or to p, which is aligned as VEC says
+template <int VEC>
+__device__ __forceinline__ u32x4 load16(const void* p) {
+  if constexpr (VEC == kOdd) {
+    u32x4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+  } else if constexpr (VEC == kVec) {
+    return *(const u32x4*)p;
+  } else {
+    return __builtin_nontemporal_load((const u32x4*)p);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store16(void* p, u32x4 v) {
+  if constexpr (VEC == kOdd)
+    __builtin_memcpy(p, &v, 16);
+  else if constexpr (VEC == kVec)
+    *(u32x4*)p = v;
+  else
+    __builtin_nontemporal_store(v, (u32x4*)p);
+}
+
+template <class T, int VEC>
 __device__ __forceinline__ Eight load8_raw(const typename T::raw* row, int c,
                                            int C) {
   Eight e{{0, 0, 0, 0}, {0, 0, 0, 0}};
-  if constexpr (VEC) {
-    if (c < C) {
-      e.a = *(const u32x4*)(row + c);
-      if constexpr (sizeof(typename T::raw) == 4)
-        e.b = *(const u32x4*)(row + c + 4);
-    }
-  } else if (c + 8 <= C) {  // by the same loads, aligned to a value only
-    __builtin_memcpy(&e.a, row + c, 16);
+  if (VEC ? c < C : c + 8 <= C) {
+    e.a = load16<VEC>(row + c);
     if constexpr (sizeof(typename T::raw) == 4)
-      __builtin_memcpy(&e.b, row + c + 4, 16);
-  } else if (c < C) {
+      e.b = load16<VEC>(row + c + 4);
+  } else if (!VEC && c < C) {
     // no branch a value: each would wait for its load alone
     typename T::raw v[8];
 #pragma unroll
@@ -105,13 +126,13 @@ __device__ __forceinline__ void widen(const Eight& e, float (&v)[8]) {
   }
 }
 
-template <class T, bool VEC>
+template <class T, int VEC>
 __device__ __forceinline__ void load8(const typename T::raw* row, int c,
                                       int C, float (&v)[8]) {
   widen<T>(load8_raw<T, VEC>(row, c, C), v);
 }
 
-template <class T, bool VEC>
+template <class T, int VEC>
 __device__ __forceinline__ void store8(typename T::raw* row, int c, int C,
                                        const float (&v)[8]) {
   if (VEC ? c < C : c + 8 <= C) {
@@ -121,19 +142,16 @@ __device__ __forceinline__ void store8(typename T::raw* row, int c, int C,
       for (int i = 0; i < 4; ++i)
         d[i] = (uint32_t)T::from_f(v[2 * i]) |
                (uint32_t)T::from_f(v[2 * i + 1]) << 16;
-      if constexpr (VEC)
-        *(u32x4*)(row + c) = d;
-      else
-        __builtin_memcpy(row + c, &d, 16);
+      store16<VEC>(row + c, d);
     } else {
-      const f32x4 lo{v[0], v[1], v[2], v[3]}, hi{v[4], v[5], v[6], v[7]};
-      if constexpr (VEC) {
-        *(f32x4*)(row + c) = lo;
-        *(f32x4*)(row + c + 4) = hi;
-      } else {
-        __builtin_memcpy(row + c, &lo, 16);
-        __builtin_memcpy(row + c + 4, &hi, 16);
+      u32x4 lo, hi;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = __builtin_bit_cast(uint32_t, v[i]);
+        hi[i] = __builtin_bit_cast(uint32_t, v[i + 4]);
       }
+      store16<VEC>(row + c, lo);
+      store16<VEC>(row + c + 4, hi);
     }
   } else if constexpr (!VEC) {
 #pragma unroll

@@ -28,8 +28,9 @@ __device__ __forceinline__ Unit unit_of(long long u, int Q) {
 // ------------------------------------------------------------ pack, unpack
 // A wave packs 512 columns of a row, four blocks of 16 lanes, so the maximum
 // takes four DPP steps and the four scales leave as one dword.  24576 x 4096
-// in bf16: packed in 61 us (4.9 TB/s), read back in 71 (4.2 TB/s).
-template <class T, bool VEC>
+// in bf16: packed in 53 us (5.7 TB/s), read back in 46 (6.5 TB/s, the codes
+// partly from the last cache).
+template <class T, int VEC>
 __global__ __launch_bounds__(kThreads) void pack_rows(
     const typename T::raw* __restrict__ x, long long ldx, long long R, int C,
     uint8_t* __restrict__ codes, int Cp, uint32_t* __restrict__ scales,
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(kThreads) void pack_rows(
   }
 }
 
-template <class T, bool VEC>
+template <class T, int VEC>
 __global__ __launch_bounds__(kThreads) void unpack_rows(
     const uint8_t* __restrict__ codes, int Cp,
     const uint32_t* __restrict__ scales, long long Rp, int Q, long long R,
@@ -85,9 +86,10 @@ __global__ __launch_bounds__(kThreads) void unpack_rows(
 // neighbouring rows, so that four rows of one column make one dword of the
 // transposed codes, and 16 lanes (one DPP row) hold a whole row of the tile.
 // Every line of the outputs is written whole.  What a pass packs is one
-// launch: 24576 x 4096 with 14336 x 4096 weights by rows 87 us (5.5 TB/s);
+// launch: 24576 x 4096 with 14336 x 4096 weights by rows 84 us (5.7 TB/s);
 // for its gradients, 24576 x 14336 both ways, the weights' columns and the
-// kept input's, 360 us (5.0 TB/s); 377 with a load at a time a thread.
+// kept input's, 332 us (5.4 TB/s); 357 before the plain rows passed by the
+// caches, 377 with a load at a time a thread.
 struct TileSpace {
   // the transposed codes: dword d of row c lies at d ^ (c / 8 % 8) * 4, so
   // that 16-byte reads take 8 lanes a row without a bank conflict, and the
@@ -132,15 +134,20 @@ __device__ __forceinline__ void pack_tile(const TileJob& a, TileSpace& space,
   } else {
     Eight e[4];
     const auto* x = (const typename T::raw*)a.x;
-    if (a.vec) {
+    if (a.vec == kStream) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        e[i] = load8_raw<T, true>(x + min(r0 + i, a.R - 1ll) * a.ldx, c0,
+        e[i] = load8_raw<T, kStream>(x + min(r0 + i, a.R - 1ll) * a.ldx, c0,
+                                     a.C);
+    } else if (a.vec == kVec) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        e[i] = load8_raw<T, kVec>(x + min(r0 + i, a.R - 1ll) * a.ldx, c0,
                                   a.C);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        e[i] = load8_raw<T, false>(x + min(r0 + i, a.R - 1ll) * a.ldx, c0,
+        e[i] = load8_raw<T, kOdd>(x + min(r0 + i, a.R - 1ll) * a.ldx, c0,
                                    a.C);
     }
 #pragma unroll
@@ -262,7 +269,8 @@ __global__ __launch_bounds__(512) void pack_tiles(TileJobs jobs) {
 // ------------------------------------------------------------ silu(g) * u
 // h = g s u with s = 1 / (1 + exp(-g)); the backward pass uses the 8-bit g~
 // and u~:  dg = dh u~ s (1 + g~ (1 - s)),  du = dh g~ s.
-// 24576 x 14336 in bf16: 612 us forward (4.6 TB/s), 572 backward (4.9 TB/s).
+// 24576 x 14336 in bf16: 560 us forward (5.0 TB/s), 622 backward (4.5 TB/s),
+// which still writes back what the forward pass left in the last cache.
 template <class T>
 __device__ __forceinline__ float sigmoid(float g) {
   if constexpr (sizeof(typename T::raw) == 4)
@@ -271,7 +279,7 @@ __device__ __forceinline__ float sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.f + __expf(-g));
 }
 
-template <class T, bool VEC>
+template <class T, int VEC>
 __global__ __launch_bounds__(kThreads) void swiglu_fwd(
     const typename T::raw* __restrict__ g, long long ldg,
     const typename T::raw* __restrict__ u, long long ldu, long long R, int C,
@@ -300,7 +308,7 @@ __global__ __launch_bounds__(kThreads) void swiglu_fwd(
   }
 }
 
-template <class T, bool VEC>
+template <class T, int VEC>
 __global__ __launch_bounds__(kThreads) void swiglu_bwd(
     const typename T::raw* __restrict__ dh, long long ldh,
     const uint8_t* __restrict__ gc, const uint8_t* __restrict__ uc, int Cp,
@@ -342,8 +350,8 @@ __global__ __launch_bounds__(kThreads) void swiglu_bwd(
 // A row belongs to WPR waves (1 up to 2048 columns, else 4), each lane
 // keeping its 8 * NI values in registers between the sum and the use: four
 // waves share a row where one would need more registers than let others hide
-// its loads.  24576 x 4096 in bf16: 97 us forward (5.2 TB/s), 114 backward
-// (4.4 TB/s) and 6 for the fold; both passes 282 before the backward loaded
+// its loads.  24576 x 4096 in bf16: 96 us forward (5.2 TB/s), 100 backward
+// (5.0 TB/s) and 6 for the fold; both passes 282 before the backward loaded
 // the next row ahead.
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
@@ -363,7 +371,7 @@ __device__ __forceinline__ float row_sum(float x, float (*part)[4],
          part[parity][3];
 }
 
-template <class T, bool VEC, int WPR, int NI>
+template <class T, int VEC, int WPR, int NI>
 __global__ __launch_bounds__(kThreads) void rms_fwd(
     const typename T::raw* __restrict__ x, long long ldx,
     const float* __restrict__ w, long long R, int C, float eps,
@@ -396,7 +404,7 @@ __global__ __launch_bounds__(kThreads) void rms_fwd(
       if (codes)
         pack512(v[i], lane, c, Cp, codes, R, r, scales + q * Rp + r);
       float g[8];
-      load8<Fp32, VEC>(w, c, C, g);
+      load8<Fp32, VEC ? kVec : kOdd>(w, c, C, g);
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[j] *= v[i][j] * inv;
       store8<T, VEC>(y + r * C, c, C, g);
@@ -406,7 +414,7 @@ __global__ __launch_bounds__(kThreads) void rms_fwd(
 
 // dw: every wave adds up its rows in registers and writes one row of
 // partials; the fold sums them in a fixed order, so results repeat.
-template <class T, bool VEC, int WPR, int NI>
+template <class T, int VEC, int WPR, int NI>
 __global__ __launch_bounds__(kThreads, NI <= 2 ? 4 : NI <= 4 ? 2 : 1) void
 rms_bwd(
     const typename T::raw* __restrict__ dy, long long ldy,
@@ -424,7 +432,7 @@ rms_bwd(
   float g[NI][8], dw[NI][8];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    load8<Fp32, VEC>(w, (q0 + i * WPR) * 512 + lane * 8, C, g[i]);
+    load8<Fp32, VEC ? kVec : kOdd>(w, (q0 + i * WPR) * 512 + lane * 8, C, g[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
   }
@@ -488,7 +496,7 @@ rms_bwd(
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int c = (q0 + i * WPR) * 512 + lane * 8;
-    store8<Fp32, VEC>(partials + row * C, c, C, dw[i]);
+    store8<Fp32, VEC ? kVec : kOdd>(partials + row * C, c, C, dw[i]);
   }
 }
 
@@ -521,25 +529,27 @@ static inline int unit_blocks(long long R, int Q) {
   return (int)(want < 8192 ? want : 8192);
 }
 
-// dtype: 0 bf16, 1 fp16, 2 fp32
-#define B8_TYPED(dtype, vec, ...)                   \
-  do {                                              \
-    if (dtype == 0) {                               \
-      using T = Bf16;                               \
-      if (vec) { constexpr bool V = true; __VA_ARGS__; }   \
-      else { constexpr bool V = false; __VA_ARGS__; }      \
-    } else if (dtype == 1) {                        \
-      using T = Fp16;                               \
-      if (vec) { constexpr bool V = true; __VA_ARGS__; }   \
-      else { constexpr bool V = false; __VA_ARGS__; }      \
-    } else {                                        \
-      using T = Fp32;                               \
-      if (vec) { constexpr bool V = true; __VA_ARGS__; }   \
-      else { constexpr bool V = false; __VA_ARGS__; }      \
-    }                                               \
+// dtype: 0 bf16, 1 fp16, 2 fp32; vec: kOdd, kVec or kStream
+#define B8_VEC(vec, ...)                                              \
+  do {                                                                \
+    if (vec == kStream) { constexpr int V = kStream; __VA_ARGS__; }   \
+    else if (vec == kVec) { constexpr int V = kVec; __VA_ARGS__; }    \
+    else { constexpr int V = kOdd; __VA_ARGS__; }                     \
+  } while (0)
+#define B8_TYPED(dtype, vec, ...)                                     \
+  do {                                                                \
+    if (dtype == 0) { using T = Bf16; B8_VEC(vec, __VA_ARGS__); }     \
+    else if (dtype == 1) { using T = Fp16; B8_VEC(vec, __VA_ARGS__); } \
+    else { using T = Fp32; B8_VEC(vec, __VA_ARGS__); }                \
   } while (0)
 
-template <class T, bool V, int WPR, int NI>
+// for results of n values
+static inline int stores_of(int vec, int dtype, long long n) {
+  if (!vec) return kOdd;
+  return n * (dtype == 2 ? 4 : 2) >= kStreamResult ? kStream : kVec;
+}
+
+template <class T, int V, int WPR, int NI>
 static void rms_fwd_run(int blocks, hipStream_t st, const void* x,
                         long long ldx, const float* w, long long R, int C,
                         float eps, void* y, float* inv, uint8_t* codes,
@@ -549,7 +559,7 @@ static void rms_fwd_run(int blocks, hipStream_t st, const void* x,
       codes, Cp, scales, Rp);
 }
 
-template <class T, bool V, int WPR, int NI>
+template <class T, int V, int WPR, int NI>
 static void rms_bwd_run(int blocks, hipStream_t st, const void* dy,
                         long long ldy, const uint8_t* codes, int Cp,
                         const uint32_t* scales, long long Rp, const float* w,
@@ -581,8 +591,8 @@ extern "C" void launch_b8_pack(int dtype, int vec, const void* x,
                                long long Rp, hipStream_t st) {
   const int Q = (Cp + 511) / 512;
   B8_TYPED(dtype, vec,
-           (launch(pack_rows<T, V>, unit_blocks(R, Q), kThreads, st,
-               (const T::raw*)x, ldx, R, C, codes, Cp, scales, Rp, Q)));
+           (launch(pack_rows<T, V ? kVec : kOdd>, unit_blocks(R, Q), kThreads,
+               st, (const T::raw*)x, ldx, R, C, codes, Cp, scales, Rp, Q)));
 }
 
 extern "C" void launch_b8_unpack(int dtype, int vec, const uint8_t* codes,
@@ -592,6 +602,7 @@ extern "C" void launch_b8_unpack(int dtype, int vec, const uint8_t* codes,
   const int Q = (Cp + 511) / 512;
   const float most =
       dtype == 0 ? 0x1.fep127f : dtype == 1 ? 65504.f : 0x1.fffffep127f;
+  vec = stores_of(vec, dtype, R * C);
   B8_TYPED(dtype, vec,
            (launch(unpack_rows<T, V>, unit_blocks(R, Q), kThreads, st,
                codes, Cp, scales, Rp, Q, R, C, (T::raw*)out, most)));
@@ -602,6 +613,8 @@ extern "C" bool launch_b8_tiles(TileJobs* jobs, hipStream_t st) {
   for (int j = 0; j < jobs->count; ++j) {
     TileJob& a = jobs->job[j];
     a.first_block = (int)blocks;
+    if (a.vec && (a.dtype ? 4ll : 2ll) * a.R * a.C >= kStreamOnce)
+      a.vec = kStream;
     blocks += (a.R + 127ll) / 128 * ((a.C + 127ll) / 128);
     // a launch has fewer than 2^32 threads
     if (blocks >= 1ll << 23) return false;
@@ -616,6 +629,7 @@ extern "C" void launch_b8_swiglu_fwd(int dtype, int vec, const void* g,
                                      void* h, uint8_t* gc, uint8_t* uc,
                                      int Cp, uint32_t* gs, uint32_t* us,
                                      long long Rp, hipStream_t st) {
+  vec = stores_of(vec, dtype, R * C);
   const int Q = (Cp + 511) / 512;
   B8_TYPED(dtype, vec,
            (launch(swiglu_fwd<T, V>, unit_blocks(R, Q), kThreads, st,
@@ -629,6 +643,7 @@ extern "C" void launch_b8_swiglu_bwd(int dtype, int vec, const void* dh,
                                      const uint32_t* gs, const uint32_t* us,
                                      long long Rp, long long R, int C,
                                      void* dg, void* du, hipStream_t st) {
+  vec = stores_of(vec, dtype, 2 * R * C);
   const int Q = (Cp + 511) / 512;
   B8_TYPED(dtype, vec,
            (launch(swiglu_bwd<T, V>, unit_blocks(R, Q), kThreads, st,
@@ -641,6 +656,7 @@ extern "C" void launch_b8_rms_fwd(int dtype, int vec, const void* x,
                                   int C, float eps, void* y, float* inv,
                                   uint8_t* codes, int Cp, uint32_t* scales,
                                   long long Rp, hipStream_t st) {
+  vec = stores_of(vec, dtype, R * C);
   const long long groups = C <= 2048 ? (R + 3) / 4 : R;
   const int blocks = (int)(groups < 8192 ? groups : 8192);
   B8_TYPED(dtype, vec,
@@ -667,6 +683,7 @@ extern "C" void launch_b8_rms_bwd(int dtype, int vec, const void* dy,
                                   const float* inv, long long R, int C,
                                   void* dx, float* partials, float* dw,
                                   hipStream_t st) {
+  vec = stores_of(vec, dtype, R * C);
   const int blocks = b8_rms_bwd_blocks(R, C);
   B8_TYPED(dtype, vec,
            B8_ROWS(rms_bwd_run, C, blocks, st, dy, ldy, codes, Cp, scales,

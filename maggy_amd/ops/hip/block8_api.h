@@ -6,6 +6,17 @@
 
 namespace b8 {
 
+// From these sizes on plain rows pass by the caches, so that these keep the
+// packed operands, which every tile of a product reads again: results that
+// the next kernel may want, and what is read once or wanted much later
+// (operands to pack, gradients of weights).  Measured in us, streamed and
+// not: linear8 24576x4096 -> 14336 trained 3480 and 3637, 4096x2048 -> 2 x
+// 8192 427 and 471; 24576 x 4096 normed, with gradients, 198 and 216, packed
+// and read back 100 and 125.  Small results are better found in a cache: a
+// feed-forward of 64 rows takes 57.9 with all streamed and 57.5 with none.
+// Codes always stay: a feed-forward of 512 rows 128, with codes streamed 132.
+constexpr long long kStreamResult = 64 << 20, kStreamOnce = 32 << 20;
+
 // What is packed of a matrix by 128 x 128 tiles (block8.hip): its rows, its
 // columns (the transpose) or both, by blocks of their own or by one scale a
 // tile, from plain numbers or from a packed matrix
@@ -20,6 +31,7 @@ enum TileKind {
 struct TileJob {
   TileKind kind;
   int dtype, vec;       // 0 bf16, 2 fp32; whether 16-byte loads may be used
+                        // (the launcher decides on how)
   int first_block;      // of the launch; a workgroup packs a tile
   const void* x;        // plain numbers, or codes
   const uint32_t* xs;   // codes: their scales
@@ -59,6 +71,7 @@ struct GemmArgs {
   int count[kMaxParts];  // columns of the output
   int parts;
   int f32;  // outputs are fp32, else bf16
+  int stream;  // outputs in bf16 pass by the caches
 };
 
 #ifdef __HIPCC__

@@ -22,6 +22,7 @@
 // The weights are the instruction's first operand: a lane then ends with
 // four neighbouring columns of one row of Y, one 8-byte store.
 #include <hip/hip_runtime.h>
+#include <type_traits>
 
 #include "block8.h"
 #include "block8_api.h"
@@ -100,9 +101,9 @@ __device__ __forceinline__ void store4(const Out& o, int m, int c, f32x4 v) {
 // have more workgroups and more steps in flight, for products too small to
 // fill the card with 256 x 256.
 //
-// Measured for Y of 24576 x 14336, K 4096: 1120 to 1200 us (2.4 to 2.6
+// Measured for Y of 24576 x 14336, K 4096: 1100 to 1160 us (2.5 to 2.6
 // PFLOP/s) on warm cards; 24576 x 4096, K 14336: 1010 to 1060;
-// 14336 x 4096, K 24576 with its split last round: 1040 to 1090.  What
+// 14336 x 4096, K 24576 with its split last round: 1050 to 1070.  What
 // bounds them is power: the matrix units are busy 72, 80 and 79 % of the
 // cycles at a clock that falls from 2.4 to 1.64 GHz, and the products alone,
 // without any load, take 840 us of the 1010.  Of the LDS cycles 5, 1.5 and
@@ -400,21 +401,32 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
   if (left <= 0) return;
   uint16_t* out = (uint16_t*)o.p + o.c0 + c * 8;
   constexpr int kRowsEach = 64 / kChunks;
+  using Pair __attribute__((aligned(2))) = u32x4;
+  auto write = [&](auto stream) {
 #pragma unroll 8
-  for (int k = 0; k < FX * 32 / kRowsEach; ++k) {
-    const int row = k * kRowsEach + lane / kChunks, m = m0 + wm + row;
-    const u32x4 v = *(const u32x4*)(mine + row * kRowBytes +
-                                    ((c ^ row % kChunks) << 4));
-    if (m >= a.M) continue;
-    uint16_t* to = out + (long long)m * o.count;
-    if (left >= 8) {
-      __builtin_memcpy(to, &v, 16);
-    } else {
+    for (int k = 0; k < FX * 32 / kRowsEach; ++k) {
+      const int row = k * kRowsEach + lane / kChunks, m = m0 + wm + row;
+      const u32x4 v = *(const u32x4*)(mine + row * kRowBytes +
+                                      ((c ^ row % kChunks) << 4));
+      if (m >= a.M) continue;
+      uint16_t* to = out + (long long)m * o.count;
+      if (left >= 8) {
+        if constexpr (stream)
+          __builtin_nontemporal_store(v, (Pair*)to);
+        else
+          *(Pair*)to = v;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 7; ++i)
-        if (i < left) to[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+        for (int i = 0; i < 7; ++i)
+          if (i < left) to[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+      }
     }
-  }
+  };
+  // two loops: stores of one loop's two branches would become one store
+  if (a.stream)
+    write(std::true_type());
+  else
+    write(std::false_type());
 }
 
 // the sums of a split tile, in the order of the splits, to the outputs: 4
