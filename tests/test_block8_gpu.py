@@ -674,6 +674,37 @@ def test_offsets_past_32_bits():
     oracle.assert_within(dg[last], wdg, bdg)
 
 
+# operands from 32 MB and results from 64 MB on pass by the caches
+@pytest.mark.parametrize("R,C,dtype", [
+    (9000, 4096, torch.bfloat16), (8191, 4104, torch.float16),
+    (4100, 4096, torch.float32)])
+def test_large_rows_pass_by_the_caches(R, C, dtype):
+    x = _normal((R, C), 1, 2.0, dtype).requires_grad_(True)
+    u = _normal((R, C), 2, 1.0, dtype).requires_grad_(True)
+    w = (1 + 0.2 * _normal((C,), 3, dtype=torch.float32)).requires_grad_(True)
+    d = _normal((R, C), 4, 1.0, dtype)
+    got = ops.unpack8(ops.pack8(x))
+    want = oracle.held(x.detach())
+    assert torch.equal(got.double(), want.to(dtype).double())
+    y = ops.rms_norm8(x, w)
+    grads = torch.autograd.grad(y, (x, w), d)
+    for got, (want, bound) in zip((y, *grads), oracle.rms(
+            x.detach(), w.detach(), d, 1e-5)):
+        oracle.assert_within(got, want, bound)
+    h = ops.swiglu8(x, u)
+    grads = torch.autograd.grad(h, (x, u), d)
+    for got, (want, bound) in zip((h, *grads), oracle.swiglu(
+            x.detach(), u.detach(), d)):
+        oracle.assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("M,K,Ns", [
+    (4500, 4096, (128,)), (64, 4096, (4200,)), (9000, 200, (4096,)),
+    (9001, 130, (4097,)), (300, 4097, (4101, 64))])
+def test_large_operands_pass_by_the_caches(M, K, Ns):
+    _check_linear(*_linear_inputs(M, K, Ns))
+
+
 def test_a_batch_of_many_tokens_trains():
     """dW over a long axis: more K steps than a tile has rows."""
     x, ws, dys = _linear_inputs(40000, 130, (70,))
