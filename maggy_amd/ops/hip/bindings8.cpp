@@ -503,13 +503,17 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
   for (const Tensor* t : {&wcodes, &wscales})
     c10::cuda::CUDACachingAllocator::recordStream(
         t->storage().data_ptr(), at::cuda::getCurrentCUDAStream());
-  // a launch has fewer than 2^32 threads, 16 a row of w
-  if (M >= 1 && M <= 16 && vec8(x) && w.rows() < (int64_t)1 << 28) {
-    std::vector<Tensor> out;
-    const b8::GemmArgs a =
-        gemm_args(mat8(w), M, counts, torch::kBFloat16, x, &out);
-    launch_b8_gemm_bf16(&a, x.data_ptr(), ld(x), (int)K, stream_of(x));
-    return out;
+  if (M >= 1 && vec8(x)) {
+    b8::GemmArgs a{};
+    a.M = (int)std::min(M, (int64_t)1 << 30);
+    a.N = (int)std::min(w.rows(), (int64_t)1 << 30);
+    a.KT = (int)(w.Cp() / 128);
+    if (b8_packs_on_the_way(&a)) {
+      std::vector<Tensor> out;
+      a = gemm_args(mat8(w), M, counts, torch::kBFloat16, x, &out);
+      launch_b8_gemm_bf16(&a, x.data_ptr(), ld(x), (int)K, stream_of(x));
+      return out;
+    }
   }
   return product(mat8(pack_rows(x)), mat8(w), M, counts, torch::kBFloat16, x);
 }

@@ -120,6 +120,8 @@ void launch_b8_rms_bwd(int dtype, int vec, const void* dy, long long ldy,
 long long b8_gemm_workspace(const b8::GemmArgs* args);
 void launch_b8_gemm(const b8::GemmArgs* args, float* workspace,
                     hipStream_t st);
+// the same with x in bf16, packed on the way, if that is the better choice
+bool b8_packs_on_the_way(const b8::GemmArgs* args);
 void launch_b8_gemm_bf16(const b8::GemmArgs* args, const void* x,
                          long long ldx, int K, hipStream_t st);
 }

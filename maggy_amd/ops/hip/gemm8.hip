@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256) void join_splits(GemmArgs a,
 // waves share K, U steps at a time, and load their operands straight from
 // global memory: within a workgroup nothing is read twice, so LDS would save
 // nothing, and there is no barrier before the sums meet in LDS, added in the
-// order of the waves.  With FUSED, for up to 16 rows of bf16, x is packed on
+// order of the waves.  With FUSED, for up to 32 rows of bf16, x is packed on
 // the way: each lane needs 32 neighbouring values a step, which four lanes
 // share a scale for, so the codes are those of pack_rows and a launch is
 // saved.  Bound by the read of w: 8 x 14336, K 4096 takes 13 us (4.5
@@ -552,7 +552,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
   static_assert(4 % U == 0);  // so that U steps have one scale dword a row
   for (int k0 = wave * U; k0 < a.KT; k0 += WAVES * U) {
     i32x4 wv[U][FN][2], xv[U][FUSED ? 1 : FM][2];
-    u32x4 raw[FUSED ? U : 1][4];
+    u32x4 raw[FUSED ? U : 1][FM][4];
     uint32_t wq[FN], xq[FM];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
@@ -569,12 +569,14 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int k = (k0 + u) * 128 + g * 32 + c * 8;
-          raw[u][c] = r < a.M && k < sa.K
-                          ? *(const u32x4*)(sa.x + r * sa.ldx + k)
-                          : u32x4{0, 0, 0, 0};
-        }
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int k = (k0 + u) * 128 + g * 32 + c * 8, m = i * 16 + r;
+            raw[u][i][c] = m < a.M && k < sa.K
+                               ? *(const u32x4*)(sa.x + m * sa.ldx + k)
+                               : u32x4{0, 0, 0, 0};
+          }
     } else {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
         int sx;
         i32x8 xf;
         if constexpr (FUSED) {
-          xf = pack_step(raw[u], &sx);
+          xf = pack_step(raw[u][i], &sx);
         } else {
           const i32x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
           xf = inside ? __builtin_shufflevector(xv[u][i][0], xv[u][i][1], 0,
@@ -765,15 +767,30 @@ extern "C" void launch_b8_gemm(const GemmArgs* args, float* workspace,
     split_run<2, 1, 1, 16, false>(SplitArgs{a}, st);
 }
 
-// x in bf16, at most 16 rows of K columns, K and ldx multiples of 8, packed
-// on the way; the codes of x in args are not read.  A workgroup takes 16
-// columns of y for each FN: more share the packing of x, fewer are more
-// workgroups.  Measured with 1, 2 and 4: 1x2048x2048 4.4, 5.1 and 7.2 us;
-// 16x8192x2048 11.7, 8.7 and 10.3; 8x14336x4096 31, 23.7 and 22.2.
+// Whether x in bf16 is packed on the way: up to 16 rows always, up to 32 where
+// few workgroups repeat the packing.  Measured with a launch for packing and
+// without, 24 rows (N x K): 2048 x 2048 8.0 and 7.1 us, 8192 x 2048 11.0 and
+// 9.0, 8192 x 512 6.9 and 4.9; but 4096 x 4096 11.1 and 11.9, 14336 x 4096
+// 16.9 and 27.9.
+extern "C" bool b8_packs_on_the_way(const GemmArgs* args) {
+  // a launch has fewer than 2^32 threads, 16 a row of w
+  return args->M <= 16 ? args->N < 1 << 28
+                       : args->M <= 32 && args->N <= 8192 && args->KT <= 16;
+}
+
+// x in rows of K columns, K and ldx multiples of 8; the codes of x in args
+// are not read.  A workgroup takes 16 columns of y for each FN: more share
+// the packing of x, fewer are more workgroups.  Measured with 1, 2 and 4:
+// 1x2048x2048 4.4, 5.1 and 7.2 us; 16x8192x2048 11.7, 8.7 and 10.3;
+// 8x14336x4096 31, 23.7 and 22.2; 24x8192x2048 12.7, 9.0 and 17.5.
 extern "C" void launch_b8_gemm_bf16(const GemmArgs* args, const void* x,
                                     long long ldx, int K, hipStream_t st) {
   const SplitArgs sa{*args, (const uint16_t*)x, ldx, K};
-  if (args->N <= 6144)
+  if (args->M > 16 && args->N <= 4096)
+    split_run<2, 1, 1, 16, true>(sa, st);
+  else if (args->M > 16)
+    split_run<2, 2, 1, 16, true>(sa, st);
+  else if (args->N <= 6144)
     split_run<1, 1, 1, 16, true>(sa, st);
   else if (args->N <= 12288)
     split_run<1, 2, 1, 16, true>(sa, st);

@@ -584,7 +584,8 @@ PLANS = [(1, 64, (48,)), (5, 700, (300, 20)), (16, 8, (16,)),
          (700, 384, (700,)), (1025, 1024, (1025,)), (2048, 512, (2048, 700)),
          (3000, 200, (3000,)), (4200, 1536, (2500,)), (4352, 4096, (4352,)),
          (520, 12000, (390,)), (3001, 200, (2999,)), (2047, 512, (2701,)),
-         (4617, 1792, (3457,))]
+         (4617, 1792, (3457,)), (24, 512, (700, 60)), (32, 2048, (4100,)),
+         (31, 1024, (8000,))]
 
 
 @pytest.mark.parametrize("M,K,Ns", PLANS)
@@ -601,20 +602,21 @@ def test_linear8_over_its_kernels(M, K, Ns):
                                      oracle.product_bound(xq, wq))
 
 
-def test_linear8_of_few_rows_holds_what_pack8_holds():
+@pytest.mark.parametrize("M,K", [(16, 3000), (32, 2000)])
+def test_linear8_of_few_rows_holds_what_pack8_holds(M, K):
     """Rows packed on the way are rows packed before: the same codes, so
     results differ by the order of a sum only."""
-    x, ws, _ = _linear_inputs(16, 3000, (200,))
+    x, ws, _ = _linear_inputs(M, K, (200,))
     x[3, 100] = float("inf")
-    x[4, 2999] = float("nan")
+    x[M - 2, K - 1] = float("nan")
     x[5] = 0
     x[6, :] = 1e-39
     x[7, 5] = torch.finfo(torch.bfloat16).max
     xq, wq = oracle.held(x), oracle.held_weight(ws[0])
     with torch.no_grad():
         y = ops.linear8(x, ops.pack_weight8(ws[0]))
-    bad = torch.zeros(16, dtype=torch.bool, device="cuda")
-    bad[[3, 4]] = True
+    bad = torch.zeros(M, dtype=torch.bool, device="cuda")
+    bad[[3, M - 2]] = True
     assert y[bad].isnan().all()
     oracle.assert_within(y[~bad], (xq[~bad] @ wq.t()),
                          oracle.product_bound(xq[~bad], wq))
