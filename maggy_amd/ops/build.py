@@ -48,11 +48,13 @@ def build(verbose=False, force=False):
     os.makedirs(BUILD_DIR, exist_ok=True)
     from torch.utils.cpp_extension import load
 
-    # the generated ninja file knows no header of a .hip source
+    # the generated ninja file knows no header of a .hip source; force
+    # compiles all of it
     newest = max(os.path.getmtime(h) for h in HEADERS)
     for f in os.listdir(BUILD_DIR):
         path = os.path.join(BUILD_DIR, f)
-        if f.endswith(".cuda.o") and os.path.getmtime(path) < newest:
+        if f.endswith(".o") and (force or (
+                f.endswith(".cuda.o") and os.path.getmtime(path) < newest)):
             os.remove(path)
     load(
         name=SO_NAME,
