@@ -121,7 +121,57 @@ Tensor unpack8(Tensor codes, Tensor scales, int64_t C,
   return out;
 }
 
+// A packed matrix in memory that a tensor somewhere owns
+struct Mat8 {
+  uint8_t* c = nullptr;
+  uint32_t* s = nullptr;
+  int64_t rows = 0, Cp = 0, Rp = 0;
+  int64_t code_bytes() const { return up(rows * Cp, 256); }
+  int64_t scale_bytes() const { return up((Cp + 511) / 512 * Rp * 4, 256); }
+};
+Mat8 mat8(const Packed& p) {
+  return {p.c(), p.s(), p.rows(), p.Cp(), p.Rp()};
+}
+
+// Packed matrices, and a run of floats, in one tensor: the temporaries of a
+// call, or what is kept for its backward pass, which lays them out again.
+struct Arena {
+  std::vector<Mat8*> mats;
+  float* floats = nullptr;
+  int64_t n_floats = 0;
+
+  void want(Mat8* m, int64_t rows, int64_t C) {
+    *m = Mat8{nullptr, nullptr, rows, up(C, 128), up(rows, 256)};
+    mats.push_back(m);
+  }
+  int64_t bytes() const {
+    int64_t n = 4 * n_floats;
+    for (const Mat8* m : mats) n += m->code_bytes() + m->scale_bytes();
+    return n;
+  }
+  void lay_out(const Tensor& space, const char* name) {
+    TORCH_CHECK(space.is_cuda() && space.is_contiguous() &&
+                    space.scalar_type() == torch::kUInt8 &&
+                    space.numel() == bytes(),
+                name, ": the gradient does not fit what was kept");
+    uint8_t* at = space.data_ptr<uint8_t>();
+    for (Mat8* m : mats) {
+      m->c = at;
+      m->s = (uint32_t*)(at + m->code_bytes());
+      at += m->code_bytes() + m->scale_bytes();
+    }
+    floats = (float*)at;
+  }
+  Tensor take(const Tensor& like) {
+    Tensor space = torch::empty(
+        {bytes()}, like.options().dtype(torch::kUInt8).requires_grad(false));
+    lay_out(space, "");
+    return space;
+  }
+};
+
 // ------------------------------------------------------------------ swiglu
+// h, then with keep what the backward pass reads
 std::vector<Tensor> swiglu8_fwd(Tensor g, Tensor u, bool keep) {
   g = matrix(g, "g");
   u = matrix(u, "u");
@@ -130,37 +180,39 @@ std::vector<Tensor> swiglu8_fwd(Tensor g, Tensor u, bool keep) {
   same_device(g, u, "u");
   const CUDAGuard guard(g.device());
   const int64_t R = g.size(0), C = g.size(1);
-  Tensor h = torch::empty({R, C}, g.options().requires_grad(false));
-  Packed pg, pu;
-  if (keep) pg = new_packed(R, C, g), pu = new_packed(R, C, g);
+  std::vector<Tensor> out{torch::empty({R, C},
+                                       g.options().requires_grad(false))};
+  Mat8 mg, mu;
+  if (keep) {
+    Arena arena;
+    arena.want(&mg, R, C);
+    arena.want(&mu, R, C);
+    out.push_back(arena.take(g));
+  }
   if (R)
     launch_b8_swiglu_fwd(type_of(g, "g"), vec8(g) && vec8(u), g.data_ptr(),
-                         ld(g), u.data_ptr(), ld(u), R, (int)C, h.data_ptr(),
-                         keep ? pg.c() : nullptr, keep ? pu.c() : nullptr,
-                         (int)up(C, 128), keep ? pg.s() : nullptr,
-                         keep ? pu.s() : nullptr, keep ? pg.Rp() : 0,
-                         stream_of(g));
-  if (!keep) return {h};
-  return {h, pg.codes, pg.scales, pu.codes, pu.scales};
+                         ld(g), u.data_ptr(), ld(u), R, (int)C,
+                         out[0].data_ptr(), mg.c, mu.c, (int)up(C, 128), mg.s,
+                         mu.s, mg.Rp, stream_of(g));
+  return out;
 }
 
-std::vector<Tensor> swiglu8_bwd(Tensor dh, Tensor gc, Tensor gs, Tensor uc,
-                                Tensor us) {
+std::vector<Tensor> swiglu8_bwd(Tensor dh, const Tensor& kept) {
   dh = matrix(dh, "dh");
-  const Packed g = packed(gc, gs, "swiglu8"), u = packed(uc, us, "swiglu8");
   const int64_t R = dh.size(0), C = dh.size(1);
-  TORCH_CHECK(gc.sizes() == uc.sizes() && g.rows() == R &&
-                  g.Cp() == up(C, 128),
-              "swiglu8: the gradient does not fit what was kept");
-  same_device(dh, gc, "g");
-  same_device(dh, uc, "u");
+  Mat8 g, u;
+  Arena arena;
+  arena.want(&g, R, C);
+  arena.want(&u, R, C);
+  arena.lay_out(kept, "swiglu8");
+  same_device(dh, kept, "g");
   const CUDAGuard guard(dh.device());
   const auto o = dh.options().requires_grad(false);
   Tensor dg = torch::empty({R, C}, o), du = torch::empty({R, C}, o);
   if (R)
     launch_b8_swiglu_bwd(type_of(dh, "dh"), vec8(dh), dh.data_ptr(), ld(dh),
-                         g.c(), u.c(), (int)g.Cp(), g.s(), u.s(), g.Rp(), R,
-                         (int)C, dg.data_ptr(), du.data_ptr(), stream_of(dh));
+                         g.c, u.c, (int)g.Cp, g.s, u.s, g.Rp, R, (int)C,
+                         dg.data_ptr(), du.data_ptr(), stream_of(dh));
   return {dg, du};
 }
 
@@ -175,6 +227,7 @@ void check_rms_weight(const Tensor& x, const Tensor& w) {
   same_device(x, w, "weight");
 }
 
+// y, then with keep what the backward pass reads: x and a float a row
 std::vector<Tensor> rms8_fwd(Tensor x, Tensor w, double eps, bool keep) {
   x = matrix(x, "x");
   const int64_t R = x.size(0), C = x.size(1);
@@ -182,42 +235,36 @@ std::vector<Tensor> rms8_fwd(Tensor x, Tensor w, double eps, bool keep) {
               " columns, got ", C);
   check_rms_weight(x, w);
   const CUDAGuard guard(x.device());
-  const auto o = x.options().requires_grad(false);
-  Tensor y = torch::empty({R, C}, o);
-  Packed p;
-  Tensor inv;
+  std::vector<Tensor> out{torch::empty({R, C},
+                                       x.options().requires_grad(false))};
+  Mat8 m;
+  Arena arena;
   if (keep) {
-    p = new_packed(R, C, x);
-    inv = torch::empty({R}, o.dtype(torch::kFloat32));
+    arena.want(&m, R, C);
+    arena.n_floats = R;
+    out.push_back(arena.take(x));
   }
   if (R)
     launch_b8_rms_fwd(type_of(x, "x"),
                       vec8(x) && (uintptr_t)w.data_ptr() % 16 == 0,
                       x.data_ptr(), ld(x), w.data_ptr<float>(), R, (int)C,
-                      (float)eps, y.data_ptr(),
-                      keep ? inv.data_ptr<float>() : nullptr,
-                      keep ? p.c() : nullptr, (int)up(C, 128),
-                      keep ? p.s() : nullptr, keep ? p.Rp() : 0,
-                      stream_of(x));
-  if (!keep) return {y};
-  return {y, p.codes, p.scales, inv};
+                      (float)eps, out[0].data_ptr(), arena.floats, m.c,
+                      (int)up(C, 128), m.s, m.Rp, stream_of(x));
+  return out;
 }
 
-std::vector<c10::optional<Tensor>> rms8_bwd(Tensor dy, Tensor codes,
-                                            Tensor scales, Tensor w,
-                                            Tensor inv, bool need_dx,
+std::vector<c10::optional<Tensor>> rms8_bwd(Tensor dy, const Tensor& kept,
+                                            const Tensor& w, bool need_dx,
                                             bool need_dw) {
   dy = matrix(dy, "dy");
-  const Packed p = packed(codes, scales, "rms_norm8");
   const int64_t R = dy.size(0), C = dy.size(1);
-  TORCH_CHECK(C <= kRmsMost && p.rows() == R && p.Cp() == up(C, 128),
-              "rms_norm8: the gradient does not fit what was kept");
-  TORCH_CHECK(inv.numel() == R && inv.is_contiguous() &&
-                  inv.scalar_type() == torch::kFloat32,
-              "rms_norm8: inv must be float32 [", R, "]");
+  Mat8 x;
+  Arena arena;
+  arena.want(&x, R, C);
+  arena.n_floats = R;
+  arena.lay_out(kept, "rms_norm8");
   check_rms_weight(dy, w);
-  same_device(dy, codes, "codes");
-  same_device(dy, inv, "inv");
+  same_device(dy, kept, "x");
   const CUDAGuard guard(dy.device());
   const auto f32 = dy.options().dtype(torch::kFloat32).requires_grad(false);
   c10::optional<Tensor> dx, dw;
@@ -235,9 +282,9 @@ std::vector<c10::optional<Tensor>> rms8_bwd(Tensor dy, Tensor codes,
   if (R && (need_dx || need_dw))
     launch_b8_rms_bwd(type_of(dy, "dy"),
                       vec8(dy) && (uintptr_t)w.data_ptr() % 16 == 0,
-                      dy.data_ptr(), ld(dy), p.c(), (int)p.Cp(), p.s(),
-                      p.Rp(), w.data_ptr<float>(), inv.data_ptr<float>(), R,
-                      (int)C, dx ? dx->data_ptr() : nullptr,
+                      dy.data_ptr(), ld(dy), x.c, (int)x.Cp, x.s, x.Rp,
+                      w.data_ptr<float>(), arena.floats, R, (int)C,
+                      dx ? dx->data_ptr() : nullptr,
                       need_dw ? partials.data_ptr<float>() : nullptr,
                       need_dw ? dw->data_ptr<float>() : nullptr,
                       stream_of(dy));
@@ -257,40 +304,6 @@ void check_counts(const std::vector<int64_t>& counts) {
               "linear8 takes 1 to ", b8::kMaxParts, " weights, got ",
               counts.size());
 }
-
-// A packed matrix in memory that a tensor somewhere owns
-struct Mat8 {
-  uint8_t* c = nullptr;
-  uint32_t* s = nullptr;
-  int64_t rows = 0, Cp = 0, Rp = 0;
-  int64_t code_bytes() const { return up(rows * Cp, 256); }
-  int64_t scale_bytes() const { return up((Cp + 511) / 512 * Rp * 4, 256); }
-};
-Mat8 mat8(const Packed& p) {
-  return {p.c(), p.s(), p.rows(), p.Cp(), p.Rp()};
-}
-
-// temporaries of one call, in one allocation
-struct Arena {
-  std::vector<Mat8*> mats;
-  void want(Mat8* m, int64_t rows, int64_t C) {
-    *m = Mat8{nullptr, nullptr, rows, up(C, 128), up(rows, 256)};
-    mats.push_back(m);
-  }
-  Tensor take(const Tensor& like) {
-    int64_t bytes = 0;
-    for (Mat8* m : mats) bytes += m->code_bytes() + m->scale_bytes();
-    Tensor space = torch::empty(
-        {bytes}, like.options().dtype(torch::kUInt8).requires_grad(false));
-    uint8_t* at = space.data_ptr<uint8_t>();
-    for (Mat8* m : mats) {
-      m->c = at;
-      m->s = (uint32_t*)(at + m->code_bytes());
-      at += m->code_bytes() + m->scale_bytes();
-    }
-    return space;
-  }
-};
 
 // The packing that a call needs, in one launch.  A job's outputs start at
 // (row_r0, row_c0) of rows and at (col_r0, col_c0) of cols.
@@ -456,8 +469,9 @@ std::vector<Tensor> pack8_weights(std::vector<Tensor> weights) {
   return {p.codes, p.scales};
 }
 
-// outputs, then the codes and scales of x
-std::vector<Tensor> linear8_fwd(Tensor x, std::vector<Tensor> weights) {
+// outputs, then with keep the packed x
+std::vector<Tensor> linear8_fwd(Tensor x, std::vector<Tensor> weights,
+                                bool keep) {
   check_bf16(x);
   x = matrix(x, "x");
   std::vector<int64_t> counts;
@@ -467,11 +481,12 @@ std::vector<Tensor> linear8_fwd(Tensor x, std::vector<Tensor> weights) {
   same_device(x, ws[0], "weight");
   const CUDAGuard guard(x.device());
   const auto first = firsts(counts);
-  const Packed p = new_packed(x.size(0), x.size(1), x);
-  const Mat8 held = mat8(p);
-  Mat8 w;
-  Arena arena;
+  Mat8 held, w;
+  Arena kept, arena;
+  (keep ? kept : arena).want(&held, x.size(0), x.size(1));
   arena.want(&w, first.back(), x.size(1));
+  Tensor kept_space;
+  if (keep) kept_space = kept.take(x);
   const Tensor space = arena.take(x);
   Jobs jobs;
   if (x.size(0))
@@ -479,8 +494,7 @@ std::vector<Tensor> linear8_fwd(Tensor x, std::vector<Tensor> weights) {
   stack_weights(jobs, ws, first, w);
   jobs.run(stream_of(x));
   auto out = product(held, w, x.size(0), counts, torch::kBFloat16, x);
-  out.push_back(p.codes);
-  out.push_back(p.scales);
+  if (keep) out.push_back(kept_space);
   return out;
 }
 
@@ -519,9 +533,7 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
 }
 
 // dx and one dw a weight; dx empty or no dw where they are not asked for
-std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys,
-                                c10::optional<Tensor> codes,
-                                c10::optional<Tensor> scales,
+std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys, const Tensor& kept,
                                 std::vector<Tensor> weights, bool need_dx,
                                 bool need_dw) {
   std::vector<int64_t> counts;
@@ -554,12 +566,11 @@ std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys,
     arena.want(&wt, up(K, 128), N);
   }
   if (need_dw) {
-    TORCH_CHECK(codes && scales, "linear8: nothing was kept of x");
-    const Packed kept = packed(*codes, *scales, "linear8");
-    TORCH_CHECK(kept.rows() == M && kept.Cp() == up(K, 128),
-                "linear8: the gradient does not fit what was kept");
-    same_device(ws[0], kept.codes, "x");
-    x = mat8(kept);
+    TORCH_CHECK(kept.defined(), "linear8: nothing was kept of x");
+    Arena before;
+    before.want(&x, M, K);
+    before.lay_out(kept, "linear8");
+    same_device(ws[0], kept, "x");
     arena.want(&cols, N, M);
     arena.want(&xt, x.Cp, M);
   }
@@ -649,14 +660,14 @@ void no_eager_leaves(const char* name) {
 struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
   static Tensor forward(AutogradContext* ctx, Tensor g, Tensor u) {
     auto out = swiglu8_fwd(g, u, true);
-    ctx->save_for_backward({out[1], out[2], out[3], out[4]});
+    ctx->save_for_backward({out[1]});
     return out[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list dh) {
     no_second_derivative("swiglu8");
     no_eager_leaves("swiglu8");
     const auto k = ctx->get_saved_variables();
-    return swiglu8_bwd(dh[0], k[0], k[1], k[2], k[3]);
+    return swiglu8_bwd(dh[0], k[0]);
   }
 };
 
@@ -673,15 +684,15 @@ struct RMSNorm8 : torch::autograd::Function<RMSNorm8> {
   static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w,
                         double eps) {
     auto out = rms8_fwd(x, w, eps, true);
-    ctx->save_for_backward({out[1], out[2], out[3], w});
+    ctx->save_for_backward({out[1], w});
     return out[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
     no_second_derivative("rms_norm8");
     no_eager_leaves("rms_norm8");
     const auto k = ctx->get_saved_variables();
-    auto d = rms8_bwd(dy[0], k[0], k[1], k[3], k[2],
-                      ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    auto d = rms8_bwd(dy[0], k[0], k[1], ctx->needs_input_grad(0),
+                      ctx->needs_input_grad(1));
     return {d[0].value_or(Tensor()), d[1].value_or(Tensor()), Tensor()};
   }
 };
@@ -702,13 +713,12 @@ struct Linear8 : torch::autograd::Function<Linear8> {
     variable_list weights{w0};
     for (const Maybe& w : {w1, w2, w3})
       if (w) weights.push_back(*w);
-    auto out = linear8_fwd(x, weights);
+    // dX does not read x
     bool dw = false;
     for (const Tensor& w : weights) dw = dw || w.requires_grad();
+    auto out = linear8_fwd(x, weights, dw);
     variable_list kept(weights);
-    // dX does not read x
     kept.push_back(dw ? out[weights.size()] : Tensor());
-    kept.push_back(dw ? out[weights.size() + 1] : Tensor());
     ctx->save_for_backward(kept);
     out.resize(weights.size());
     return out;
@@ -717,15 +727,13 @@ struct Linear8 : torch::autograd::Function<Linear8> {
     no_second_derivative("linear8");
     no_eager_leaves("linear8");
     auto kept = ctx->get_saved_variables();
-    const size_t n = kept.size() - 2;
-    c10::optional<Tensor> codes, scales;
-    if (kept[n].defined()) codes = kept[n], scales = kept[n + 1];
+    const size_t n = kept.size() - 1;
+    const Tensor x = kept[n];
     kept.resize(n);
     bool need_dw = false;
     for (size_t i = 0; i < n; ++i)
       need_dw = need_dw || ctx->needs_input_grad(1 + i);
-    auto d = linear8_bwd(dys, codes, scales, kept, ctx->needs_input_grad(0),
-                         need_dw);
+    auto d = linear8_bwd(dys, x, kept, ctx->needs_input_grad(0), need_dw);
     d.resize(1 + b8::kMaxParts);
     for (size_t i = 0; i < n; ++i)
       if (!ctx->needs_input_grad(1 + i)) d[1 + i] = Tensor();
@@ -746,8 +754,7 @@ std::vector<Tensor> linear8(Tensor x, std::vector<Tensor> weights) {
     };
     out = Linear8::apply(x, weights[0], at(1), at(2), at(3));
   } else {
-    out = linear8_fwd(x, weights);
-    out.resize(weights.size());
+    out = linear8_fwd(x, weights, false);
   }
   for (Tensor& y : out) y = as_shape(y, lead);
   return out;
