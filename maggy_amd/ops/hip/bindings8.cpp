@@ -10,8 +10,6 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 
-#include <limits>
-
 #include "block8_api.h"
 
 namespace {

@@ -833,3 +833,31 @@ def test_two_threads_at_once():
         for out in outs:
             for a, b in zip(out, exact):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("how", ["again", "again, reentrant", "on the CPU"])
+def test_what_is_kept_may_be_kept_elsewhere(how):
+    """Recomputed in the backward pass, or held in host memory meanwhile."""
+    from torch.utils.checkpoint import checkpoint
+
+    norm = ops.MaggyRMSNorm8(256).cuda()
+    ff = ops.MaggyFeedForward8(256, 384).cuda().bfloat16()
+    x = _normal((70, 256), 1).requires_grad_(True)
+    dy = _normal((70, 256), 2)
+    params = [x, *norm.parameters(), *ff.parameters()]
+
+    def grads(y):
+        for p in params:
+            p.grad = None
+        y.backward(dy)
+        return [p.grad for p in params]
+
+    want = grads(ff(norm(x)))
+    if how == "on the CPU":
+        with torch.autograd.graph.save_on_cpu():
+            y = ff(norm(x))
+    else:
+        y = checkpoint(lambda x: ff(norm(x)), x,
+                       use_reentrant="reentrant" in how)
+    for a, b in zip(grads(y), want):
+        assert torch.equal(a, b)
