@@ -439,8 +439,9 @@ class Linear8Group:
         """``owner``: the ident of the one thread that reads what is packed.
         It orders its streams after this one and keeps what its graphs
         read."""
-        self._held = (pack_weight8(*(m.weight for m in self.linears)),
-                      self._state(), owner)
+        of = self._state()  # before: what changes meanwhile is noticed
+        self._held = (pack_weight8(*(m.weight for m in self.linears)), of,
+                      owner)
 
     def drop(self, captured=False):
         self._held = None

@@ -308,6 +308,24 @@ def test_weights_made_in_inference_mode_pack():
 
 
 @torch.no_grad()
+def test_weights_changed_while_they_are_packed(monkeypatch):
+    from maggy_amd.ops import block8
+
+    m, x = _group()
+    want = 2 * m(x)
+    pack = block8.pack_weight8
+
+    def changed_meanwhile(*weights):
+        packed = pack(*weights)
+        m.weight.mul_(2)
+        return packed
+
+    monkeypatch.setattr(block8, "pack_weight8", changed_meanwhile)
+    ops.pack8_model(m)
+    assert torch.equal(m(x), want)
+
+
+@torch.no_grad()
 def test_weights_dropped_by_another_thread_meanwhile(monkeypatch):
     m, x = _group()
     want = m(x)
