@@ -164,9 +164,11 @@ class Attention(nn.Module):
             # whole cache every decoded token (~1 GB/token at 8B b8)
             if cache.get("kbuf") is None:
                 cap = int(cache.get("cap", pos + T + 256))
-                cache["kbuf"] = k.new_empty(
+                # zeros: the masked step reads all of it, and a masked value
+                # times a NaN that happens to be there is NaN
+                cache["kbuf"] = k.new_zeros(
                     B, self.n_kv_heads, cap, self.head_dim)
-                cache["vbuf"] = v.new_empty(
+                cache["vbuf"] = v.new_zeros(
                     B, self.n_kv_heads, cap, self.head_dim)
                 cache["len"] = 0
             if cache.get("idx") is not None:

@@ -272,6 +272,18 @@ def test_llama_in_8_bits_decodes():
     assert torch.equal(got, out)
 
 
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_masked_decoding_reads_no_memory_as_it_was(eight_bit, monkeypatch):
+    m = _llama(eight_bit).eval()
+    prompt = torch.randint(0, 97, (2, 5))
+    want = m.generate(prompt, max_new_tokens=6)
+    monkeypatch.setattr(
+        torch.Tensor, "new_empty",
+        lambda self, *size: self.new_full(size, float("nan")))
+    got = m.generate_captured(prompt, max_new_tokens=6, use_graph=False)
+    assert torch.equal(got, want)
+
+
 def _group(N=48, K=96, dtype=torch.float32):
     torch.manual_seed(0)
     m = ops.MaggyLinear8(K, N).to(dtype)
