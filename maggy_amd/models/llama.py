@@ -139,8 +139,8 @@ class Attention(nn.Module):
         self.wo = MaggyLinear(cfg.n_heads * self.head_dim, cfg.dim)
         self.qkv8 = self.out8 = None
         if cfg.eight_bit:
-            self.qkv8 = Linear8Group(self.wq, self.wk, self.wv)
-            self.out8 = Linear8Group(self.wo)
+            self.qkv8 = Linear8Group(self, "wq", "wk", "wv")
+            self.out8 = Linear8Group(self, "wo")
 
     def _project_out(self, x):
         return self.wo(x) if self.out8 is None else self.out8(x)

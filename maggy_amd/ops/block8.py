@@ -403,26 +403,70 @@ def _linear8_packed_cpu(x, w):
 
 
 # ------------------------------------------------------------------- modules
+_FORWARDS = [nn.Linear.forward, MaggyLinear.forward]
+
+
+def _plain(m):
+    """Whether calling ``m`` is x @ weight^T and nothing else."""
+    return (isinstance(m, nn.Linear) and type(m).forward in _FORWARDS
+            and "forward" not in vars(m)
+            and m._parameters.get("weight") is not None and m.bias is None)
+
+
+def _agree(weights):
+    first = weights[0]
+    return all(w.shape[1] == first.shape[1] and w.dtype == first.dtype
+               and w.device == first.device for w in weights[1:])
+
+
+def _products(x, weights):
+    """``linear8``, one product where the weights allow it."""
+    if _agree(weights):
+        return linear8(x, *weights)
+    return tuple(linear8(x, w) for w in weights)
+
+
 class Linear8Group:
     """Bias-free linear modules that read the same input, run as one
-    ``linear8``.  ``pack`` keeps their weights packed for calls without
+    ``linear8``: the children of ``module`` that have these ``names`` when
+    the group is called, or ``module`` itself.  A child that is no plain
+    bias-free linear (an ablated one, an adapter) is called as it is; the
+    others stay one product.
+
+    ``pack`` keeps their weights packed for calls without
     gradients, until ``drop``, a call with gradients (training is about to
     change them) or a change of the weights themselves.  A HIP graph goes on
     with the weights as they were packed when it was captured; they are kept
     for it until ``drop(captured=True)``."""
 
-    def __init__(self, *linears):
-        for m in linears:
-            if m.bias is not None:
-                raise ValueError("linear8 has no bias")
-        self.linears = linears
+    def __init__(self, module, *names):
+        self.module = module
+        self.names = names
         # (Weight8, what it was packed from, the only thread that reads it)
         self._held = None
         self._captured = []
+        for m in self.linears:
+            if m.bias is not None:
+                raise ValueError("linear8 has no bias")
 
     def __getstate__(self):
         # a copy packs its own: its weights count their versions anew
-        return {"linears": self.linears, "_held": None, "_captured": []}
+        return {"module": self.module, "names": self.names, "_held": None,
+                "_captured": []}
+
+    @property
+    def linears(self):
+        if not self.names:
+            return (self.module,)
+        return tuple(getattr(self.module, n) for n in self.names)
+
+    def _plain(self):
+        """Whether each linear's part is its product and nothing else."""
+        if self.names:
+            return [_plain(m) for m in self.linears]
+        if self.module.bias is not None:
+            raise ValueError("linear8 has no bias")
+        return [True]  # its call is what runs this
 
     @property
     def packed(self):
@@ -438,10 +482,14 @@ class Linear8Group:
     def pack(self, owner=None):
         """``owner``: the ident of the one thread that reads what is packed.
         It orders its streams after this one and keeps what its graphs
-        read."""
+        read.  Linears that cannot be one product are not packed."""
+        linears = self.linears
+        if not (all(self._plain()) and
+                _agree([m.weight for m in linears])):
+            self._held = None
+            return
         of = self._state()  # before: what changes meanwhile is noticed
-        self._held = (pack_weight8(*(m.weight for m in self.linears)), of,
-                      owner)
+        self._held = (pack_weight8(*(m.weight for m in linears)), of, owner)
 
     def drop(self, captured=False):
         self._held = None
@@ -449,6 +497,9 @@ class Linear8Group:
             self._captured = []
 
     def __call__(self, x):
+        linears, plain = self.linears, self._plain()
+        if not all(plain):
+            return self._apart(x, linears, plain)
         held = self._held  # another thread may drop it meanwhile
         if held is not None:
             packed, of, owner = held
@@ -458,7 +509,17 @@ class Linear8Group:
                 self.drop()
             elif self._may_read(x, packed, owner):
                 return linear8(x, packed)
-        return linear8(x, *(m.weight for m in self.linears))
+        return _products(x, [m.weight for m in linears])
+
+    def _apart(self, x, linears, plain):
+        """What is no plain linear runs by its own call."""
+        if torch.is_grad_enabled():
+            self.drop()
+        weights = [m.weight for m, p in zip(linears, plain) if p]
+        ys = _products(x, weights) if weights else ()
+        ys = iter(ys if isinstance(ys, tuple) else (ys,))
+        out = [next(ys) if p else m(x) for m, p in zip(linears, plain)]
+        return tuple(out) if len(out) > 1 else out[0]
 
     def _may_read(self, x, packed, owner):
         if owner is not None:
@@ -481,6 +542,9 @@ class MaggyLinear8(MaggyLinear):
         return self.group(x)
 
 
+_FORWARDS.append(MaggyLinear8.forward)
+
+
 class MaggyRMSNorm8(MaggyRMSNorm):
     """Drop-in MaggyRMSNorm on ``rms_norm8``."""
 
@@ -495,8 +559,8 @@ class MaggyFeedForward8(MaggyFeedForward):
 
     def __init__(self, dim, ffn_hidden):
         super().__init__(dim, ffn_hidden)
-        self.up8 = Linear8Group(self.w1, self.w3)
-        self.down8 = Linear8Group(self.w2)
+        self.up8 = Linear8Group(self, "w1", "w3")
+        self.down8 = Linear8Group(self, "w2")
 
     def forward(self, x):
         return self.down8(swiglu8(*self.up8(x)))
@@ -517,7 +581,8 @@ def pack8_model(module):
     devices = set()
     for g in groups8(module):
         g.pack()
-        devices.add(g.packed.device)
+        if g.packed is not None:
+            devices.add(g.packed.device)
     for device in devices:
         if device.type == "cuda" and \
                 not torch.cuda.is_current_stream_capturing():

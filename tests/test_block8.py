@@ -360,3 +360,113 @@ def test_bench_refuses_8_bits_of_other_models(monkeypatch):
     monkeypatch.setattr("sys.argv", ["bench.py", "--eight-bit", "--model",
                                      "llama8b"])
     assert bench.parse_args().eight_bit
+
+
+# ------------------------------------------ what a group's owner holds now
+class _Doubled(torch.nn.Module):
+    def __init__(self, linear):
+        super().__init__()
+        self.linear = linear
+
+    def forward(self, x):
+        return 2 * self.linear(x)
+
+
+def _set(model, path, child):
+    parent = model.get_submodule(path.rpartition(".")[0])
+    setattr(parent, path.rpartition(".")[2], child)
+
+
+@pytest.mark.parametrize("path", ["layers.0.attn.wq", "layers.0.attn.wo"])
+@torch.no_grad()
+def test_an_ablated_projection_is_gone(path):
+    from maggy_amd.ablation.ablationstudy import drop_layers
+
+    m = _llama(True).eval()
+    tokens = torch.randint(0, 97, (2, 9))
+    before = m(tokens)
+    other = copy.deepcopy(m)
+    attn = other.layers[0].attn
+    if path.endswith("wq"):
+        attn.qkv8 = lambda x: (x, *ops.linear8(x, attn.wk.weight,
+                                               attn.wv.weight))
+    else:
+        attn.out8 = lambda x: x
+    want = other(tokens)
+    drop_layers(m, path)
+    assert torch.equal(m(tokens), want) and not torch.equal(want, before)
+    ops.pack8_model(m)
+    assert torch.equal(m(tokens), want)
+    assert torch.equal(m.generate(tokens, 3), m.generate_captured(
+        tokens, 3, use_graph=False))
+
+
+@pytest.mark.parametrize("path", ["layers.0.attn.wk", "layers.1.attn.wo",
+                                  "layers.0.ffn.w1", "layers.0.ffn.w3",
+                                  "layers.1.ffn.w2"])
+def test_a_replaced_linear_is_the_one_that_runs(path):
+    m = _llama(True)
+    other = copy.deepcopy(m)
+    tokens = torch.randint(0, 97, (2, 9))
+    old = m.get_submodule(path)
+    new = torch.nn.Linear(old.in_features, old.out_features, bias=False)
+    _set(m, path, new)
+    with torch.no_grad():
+        other.get_submodule(path).weight.copy_(new.weight)
+        want = other(tokens)
+        assert torch.equal(m(tokens), want)
+        ops.pack8_model(m)
+        assert torch.equal(m(tokens), want)
+    m(tokens).sum().backward()
+    assert new.weight.grad is not None and old.weight.grad is None
+    # every parameter that is listed takes part
+    assert all(p.grad is not None for p in m.parameters())
+
+
+def test_an_adapter_around_a_linear_runs():
+    m = _llama(True)
+    other = copy.deepcopy(m)
+    tokens = torch.randint(0, 97, (2, 9))
+    attn, theirs = m.layers[0].attn, other.layers[0].attn
+    v = torch.nn.Linear(*attn.wv.weight.t().shape, bias=False)
+    o = torch.nn.Linear(*attn.wo.weight.t().shape, bias=False)
+    attn.wv, attn.wo = _Doubled(v), _Doubled(o)
+    theirs.qkv8 = lambda x: (*ops.linear8(x, theirs.wq.weight,
+                                          theirs.wk.weight), 2 * v(x))
+    theirs.out8 = lambda x: 2 * o(x)
+    assert torch.equal(m(tokens), other(tokens))
+    m(tokens).sum().backward()
+    assert all(p.grad is not None for p in m.parameters())
+
+
+@torch.no_grad()
+def test_a_linear_with_a_bias_and_one_of_another_type_run():
+    ff = ops.MaggyFeedForward8(64, 96)
+    x = _normal(5, 64)
+    biased = torch.nn.Linear(96, 64)
+    ff.w2 = biased
+    want = biased(ops.swiglu8(*ops.linear8(x, ff.w1.weight, ff.w3.weight)))
+    assert torch.equal(ff(x), want)
+    ff.w3.bfloat16()  # not of w1's type: not one product with it
+    want = biased(ops.swiglu8(ops.linear8(x, ff.w1.weight),
+                              ops.linear8(x, ff.w3.weight)))
+    assert torch.equal(ff(x), want)
+    ops.pack8_model(ff)
+    assert torch.equal(ff(x), want)
+    lin = ops.MaggyLinear8(40, 30)
+    lin.bias = torch.nn.Parameter(torch.ones(30))
+    with pytest.raises(ValueError, match="bias"):
+        lin(_normal(3, 40))
+
+
+@torch.no_grad()
+def test_a_module_that_extends_the_8_bit_linear():
+    class Doubled(ops.MaggyLinear8):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    m, x = Doubled(40, 30), _normal(3, 40)
+    want = 2 * ops.linear8(x, m.weight)
+    assert torch.equal(m(x), want)
+    ops.pack8_model(m)
+    assert torch.equal(m(x), want) and m.group.packed is not None
