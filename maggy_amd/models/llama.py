@@ -19,6 +19,7 @@ import torch.nn.functional as F
 
 from maggy_amd.ops.block8 import (
     Linear8Group,
+    Linear8Member,
     MaggyFeedForward8,
     MaggyRMSNorm8,
     groups8,
@@ -133,10 +134,11 @@ class Attention(nn.Module):
         # MaggyLinear = nn.Linear running on the in-tree MFMA GEMM
         # (fwd + both backward layouts) when the shapes tile; eager/rocBLAS
         # fallback otherwise (tiny CPU configs)
-        self.wq = MaggyLinear(cfg.dim, cfg.n_heads * self.head_dim)
-        self.wk = MaggyLinear(cfg.dim, cfg.n_kv_heads * self.head_dim)
-        self.wv = MaggyLinear(cfg.dim, cfg.n_kv_heads * self.head_dim)
-        self.wo = MaggyLinear(cfg.n_heads * self.head_dim, cfg.dim)
+        linear = Linear8Member if cfg.eight_bit else MaggyLinear
+        self.wq = linear(cfg.dim, cfg.n_heads * self.head_dim)
+        self.wk = linear(cfg.dim, cfg.n_kv_heads * self.head_dim)
+        self.wv = linear(cfg.dim, cfg.n_kv_heads * self.head_dim)
+        self.wo = linear(cfg.n_heads * self.head_dim, cfg.dim)
         self.qkv8 = self.out8 = None
         if cfg.eight_bit:
             self.qkv8 = Linear8Group(self, "wq", "wk", "wv")

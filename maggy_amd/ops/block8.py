@@ -29,6 +29,7 @@ import threading
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
+from torch.nn.modules.module import _has_any_global_hook
 
 from maggy_amd import ops
 from maggy_amd.ops.fused_rms import MaggyRMSNorm
@@ -403,14 +404,31 @@ def _linear8_packed_cpu(x, w):
 
 
 # ------------------------------------------------------------------- modules
-_FORWARDS = [nn.Linear.forward, MaggyLinear.forward]
+class Linear8Member(MaggyLinear):
+    """A child of a ``Linear8Group``'s module, in 8 bits also by a call of
+    its own: the group makes that call where somebody waits for it (hooks, a
+    pruned or parametrized weight)."""
+
+    def forward(self, x):
+        return linear8(x, self.weight)
 
 
-def _plain(m):
-    """Whether calling ``m`` is x @ weight^T and nothing else."""
-    return (isinstance(m, nn.Linear) and type(m).forward in _FORWARDS
-            and "forward" not in vars(m)
-            and m._parameters.get("weight") is not None and m.bias is None)
+_FORWARDS = [nn.Linear.forward, MaggyLinear.forward, Linear8Member.forward]
+
+
+def _plain_weight(m):
+    """The weight of ``m`` if calling it is x @ weight^T and nothing else."""
+    if type(m) is not Linear8Member and not (
+            isinstance(m, nn.Linear) and type(m).forward in _FORWARDS
+            and m.bias is None):
+        return None
+    own = m.__dict__
+    if (own["_forward_hooks"] or own["_forward_pre_hooks"]
+            or own["_backward_hooks"] or own["_backward_pre_hooks"]
+            or "forward" in own or "bias" in own):
+        return None
+    params = own["_parameters"]
+    return params.get("weight") if params.get("bias") is None else None
 
 
 def _agree(weights):
@@ -426,12 +444,19 @@ def _products(x, weights):
     return tuple(linear8(x, w) for w in weights)
 
 
+def _same(now, then):
+    for a, b in zip(now, then):
+        if not a or a[0] is not b[0] or a[1:] != b[1:]:
+            return False
+    return True
+
+
 class Linear8Group:
     """Bias-free linear modules that read the same input, run as one
     ``linear8``: the children of ``module`` that have these ``names`` when
     the group is called, or ``module`` itself.  A child that is no plain
-    bias-free linear (an ablated one, an adapter) is called as it is; the
-    others stay one product.
+    bias-free linear (an ablated one, an adapter) or has hooks is called as
+    it is; the others stay one product.
 
     ``pack`` keeps their weights packed for calls without
     gradients, until ``drop``, a call with gradients (training is about to
@@ -460,13 +485,18 @@ class Linear8Group:
             return (self.module,)
         return tuple(getattr(self.module, n) for n in self.names)
 
-    def _plain(self):
-        """Whether each linear's part is its product and nothing else."""
-        if self.names:
-            return [_plain(m) for m in self.linears]
-        if self.module.bias is not None:
-            raise ValueError("linear8 has no bias")
-        return [True]  # its call is what runs this
+    def _weights(self):
+        """The weights, None for a linear whose call is more than its
+        product."""
+        if not self.names:  # the module's own call is what runs this
+            if self.module.bias is not None:
+                raise ValueError("linear8 has no bias")
+            return [self.module.weight]
+        if _has_any_global_hook():
+            return [None] * len(self.names)
+        # this is part of every decoded token: no attribute lookups
+        children = self.module._modules
+        return [_plain_weight(children.get(n)) for n in self.names]
 
     @property
     def packed(self):
@@ -475,21 +505,20 @@ class Linear8Group:
 
     def _state(self):
         # tensors made in inference mode count no versions
-        return [(m.weight, m.weight.device, m.weight.dtype,
-                 None if m.weight.is_inference() else m.weight._version)
-                for m in self.linears]
+        return [w is not None and (
+            w, w.device, w.dtype, None if w.is_inference() else w._version)
+                for w in self._weights()]
 
     def pack(self, owner=None):
         """``owner``: the ident of the one thread that reads what is packed.
         It orders its streams after this one and keeps what its graphs
         read.  Linears that cannot be one product are not packed."""
-        linears = self.linears
-        if not (all(self._plain()) and
-                _agree([m.weight for m in linears])):
+        weights = self._weights()
+        if any(w is None for w in weights) or not _agree(weights):
             self._held = None
             return
         of = self._state()  # before: what changes meanwhile is noticed
-        self._held = (pack_weight8(*(m.weight for m in linears)), of, owner)
+        self._held = (pack_weight8(*weights), of, owner)
 
     def drop(self, captured=False):
         self._held = None
@@ -497,28 +526,30 @@ class Linear8Group:
             self._captured = []
 
     def __call__(self, x):
-        linears, plain = self.linears, self._plain()
-        if not all(plain):
-            return self._apart(x, linears, plain)
         held = self._held  # another thread may drop it meanwhile
         if held is not None:
             packed, of, owner = held
-            if torch.is_grad_enabled() or not all(
-                    a[0] is b[0] and a[1:] == b[1:]
-                    for a, b in zip(self._state(), of)):
+            if torch.is_grad_enabled():
                 self.drop()
-            elif self._may_read(x, packed, owner):
-                return linear8(x, packed)
-        return _products(x, [m.weight for m in linears])
+            else:
+                now = self._state()
+                if _same(now, of):
+                    if self._may_read(x, packed, owner):
+                        return linear8(x, packed)
+                elif all(now):  # a hook may go again
+                    self.drop()
+        weights = self._weights()
+        if any(w is None for w in weights):
+            return self._apart(x, weights)
+        return _products(x, weights)
 
-    def _apart(self, x, linears, plain):
+    def _apart(self, x, weights):
         """What is no plain linear runs by its own call."""
-        if torch.is_grad_enabled():
-            self.drop()
-        weights = [m.weight for m, p in zip(linears, plain) if p]
-        ys = _products(x, weights) if weights else ()
+        plain = [w for w in weights if w is not None]
+        ys = _products(x, plain) if plain else ()
         ys = iter(ys if isinstance(ys, tuple) else (ys,))
-        out = [next(ys) if p else m(x) for m, p in zip(linears, plain)]
+        out = [m(x) if w is None else next(ys)
+               for m, w in zip(self.linears, weights)]
         return tuple(out) if len(out) > 1 else out[0]
 
     def _may_read(self, x, packed, owner):
@@ -556,6 +587,8 @@ class MaggyFeedForward8(MaggyFeedForward):
     """Llama FFN w2(silu(w1 x) * w3 x) in 8 bits: w1 and w3 share one packed
     input and one product, and all that the backward pass keeps is 8-bit
     (x, both halves and their product), 1 byte a value."""
+
+    linear_class = Linear8Member
 
     def __init__(self, dim, ffn_hidden):
         super().__init__(dim, ffn_hidden)

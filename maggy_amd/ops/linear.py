@@ -135,11 +135,13 @@ class MaggyFeedForward(nn.Module):
     """Llama FFN: w2(silu(w1 x) * w3 x) with the custom GEMM everywhere
     and SwiGLU fused into the w3 GEMM's epilogue."""
 
+    linear_class = MaggyLinear
+
     def __init__(self, dim, ffn_hidden):
         super().__init__()
-        self.w1 = MaggyLinear(dim, ffn_hidden)
-        self.w3 = MaggyLinear(dim, ffn_hidden)
-        self.w2 = MaggyLinear(ffn_hidden, dim)
+        self.w1 = self.linear_class(dim, ffn_hidden)
+        self.w3 = self.linear_class(dim, ffn_hidden)
+        self.w2 = self.linear_class(ffn_hidden, dim)
 
     def forward(self, x):
         if use_custom_linear(x, self.w1.weight):

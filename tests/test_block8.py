@@ -6,6 +6,7 @@ import torch
 
 from maggy_amd import ops
 from maggy_amd.exceptions import HipExtensionMissingError  # noqa: F401
+from maggy_amd.ops.block8 import groups8
 from tests import _block8_oracle as oracle
 
 
@@ -470,3 +471,90 @@ def test_a_module_that_extends_the_8_bit_linear():
     assert torch.equal(m(x), want)
     ops.pack8_model(m)
     assert torch.equal(m(x), want) and m.group.packed is not None
+
+
+@pytest.mark.parametrize("path", ["layers.0.attn.wq", "layers.0.attn.wo",
+                                  "layers.1.ffn.w1", "layers.1.ffn.w2"])
+@torch.no_grad()
+def test_hooks_of_a_linear_run(path):
+    m = _llama(True).eval()
+    tokens = torch.randint(0, 97, (2, 9))
+    want, seen = m(tokens), []
+    lin = m.get_submodule(path)
+    for packed in (False, True):
+        if packed:
+            ops.pack8_model(m)
+        hooks = [lin.register_forward_pre_hook(
+                     lambda mod, args: seen.append(args[0])),
+                 lin.register_forward_hook(
+                     lambda mod, args, out: seen.append(out))]
+        assert torch.equal(m(tokens), want)  # seen, and still in 8 bits
+        x, y = seen
+        assert torch.equal(y, ops.linear8(x, lin.weight))
+        for h in hooks:
+            h.remove()
+        seen.clear()
+        hook = lin.register_forward_hook(lambda mod, args, out: 0 * out)
+        assert not torch.equal(m(tokens), want)
+        hook.remove()
+        assert torch.equal(m(tokens), want) and not seen
+    # the group read its packed weights again
+    assert all(g.packed is not None for g in groups8(m))
+
+
+def test_hooks_of_all_modules_and_of_gradients_run():
+    from torch.nn.modules import module as every
+
+    ff, seen = ops.MaggyFeedForward8(64, 96), []
+    x = _normal(5, 64).requires_grad_(True)
+    hook = every.register_module_forward_hook(
+        lambda mod, args, out: seen.append(mod))
+    ff(x)
+    hook.remove()
+    assert all(any(m is s for s in seen) for m in (ff.w1, ff.w2, ff.w3))
+    hook = ff.w3.register_full_backward_hook(
+        lambda mod, dx, dy: seen.append(dy[0]))
+    seen.clear()
+    ff(x).sum().backward()
+    assert len(seen) == 1 and seen[0].shape == (5, 96)
+    hook.remove()
+
+
+def test_a_pruned_linear_trains():
+    from torch.nn.utils import prune
+
+    ff, x = ops.MaggyFeedForward8(64, 96), _normal(5, 64)
+    prune.l1_unstructured(ff.w1, "weight", amount=0.5)
+    mask = ff.w1.weight_mask
+    for _ in range(3):
+        y = ff(x)
+        y.sum().backward()
+        grad = ff.w1.weight_orig.grad
+        assert grad is not None and (grad[mask == 0] == 0).all()
+        with torch.no_grad():
+            for p in ff.parameters():
+                p -= 0.1 * p.grad
+                p.grad = None
+    with torch.no_grad():
+        want = ops.linear8(ops.swiglu8(*ops.linear8(
+            x, ff.w1.weight_orig * mask, ff.w3.weight)), ff.w2.weight)
+        assert torch.equal(ff(x), want)
+
+
+@torch.no_grad()
+def test_a_parametrized_and_a_patched_linear_run():
+    from torch.nn.utils import parametrize
+
+    class Halved(torch.nn.Module):
+        def forward(self, w):
+            return w / 2
+
+    ff, x = ops.MaggyFeedForward8(64, 96), _normal(5, 64)
+    parametrize.register_parametrization(ff.w3, "weight", Halved())
+    ff.w2.forward = lambda x: x
+    for _ in range(2):
+        g, u = ops.linear8(x, ff.w1.weight, ff.w3.weight)
+        want = ops.swiglu8(g, u)
+        assert torch.equal(ff(x), want)
+        ops.pack8_model(ff)
+        ff.w3.parametrizations.weight.original.mul_(3)
