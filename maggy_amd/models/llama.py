@@ -239,23 +239,23 @@ class Block(nn.Module):
 
 
 def _packed_while(generate):
-    """Decode with the 8-bit weights packed once a call, unless the caller
-    has packed them (``pack8_model``)."""
+    """Decode with the 8-bit weights packed once a call, for this thread
+    alone, unless what the caller has packed (``pack8_model``) still holds
+    for them."""
     @functools.wraps(generate)
     def run(self, *args, **kw):
-        groups = groups8(self)
-        fresh = [g for g in groups if g.packed is None]
+        me, made, kept = threading.get_ident(), [], []
         try:
-            for g in fresh:
-                g.pack(owner=threading.get_ident())
-            # a graph that generate captures reads these to its end
-            held = [g.packed for g in groups]
-            out = generate(self, *args, **kw)
-            del held
-            return out
+            for g in groups8(self):
+                packed, fresh = g.pack_own()
+                if fresh:
+                    made.append(g)
+                # a graph that generate captures reads these to its end
+                kept.append(packed)
+            return generate(self, *args, **kw)
         finally:
-            for g in fresh:
-                g.drop()
+            for g in made:
+                g.drop_own(me)
     return run
 
 

@@ -458,17 +458,17 @@ class Linear8Group:
     bias-free linear (an ablated one, an adapter) or has hooks is called as
     it is; the others stay one product.
 
-    ``pack`` keeps their weights packed for calls without
-    gradients, until ``drop``, a call with gradients (training is about to
-    change them) or a change of the weights themselves.  A HIP graph goes on
-    with the weights as they were packed when it was captured; they are kept
-    for it until ``drop(captured=True)``."""
+    ``pack`` keeps their weights packed for calls without gradients, for all
+    threads or for one, until ``drop``, a call with gradients (training is
+    about to change them) or a change of the weights themselves.  A HIP graph
+    goes on with the weights as they were packed when it was captured; they
+    are kept for it until ``drop(captured=True)``."""
 
     def __init__(self, module, *names):
         self.module = module
         self.names = names
-        # (Weight8, what it was packed from, the only thread that reads it)
-        self._held = None
+        self._held = None  # (Weight8, what it was packed from)
+        self._own = {}  # the same by the only thread that reads it
         self._captured = []
         for m in self.linears:
             if m.bias is not None:
@@ -477,7 +477,7 @@ class Linear8Group:
     def __getstate__(self):
         # a copy packs its own: its weights count their versions anew
         return {"module": self.module, "names": self.names, "_held": None,
-                "_captured": []}
+                "_own": {}, "_captured": []}
 
     @property
     def linears(self):
@@ -500,8 +500,11 @@ class Linear8Group:
 
     @property
     def packed(self):
-        held = self._held
-        return None if held is None else held[0]
+        """What is packed for all threads, else for any one."""
+        for held in (self._held, *self._own.copy().values()):
+            if held is not None:
+                return held[0]
+        return None
 
     def _state(self):
         # tensors made in inference mode count no versions
@@ -513,31 +516,65 @@ class Linear8Group:
         """``owner``: the ident of the one thread that reads what is packed.
         It orders its streams after this one and keeps what its graphs
         read.  Linears that cannot be one product are not packed."""
-        weights = self._weights()
-        if any(w is None for w in weights) or not _agree(weights):
-            self._held = None
-            return
+        held = None
         of = self._state()  # before: what changes meanwhile is noticed
-        self._held = (pack_weight8(*weights), of, owner)
+        if all(of):
+            weights = [s[0] for s in of]
+            if _agree(weights):
+                held = pack_weight8(*weights), of
+        if owner is None:
+            self._held = held
+        elif held is not None:
+            self._own[owner] = held
+        return None if held is None else held[0]
 
     def drop(self, captured=False):
         self._held = None
+        self._own.clear()
         if captured:
             self._captured = []
 
+    def drop_own(self, owner):
+        """Drop what was packed for this one thread."""
+        self._own.pop(owner, None)
+
+    def _readable(self):
+        """What this thread may read of what is packed, and whether that is
+        packed for all threads; None if nothing is."""
+        shared = self._held  # another thread may drop it meanwhile
+        own = self._own and self._own.get(threading.get_ident())
+        if not (shared or own):
+            return None
+        now = self._state()
+        if own and _same(now, own[1]):
+            return own[0], False
+        if shared and _same(now, shared[1]):
+            return shared[0], True
+        if all(now):  # changed, and not only hooked for some time
+            self.drop_own(threading.get_ident())
+            if shared is self._held:
+                self._held = None
+        return None
+
+    def pack_own(self):
+        """Pack for this thread what it could not read packed; returns what
+        it reads then, and whether this call packed it."""
+        found = self._readable()
+        if found is not None:
+            return found[0], False
+        return self.pack(owner=threading.get_ident()), True
+
     def __call__(self, x):
-        held = self._held  # another thread may drop it meanwhile
-        if held is not None:
-            packed, of, owner = held
+        if self._held or self._own:
             if torch.is_grad_enabled():
                 self.drop()
             else:
-                now = self._state()
-                if _same(now, of):
-                    if self._may_read(x, packed, owner):
-                        return linear8(x, packed)
-                elif all(now):  # a hook may go again
-                    self.drop()
+                found = self._readable()
+                if found is not None:
+                    packed, shared = found
+                    if shared:  # else the thread that packed it keeps it
+                        self._keep_for_graph(x, packed)
+                    return linear8(x, packed)
         weights = self._weights()
         if any(w is None for w in weights):
             return self._apart(x, weights)
@@ -552,14 +589,11 @@ class Linear8Group:
                for m, w in zip(self.linears, weights)]
         return tuple(out) if len(out) > 1 else out[0]
 
-    def _may_read(self, x, packed, owner):
-        if owner is not None:
-            return owner == threading.get_ident()
+    def _keep_for_graph(self, x, packed):
         # a captured call reads what it was captured with at every replay
         if x.is_cuda and torch.cuda.is_current_stream_capturing() \
                 and not any(p is packed for p in self._captured):
             self._captured.append(packed)
-        return True
 
 
 class MaggyLinear8(MaggyLinear):

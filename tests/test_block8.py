@@ -558,3 +558,95 @@ def test_a_parametrized_and_a_patched_linear_run():
         assert torch.equal(ff(x), want)
         ops.pack8_model(ff)
         ff.w3.parametrizations.weight.original.mul_(3)
+
+
+# ------------------------------------------------- packing while it decodes
+@pytest.fixture
+def packings(monkeypatch):
+    """How many weights were put in 8 bits, by a pack or on the way."""
+    from maggy_amd.ops import block8
+
+    count, held = [], block8._held_weight
+
+    def counted(w):
+        count.append(w.shape)
+        return held(w)
+
+    monkeypatch.setattr(block8, "_held_weight", counted)
+    return count
+
+
+def _decode(m, prompt, captured):
+    if captured:
+        return m.generate_captured(prompt, 9, use_graph=False)
+    return m.generate(prompt, 9)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_changed_weights_are_packed_once_a_decode(captured, packings):
+    m = _llama(True).eval()
+    prompt = torch.randint(0, 97, (2, 5))
+    _decode(m, prompt, captured)
+    once = len(packings)
+    assert once == 14  # seven a layer
+    ops.pack8_model(m)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(1.5)
+    packings.clear()
+    got = _decode(m, prompt, captured)
+    assert len(packings) == once
+    ops.drop8_model(m)
+    assert torch.equal(got, _decode(m, prompt, captured))
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_decodes_of_two_threads_pack_once_each(captured, packings):
+    import threading
+
+    m = _llama(True).eval()
+    prompt = torch.randint(0, 97, (2, 5))
+    want = _decode(m, prompt, captured)
+    once, inside, done = len(packings), threading.Event(), threading.Event()
+    packings.clear()
+
+    class Waits(torch.nn.Module):
+        def forward(self, x):
+            if threading.current_thread() is other:
+                inside.set()
+                assert done.wait(60)
+            return x
+
+    # the other thread stops in the middle of its decode
+    m.norm = torch.nn.Sequential(Waits(), m.norm)
+    got = []
+    other = threading.Thread(
+        target=lambda: got.append(_decode(m, prompt, captured)))
+    other.start()
+    try:
+        assert inside.wait(60)
+        mine = _decode(m, prompt, captured)
+        assert len(packings) == 2 * once
+    finally:
+        done.set()
+        other.join()
+    assert torch.equal(mine, want) and torch.equal(got[0], want)
+    assert len(packings) == 2 * once
+    assert all(g.packed is None for g in groups8(m))
+
+
+def test_a_decode_leaves_what_others_packed_meanwhile():
+    m = _llama(True).eval()
+    prompt = torch.randint(0, 97, (2, 5))
+    norm = m.norm
+
+    class Packs(torch.nn.Module):
+        def forward(self, x):
+            ops.pack8_model(m)
+            m.norm = norm
+            return norm(x)
+
+    m.norm = Packs()
+    got = m.generate(prompt, 6)
+    assert all(g.packed is not None for g in groups8(m))
+    assert torch.equal(m.generate(prompt, 6), got)
