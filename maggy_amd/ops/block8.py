@@ -25,6 +25,7 @@ All run as HIP kernels on GPU tensors and raise without the extension; on the
 CPU the same definitions run in torch.
 """
 import threading
+import weakref
 
 import torch
 import torch.nn as nn
@@ -444,6 +445,22 @@ def _products(x, weights):
     return tuple(linear8(x, w) for w in weights)
 
 
+_packing = weakref.WeakSet()  # the groups that ever packed their weights
+_lock = threading.Lock()
+
+
+def weights_written(params):
+    """Drop what was packed of ``params``: for code that writes weights
+    behind torch's back, as the fused optimizers' kernels do."""
+    with _lock:
+        groups = list(_packing)
+    if groups:
+        written = {id(p) for p in params}
+        for g in groups:
+            if any(id(w) in written for w in g.reads()):
+                g.drop()
+
+
 def _same(now, then):
     for a, b in zip(now, then):
         if not a or a[0] is not b[0] or a[1:] != b[1:]:
@@ -470,6 +487,7 @@ class Linear8Group:
         self._held = None  # (Weight8, what it was packed from)
         self._own = {}  # the same by the only thread that reads it
         self._captured = []
+        self._drops = 0  # how often it was dropped
         for m in self.linears:
             if m.bias is not None:
                 raise ValueError("linear8 has no bias")
@@ -477,7 +495,7 @@ class Linear8Group:
     def __getstate__(self):
         # a copy packs its own: its weights count their versions anew
         return {"module": self.module, "names": self.names, "_held": None,
-                "_own": {}, "_captured": []}
+                "_own": {}, "_captured": [], "_drops": 0}
 
     @property
     def linears(self):
@@ -516,23 +534,39 @@ class Linear8Group:
         """``owner``: the ident of the one thread that reads what is packed.
         It orders its streams after this one and keeps what its graphs
         read.  Linears that cannot be one product are not packed."""
-        held = None
+        with _lock:
+            _packing.add(self)
+        held, drops = None, self._drops
         of = self._state()  # before: what changes meanwhile is noticed
         if all(of):
             weights = [s[0] for s in of]
             if _agree(weights):
                 held = pack_weight8(*weights), of
-        if owner is None:
-            self._held = held
-        elif held is not None:
-            self._own[owner] = held
+        with _lock:
+            if drops != self._drops:  # dropped while it was packed
+                held = None
+            if owner is None:
+                self._held = held
+            elif held is not None:
+                self._own[owner] = held
         return None if held is None else held[0]
 
     def drop(self, captured=False):
-        self._held = None
-        self._own.clear()
+        with _lock:
+            self._drops += 1
+            self._held = None
+            self._own.clear()
         if captured:
             self._captured = []
+
+    def reads(self):
+        """The weights as they are, and as they were packed."""
+        linears = [self.module._modules.get(n) for n in self.names]
+        ws = [getattr(m, "weight", None) for m in linears or [self.module]]
+        for held in (self._held, *self._own.copy().values()):
+            if held is not None:
+                ws += [state[0] for state in held[1]]
+        return ws
 
     def drop_own(self, owner):
         """Drop what was packed for this one thread."""
@@ -641,10 +675,11 @@ def groups8(module):
 
 def pack8_model(module):
     """Pack the weights of every 8-bit linear of a model for serving.  A call
-    with gradients or a change of a weight drops that layer's; code that
-    writes weights behind torch's back, through ``.data`` or kernels of its
-    own, calls this again, or ``drop8_model``.  All streams and threads may
-    use what is packed."""
+    with gradients, a step of the framework's optimizers or a change of a
+    weight drops that layer's.  Code that writes weights behind torch's back
+    calls this again, or ``drop8_model``: through ``.data``, by kernels of
+    its own, by replaying a graph that trains, or into weights that were made
+    in inference mode.  All streams and threads may use what is packed."""
     devices = set()
     for g in groups8(module):
         g.pack()

@@ -160,6 +160,7 @@ class FusedAdam(_FusedOptimizerBase):
                     g["weight_decay"], 1.0 - b1 ** self._step_count,
                     1.0 - b2 ** self._step_count, norm,
                     self.max_grad_norm or 0.0, 1.0 / self.grad_scale)
+            ops.block8.weights_written(p for _, p in pairs)
         else:
             self._cpu_step(pairs)
         return loss
@@ -235,6 +236,7 @@ class FusedSGD(_FusedOptimizerBase):
                     g["weight_decay"], g["dampening"], g["nesterov"],
                     first, norm, self.max_grad_norm or 0.0,
                     1.0 / self.grad_scale)
+            ops.block8.weights_written(p for _, p in pairs)
         else:
             self._cpu_step(pairs, first)
         return loss

@@ -23,6 +23,7 @@ Only public torch.distributed APIs are used (the private
 import torch
 import torch.distributed as dist
 
+from maggy_amd.ops.block8 import weights_written
 from maggy_amd.ops.fused_adam import FusedAdam, FusedSGD
 
 # coalesced-exchange bucket: xGMI links move ~153 GB/s; 128 MB buckets keep
@@ -131,6 +132,7 @@ class _ZeroShardedBase(torch.optim.Optimizer):
                 dist.broadcast(flat, src=src, group=pg)
                 if r != self.rank:
                     _unflatten_into(flat, bucket)
+        weights_written(self._all_params)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -170,3 +172,4 @@ def broadcast_module_params(module, src=0, process_group=None):
         dist.broadcast(flat, src=src, group=pg)
         if dist.get_rank(pg) != src:
             _unflatten_into(flat, bucket)
+    weights_written(module.parameters())

@@ -650,3 +650,57 @@ def test_a_decode_leaves_what_others_packed_meanwhile():
     got = m.generate(prompt, 6)
     assert all(g.packed is not None for g in groups8(m))
     assert torch.equal(m.generate(prompt, 6), got)
+
+
+# ---------------------------------------- weights written by the framework
+def _zero_rank(rank, path):
+    import torch.distributed as dist
+
+    from maggy_amd.parallel.zero import ZeroFusedSGD, broadcast_module_params
+
+    dist.init_process_group("gloo", init_method="file://" + path, rank=rank,
+                            world_size=2)
+    torch.manual_seed(rank)
+    m = torch.nn.Sequential(*[ops.MaggyLinear8(32, 32) for _ in range(3)])
+    x = _normal(4, 32)
+
+    def agrees():
+        with torch.no_grad():
+            want = x
+            for lin in m:
+                want = ops.linear8(want, lin.weight)
+            assert torch.equal(m(x), want)
+
+    ops.pack8_model(m)
+    broadcast_module_params(m)
+    agrees()
+    opt = ZeroFusedSGD(list(m.parameters()), lr=0.5)
+    m(x).square().sum().backward()
+    ops.pack8_model(m)  # between the gradients and the step
+    opt.step()
+    agrees()
+    dist.destroy_process_group()
+
+
+@pytest.mark.timeout(120)
+def test_packed_weights_that_another_rank_updates(tmp_path):
+    torch.multiprocessing.spawn(_zero_rank, (str(tmp_path / "store"),), 2)
+
+
+@torch.no_grad()
+def test_weights_written_behind_torch_while_they_are_packed(monkeypatch):
+    from maggy_amd.ops import block8
+
+    m, x = _group()
+    want = 2 * m(x)
+    pack = block8.pack_weight8
+
+    def written_meanwhile(*weights):
+        packed = pack(*weights)
+        m.weight.data.mul_(2)
+        block8.weights_written(m.parameters())
+        return packed
+
+    monkeypatch.setattr(block8, "pack_weight8", written_meanwhile)
+    ops.pack8_model(m)
+    assert torch.equal(m(x), want)

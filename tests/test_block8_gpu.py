@@ -861,3 +861,24 @@ def test_what_is_kept_may_be_kept_elsewhere(how):
                        use_reentrant="reentrant" in how)
     for a, b in zip(grads(y), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("wtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["FusedAdam", "FusedSGD"])
+def test_packed_weights_that_the_optimizer_updates(kind, wtype):
+    """Packed between the gradients and the step, whose kernels write."""
+    m = torch.nn.Sequential(*[ops.MaggyLinear8(256, 256) for _ in range(2)])
+    m = m.cuda().to(wtype)
+    other = ops.MaggyLinear8(256, 256).cuda().bfloat16()
+    x = _normal((4, 256), 1)
+    opt = getattr(ops, kind)(m.parameters(), lr=0.1)
+    m(x).float().square().sum().backward()
+    ops.pack8_model(m)
+    ops.pack8_model(other)
+    with torch.no_grad():
+        before = m(x)
+        opt.step()
+        got = m(x)
+        want = ops.linear8(ops.linear8(x, m[0].weight), m[1].weight)
+    assert torch.equal(got, want) and not torch.equal(got, before)
+    assert other.group.packed is not None  # not of this optimizer
