@@ -22,13 +22,15 @@ matrix unit aligns the products of 8-bit numbers before it adds them, which
 is worth about 16 bits, well inside bfloat16 but not float32.
 
 All run as HIP kernels on GPU tensors and raise without the extension; on the
-CPU the same definitions run in torch.
+CPU the same definitions run in torch.  Derivatives are first ones in reverse
+mode; others are refused.
 """
 import threading
 import weakref
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.nn.modules.module import _has_any_global_hook
 
@@ -395,6 +397,8 @@ def _check_input(x, K, device):
 
 
 def _linear8_packed_cpu(x, w):
+    if forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError("linear8 has no forward-mode derivative")
     values = _unpack_cpu(w.codes, w.scales, w.columns, torch.float32)
     held, ys, at = _held(_rows(x)), [], 0
     for n in w.counts:

@@ -631,6 +631,13 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// a tangent would be lost without a word
+void no_forward_mode(const char* name, at::ArrayRef<Tensor> ts) {
+  for (const Tensor& t : ts)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), name,
+                " has no forward-mode derivative");
+}
+
 void no_second_derivative(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name,
               " has no second derivative: backward cannot create a graph");
@@ -670,6 +677,7 @@ struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
 };
 
 Tensor swiglu8(Tensor g, Tensor u) {
+  no_forward_mode("swiglu8", {g, u});
   const auto lead = g.sizes().slice(0, g.dim() - 1).vec();
   g = as_rows(g);
   u = as_rows(u);
@@ -696,6 +704,7 @@ struct RMSNorm8 : torch::autograd::Function<RMSNorm8> {
 };
 
 Tensor rms_norm8(Tensor x, Tensor w, double eps) {
+  no_forward_mode("rms_norm8", {x, w});
   const auto lead = x.sizes().slice(0, x.dim() - 1).vec();
   x = as_rows(x);
   return as_shape(wants_grad({&x, &w}) ? RMSNorm8::apply(x, w, eps)
@@ -740,6 +749,8 @@ struct Linear8 : torch::autograd::Function<Linear8> {
 };
 
 std::vector<Tensor> linear8(Tensor x, std::vector<Tensor> weights) {
+  no_forward_mode("linear8", x);
+  no_forward_mode("linear8", weights);
   const auto lead = x.sizes().slice(0, x.dim() - 1).vec();
   x = as_rows(x);
   bool grad = wants_grad({&x});
@@ -761,6 +772,7 @@ std::vector<Tensor> linear8(Tensor x, std::vector<Tensor> weights) {
 std::vector<Tensor> linear8_on_packed(Tensor x, Tensor codes, Tensor scales,
                                       std::vector<int64_t> counts,
                                       int64_t K) {
+  no_forward_mode("linear8", x);
   const auto lead = x.sizes().slice(0, x.dim() - 1).vec();
   auto out = linear8_packed(as_rows(x), codes, scales, counts, K);
   for (Tensor& y : out) y = as_shape(y, lead);

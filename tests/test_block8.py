@@ -704,3 +704,28 @@ def test_weights_written_behind_torch_while_they_are_packed(monkeypatch):
     monkeypatch.setattr(block8, "pack_weight8", written_meanwhile)
     ops.pack8_model(m)
     assert torch.equal(m(x), want)
+
+
+# ------------------------------------------------- forward-mode derivatives
+def _forward_mode_calls(x, w, n):
+    packed = ops.pack_weight8(w)
+    return [lambda t: ops.swiglu8(t, x), lambda t: ops.swiglu8(x, t),
+            lambda t: ops.rms_norm8(t, n), lambda t: ops.linear8(t, w),
+            lambda t: ops.linear8(t, w, w), lambda t: ops.linear8(t, packed)]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    from torch.autograd import forward_ad
+
+    x, w, n = _normal(4, 32), _normal(8, 32), torch.ones(32)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in _forward_mode_calls(x, w, n):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call(dual)
+            call(x)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ops.linear8(x, forward_ad.make_dual(w, torch.ones_like(w)))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ops.rms_norm8(x, forward_ad.make_dual(n, torch.ones_like(n)))

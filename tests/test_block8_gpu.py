@@ -882,3 +882,24 @@ def test_packed_weights_that_the_optimizer_updates(kind, wtype):
         want = ops.linear8(ops.linear8(x, m[0].weight), m[1].weight)
     assert torch.equal(got, want) and not torch.equal(got, before)
     assert other.group.packed is not None  # not of this optimizer
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    from torch.autograd import forward_ad
+
+    from tests.test_block8 import _forward_mode_calls
+
+    x, w = _normal((4, 32), 1), _normal((8, 32), 2)
+    n = torch.ones(32, device="cuda")
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for i, call in enumerate(_forward_mode_calls(x, w, n)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+                print("not refused:", i)
+            call(x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.linear8(x, forward_ad.make_dual(w, torch.ones_like(w)))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.rms_norm8(x, forward_ad.make_dual(n, torch.ones_like(n)))
