@@ -389,13 +389,20 @@ std::vector<Tensor> weights_of(const std::vector<Tensor>& weights,
 }
 
 // the product of packed w with x, packed (M rows) or, for a few rows, plain
-// bf16 that the kernel packs on the way; like: a tensor of their device
+// bf16 that the kernel packs on the way; like: a tensor of their device.  The
+// outputs are the parts of w that counts tells, or with width > 0 those of x,
+// of width columns each.
 b8::GemmArgs gemm_args(const Mat8& w, int64_t M,
-                       const std::vector<int64_t>& counts,
+                       const std::vector<int64_t>& counts, int64_t width,
                        torch::ScalarType dtype, const Tensor& like,
                        std::vector<Tensor>* out) {
   const auto first = firsts(counts);
-  TORCH_CHECK(M < (int64_t)1 << 30 && first.back() < (int64_t)1 << 30,
+  const int64_t N = width ? w.rows : std::min(first.back(), w.rows);
+  TORCH_CHECK(width <= w.rows && (!width || M == first[counts.size() - 1] +
+                                                    counts.back()),
+              "linear8: outputs do not match the product");
+  TORCH_CHECK(M < (int64_t)1 << 30 && first.back() < (int64_t)1 << 30 &&
+                  N < (int64_t)1 << 30,
               "linear8: too many rows");
   // the kernel reaches a matrix's scales by 32-bit offsets
   const int64_t quads = (w.Cp + 511) / 512;
@@ -408,13 +415,16 @@ b8::GemmArgs gemm_args(const Mat8& w, int64_t M,
   a.wn = w.rows;
   a.wsp = w.Rp;
   a.M = (int)M;
-  a.N = (int)std::min(first.back(), w.rows);
+  a.N = (int)N;
   a.KT = (int)(w.Cp / 128);
   a.parts = (int)counts.size();
+  a.by_rows = width > 0;
+  a.width = (int)width;
   a.f32 = dtype == torch::kFloat32;
   const auto o = like.options().dtype(dtype).requires_grad(false);
   for (size_t i = 0; i < counts.size(); ++i) {
-    out->push_back(torch::empty({M, counts[i]}, o));
+    out->push_back(width ? torch::empty({counts[i], width}, o)
+                         : torch::empty({M, counts[i]}, o));
     a.out[i] = (*out)[i].data_ptr();
     a.first[i] = (int)first[i];
     a.count[i] = (int)counts[i];
@@ -422,19 +432,20 @@ b8::GemmArgs gemm_args(const Mat8& w, int64_t M,
   return a;
 }
 
-// soon: the next kernels are going to read the outputs
+// width: the outputs are parts of x (gemm_args), gradients that are wanted
+// later; otherwise the next kernels are going to read them
 std::vector<Tensor> product(const Mat8& x, const Mat8& w, int64_t M,
                             const std::vector<int64_t>& counts,
                             torch::ScalarType dtype, const Tensor& like,
-                            bool soon = true) {
+                            int64_t width = 0) {
   TORCH_CHECK(x.Cp == w.Cp && M <= x.rows, "linear8: columns do not match");
   std::vector<Tensor> out;
-  b8::GemmArgs a = gemm_args(w, M, counts, dtype, like, &out);
+  b8::GemmArgs a = gemm_args(w, M, counts, width, dtype, like, &out);
   a.x = x.c;
   a.xs = x.s;
   a.xn = x.rows;
   a.xsp = x.Rp;
-  a.stream = 2 * M * a.N >= (soon ? b8::kStreamResult : b8::kStreamOnce);
+  a.stream = 2 * M * a.N >= (width ? b8::kStreamOnce : b8::kStreamResult);
   if (M) {
     const long long bytes = b8_gemm_workspace(&a);
     TORCH_CHECK(bytes >= 0, "linear8: matrix is too large");
@@ -522,7 +533,7 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
     a.KT = (int)(w.Cp() / 128);
     if (b8_packs_on_the_way(&a)) {
       std::vector<Tensor> out;
-      a = gemm_args(mat8(w), M, counts, torch::kBFloat16, x, &out);
+      a = gemm_args(mat8(w), M, counts, 0, torch::kBFloat16, x, &out);
       launch_b8_gemm_bf16(&a, x.data_ptr(), ld(x), (int)K, stream_of(x));
       return out;
     }
@@ -592,17 +603,11 @@ std::vector<Tensor> linear8_bwd(std::vector<Tensor> dys, const Tensor& kept,
   if (need_dx)
     out[0] = product(rows, wt, M, {K}, torch::kBFloat16, ws[0])[0];
   if (need_dw) {
-    // dW [N][K], all weights' rows in one product; a weight's own rows of it
-    // are contiguous
-    const Tensor all = product(cols, xt, first[counts.size() - 1] +
-                                             counts.back(),
-                               {K}, ws[0].scalar_type(), ws[0], false)[0];
-    for (size_t i = 0; i < counts.size(); ++i)
-      out.push_back(counts.size() == 1
-                        ? all
-                        : torch::empty({0}, o).set_(
-                              all.storage(), first[i] * K, {counts[i], K},
-                              {K, 1}));
+    // all weights' dW in one product, a tensor each
+    for (Tensor& dw : product(cols, xt, first[counts.size() - 1] +
+                                            counts.back(),
+                              counts, ws[0].scalar_type(), ws[0], K))
+      out.push_back(std::move(dw));
   }
   return out;
 }

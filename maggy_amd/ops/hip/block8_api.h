@@ -49,7 +49,8 @@ struct TileJob {
 
 // Y[m][n] = sum_k X[m][k] W[n][k], X and W packed along k (gemm8.hip).
 // The rows of W are up to four matrices, each padded to a multiple of 128
-// rows; each has a contiguous output of its own.
+// rows; each has a contiguous output of its own.  Or the rows of X are, where
+// X is the gradients of several outputs and Y those of their weights.
 constexpr int kMaxParts = 4;
 // all packing that one call of linear8 needs is one launch
 constexpr int kMaxJobs = 2 * kMaxParts + 1;
@@ -67,9 +68,11 @@ struct GemmArgs {
   int M, N;  // rows of x and of w that take part
   int KT;    // K steps of 128
   void* out[kMaxParts];
-  int first[kMaxParts];  // first row of w
-  int count[kMaxParts];  // columns of the output
+  int first[kMaxParts];  // first row of w, or of x
+  int count[kMaxParts];  // columns of the output, or rows
   int parts;
+  int by_rows;  // the parts are rows of x
+  int width;    // then: columns of every output
   int f32;  // outputs are fp32, else bf16
   int stream;  // outputs in bf16 pass by the caches
 };

@@ -41,18 +41,29 @@ __device__ __forceinline__ int swizzled(int row, int chunk) {
   return row * 128 + ((chunk ^ (row >> 1 & 7)) << 4);
 }
 
-// where a wave's columns go: they lie inside one of the outputs, as both
-// start at multiples of 128 rows of w
+// where a wave's results go: its rows and columns lie inside one of the
+// outputs, as both start at multiples of 128 rows of w, or of x
 struct Out {
-  void* p;
-  int c0, count, f32;
+  char* p;  // of row 0, column 0
+  int c0, count, rows, f32;
 };
-__device__ __forceinline__ Out out_of(const GemmArgs& a, int n) {
-  Out o{a.out[0], n - a.first[0], a.count[0], a.f32};
+__device__ __forceinline__ Out out_of(const GemmArgs& a, int m, int n) {
+  const int at = a.by_rows ? m : n;
+  Out o{(char*)a.out[0], 0, a.count[0], 0, a.f32};
+  int first = 0;
 #pragma unroll
   for (int k = 1; k < kMaxParts; ++k)
-    if (k < a.parts && n >= a.first[k])
-      o.p = a.out[k], o.c0 = n - a.first[k], o.count = a.count[k];
+    if (k < a.parts && at >= a.first[k])
+      o.p = (char*)a.out[k], first = a.first[k], o.count = a.count[k];
+  if (a.by_rows) {
+    o.p -= (long long)first * a.width * (a.f32 ? 4 : 2);
+    o.rows = first + o.count;
+    o.count = a.width;
+    o.c0 = n;
+  } else {
+    o.rows = a.M;
+    o.c0 = n - first;
+  }
   return o;
 }
 
@@ -355,12 +366,12 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
                                     acc[i][4 * r + 2], acc[i][4 * r + 3]};
     return;
   }
-  const Out o = out_of(a, n0 + wn);
+  const Out o = out_of(a, m0 + wm, n0 + wn);
   if (o.f32) {
 #pragma unroll
     for (int i = 0; i < FX; ++i) {
       const int m = m0 + wm + i * 32 + frow;
-      if (m < a.M) {
+      if (m < o.rows) {
 #pragma unroll
         for (int j = 0; j < FW; ++j)
 #pragma unroll
@@ -408,7 +419,7 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
       const int row = k * kRowsEach + lane / kChunks, m = m0 + wm + row;
       const u32x4 v = *(const u32x4*)(mine + row * kRowBytes +
                                       ((c ^ row % kChunks) << 4));
-      if (m >= a.M) continue;
+      if (m >= o.rows) continue;
       uint16_t* to = out + (long long)m * o.count;
       if (left >= 8) {
         if constexpr (stream)
@@ -447,12 +458,11 @@ __global__ __launch_bounds__(256) void join_splits(GemmArgs a,
   f32x4 v = p[0];
   for (int s = 1; s < work.splits; ++s)
     v += p[(long long)s * 4 * kProducts * 256];
-  const int m = it.m0 + (wave >> 1) * (BM / 2) + frag / FW * 32 + (lane & 31);
-  const int wn = (wave & 1) * (BN / 2);
-  if (m < a.M) {
-    const Out o = out_of(a, it.n0 + wn);
+  const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+  const int m = it.m0 + wm + frag / FW * 32 + (lane & 31);
+  const Out o = out_of(a, it.m0 + wm, it.n0 + wn);
+  if (m < o.rows)
     store4(o, m, o.c0 + frag % FW * 32 + r * 8 + (lane >> 5) * 4, v);
-  }
 }
 
 // ------------------------------------------------------- K over the waves
@@ -632,10 +642,8 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
     for (int k = 1; k < WAVES; ++k)
       v += sums[(k * FM * FN + f + wave) * 64 + lane];
     const int m = m0 + i * 16 + r;
-    if (m < a.M) {
-      const Out o = out_of(a, n0 + j * 16);
-      store4(o, m, o.c0 + 4 * g, v);
-    }
+    const Out o = out_of(a, m0, n0 + j * 16);
+    if (m < o.rows) store4(o, m, o.c0 + 4 * g, v);
   }
 }
 

@@ -903,3 +903,25 @@ def test_forward_mode_is_refused(grad):
             ops.linear8(x, forward_ad.make_dual(w, torch.ones_like(w)))
         with pytest.raises(RuntimeError, match="forward-mode"):
             ops.rms_norm8(x, forward_ad.make_dual(n, torch.ones_like(n)))
+
+
+# M rows, so that the weights' gradients sum over M; N and K make every tile
+# size, with K split and not, and tiles that reach over two weights
+@pytest.mark.parametrize("M,K,Ns", [
+    (70, 130, (60, 50)), (150, 300, (129, 1, 77)), (600, 1024, (700, 500)),
+    (2048, 1030, (300, 1000)), (4096, 256, (130, 129, 128, 127)),
+    (300, 4000, (2600, 1500)), (6000, 4096, (4100, 200))])
+@pytest.mark.parametrize("wtype", [torch.bfloat16, torch.float32])
+def test_gradients_of_several_weights_are_tensors_of_their_own(M, K, Ns,
+                                                               wtype):
+    x, ws, dys = _linear_inputs(M, K, Ns, wtype)
+    ws = [w.requires_grad_(True) for w in ws]
+    dws = torch.autograd.grad(ops.linear8(x, *ws), ws, dys)
+    _, _, want = oracle.linear(x, [w.detach() for w in ws], dys)
+    for i, (d, (exact, bound)) in enumerate(zip(dws, want)):
+        assert d.shape == ws[i].shape and d.is_contiguous()
+        oracle.assert_within(d, exact, bound, "dw{}".format(i))
+        size = d.untyped_storage().nbytes()
+        assert d.storage_offset() == 0
+        assert size == d.numel() * d.element_size()
+    assert len({d.untyped_storage().data_ptr() for d in dws}) == len(dws)
