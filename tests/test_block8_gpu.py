@@ -925,3 +925,14 @@ def test_gradients_of_several_weights_are_tensors_of_their_own(M, K, Ns,
         assert d.storage_offset() == 0
         assert size == d.numel() * d.element_size()
     assert len({d.untyped_storage().data_ptr() for d in dws}) == len(dws)
+
+
+# M, K and rows of the weights, so that dW takes: 256 x 256, 128 x 256,
+# 128 x 128 and 64 x 64 tiles, each whole and with K split and joined
+@pytest.mark.parametrize("M,K,Ns", [
+    (300, 3001, (60, 2500, 60)), (6000, 3001, (2500, 2500, 1500)),
+    (300, 3001, (300, 700, 129)), (6000, 3001, (129, 1000, 1500)),
+    (300, 130, (1500, 60, 2500)), (12000, 130, (300, 129)),
+    (300, 130, (700, 60, 129)), (6000, 130, (60,))])
+def test_gradients_of_fp32_weights_over_the_kernels(M, K, Ns):
+    _check_linear(*_linear_inputs(M, K, Ns, torch.float32))
