@@ -23,6 +23,12 @@ hipStream_t stream_of(const Tensor& t) {
   return at::cuda::getCurrentCUDAStream(t.get_device()).stream();
 }
 
+// outputs come uninitialised: a launch that was refused must not pass
+void launched(const char* name, hipError_t e) {
+  TORCH_CHECK(e == hipSuccess, name, ": the GPU refused the launch: ",
+              hipGetErrorString(e));
+}
+
 int type_of(const Tensor& t, const char* name) {
   if (t.scalar_type() == torch::kBFloat16) return 0;
   if (t.scalar_type() == torch::kFloat16) return 1;
@@ -91,9 +97,10 @@ Packed packed(const Tensor& codes, const Tensor& scales, const char* name) {
 Packed pack_rows(const Tensor& x) {
   Packed p = new_packed(x.size(0), x.size(1), x);
   if (x.size(0))
-    launch_b8_pack(type_of(x, "x"), vec8(x), x.data_ptr(), ld(x), x.size(0),
-                   (int)x.size(1), p.c(), (int)p.Cp(), p.s(), p.Rp(),
-                   stream_of(x));
+    launched("pack8",
+             launch_b8_pack(type_of(x, "x"), vec8(x), x.data_ptr(), ld(x),
+                            x.size(0), (int)x.size(1), p.c(), (int)p.Cp(),
+                            p.s(), p.Rp(), stream_of(x)));
   return p;
 }
 
@@ -113,9 +120,10 @@ Tensor unpack8(Tensor codes, Tensor scales, int64_t C,
   const int64_t R = p.rows();
   Tensor out = torch::empty({R, C}, codes.options().dtype(dtype));
   if (R)
-    launch_b8_unpack(type_of(out, "out"), C % 8 == 0, p.c(), (int)p.Cp(),
-                     p.s(), p.Rp(), R, (int)C, out.data_ptr(),
-                     stream_of(codes));
+    launched("unpack8",
+             launch_b8_unpack(type_of(out, "out"), C % 8 == 0, p.c(),
+                              (int)p.Cp(), p.s(), p.Rp(), R, (int)C,
+                              out.data_ptr(), stream_of(codes)));
   return out;
 }
 
@@ -188,10 +196,12 @@ std::vector<Tensor> swiglu8_fwd(Tensor g, Tensor u, bool keep) {
     out.push_back(arena.take(g));
   }
   if (R)
-    launch_b8_swiglu_fwd(type_of(g, "g"), vec8(g) && vec8(u), g.data_ptr(),
-                         ld(g), u.data_ptr(), ld(u), R, (int)C,
-                         out[0].data_ptr(), mg.c, mu.c, (int)up(C, 128), mg.s,
-                         mu.s, mg.Rp, stream_of(g));
+    launched("swiglu8",
+             launch_b8_swiglu_fwd(type_of(g, "g"), vec8(g) && vec8(u),
+                                  g.data_ptr(), ld(g), u.data_ptr(), ld(u), R,
+                                  (int)C, out[0].data_ptr(), mg.c, mu.c,
+                                  (int)up(C, 128), mg.s, mu.s, mg.Rp,
+                                  stream_of(g)));
   return out;
 }
 
@@ -208,9 +218,11 @@ std::vector<Tensor> swiglu8_bwd(Tensor dh, const Tensor& kept) {
   const auto o = dh.options().requires_grad(false);
   Tensor dg = torch::empty({R, C}, o), du = torch::empty({R, C}, o);
   if (R)
-    launch_b8_swiglu_bwd(type_of(dh, "dh"), vec8(dh), dh.data_ptr(), ld(dh),
-                         g.c, u.c, (int)g.Cp, g.s, u.s, g.Rp, R, (int)C,
-                         dg.data_ptr(), du.data_ptr(), stream_of(dh));
+    launched("swiglu8",
+             launch_b8_swiglu_bwd(type_of(dh, "dh"), vec8(dh), dh.data_ptr(),
+                                  ld(dh), g.c, u.c, (int)g.Cp, g.s, u.s, g.Rp,
+                                  R, (int)C, dg.data_ptr(), du.data_ptr(),
+                                  stream_of(dh)));
   return {dg, du};
 }
 
@@ -243,11 +255,13 @@ std::vector<Tensor> rms8_fwd(Tensor x, Tensor w, double eps, bool keep) {
     out.push_back(arena.take(x));
   }
   if (R)
-    launch_b8_rms_fwd(type_of(x, "x"),
-                      vec8(x) && (uintptr_t)w.data_ptr() % 16 == 0,
-                      x.data_ptr(), ld(x), w.data_ptr<float>(), R, (int)C,
-                      (float)eps, out[0].data_ptr(), arena.floats, m.c,
-                      (int)up(C, 128), m.s, m.Rp, stream_of(x));
+    launched("rms_norm8",
+             launch_b8_rms_fwd(type_of(x, "x"),
+                               vec8(x) && (uintptr_t)w.data_ptr() % 16 == 0,
+                               x.data_ptr(), ld(x), w.data_ptr<float>(), R,
+                               (int)C, (float)eps, out[0].data_ptr(),
+                               arena.floats, m.c, (int)up(C, 128), m.s, m.Rp,
+                               stream_of(x)));
   return out;
 }
 
@@ -278,14 +292,15 @@ std::vector<c10::optional<Tensor>> rms8_bwd(Tensor dy, const Tensor& kept,
     }
   }
   if (R && (need_dx || need_dw))
-    launch_b8_rms_bwd(type_of(dy, "dy"),
-                      vec8(dy) && (uintptr_t)w.data_ptr() % 16 == 0,
-                      dy.data_ptr(), ld(dy), x.c, (int)x.Cp, x.s, x.Rp,
-                      w.data_ptr<float>(), arena.floats, R, (int)C,
-                      dx ? dx->data_ptr() : nullptr,
-                      need_dw ? partials.data_ptr<float>() : nullptr,
-                      need_dw ? dw->data_ptr<float>() : nullptr,
-                      stream_of(dy));
+    launched("rms_norm8",
+             launch_b8_rms_bwd(type_of(dy, "dy"),
+                               vec8(dy) && (uintptr_t)w.data_ptr() % 16 == 0,
+                               dy.data_ptr(), ld(dy), x.c, (int)x.Cp, x.s,
+                               x.Rp, w.data_ptr<float>(), arena.floats, R,
+                               (int)C, dx ? dx->data_ptr() : nullptr,
+                               need_dw ? partials.data_ptr<float>() : nullptr,
+                               need_dw ? dw->data_ptr<float>() : nullptr,
+                               stream_of(dy)));
   return {dx, dw};
 }
 
@@ -358,7 +373,9 @@ struct Jobs {
     a.C = (int)m.Cp;
   }
   void run(hipStream_t st) {
-    TORCH_CHECK(launch_b8_tiles(&jobs, st), "linear8: matrix is too large");
+    const long long blocks = b8_tile_blocks(&jobs);
+    TORCH_CHECK(blocks >= 0, "linear8: matrix is too large");
+    if (blocks) launched("linear8", launch_b8_tiles(&jobs, blocks, st));
   }
 };
 
@@ -454,8 +471,9 @@ std::vector<Tensor> product(const Mat8& x, const Mat8& w, int64_t M,
       space = torch::empty({bytes}, like.options()
                                         .dtype(torch::kUInt8)
                                         .requires_grad(false));
-    launch_b8_gemm(&a, bytes ? (float*)space.data_ptr() : nullptr,
-                   stream_of(like));
+    launched("linear8",
+             launch_b8_gemm(&a, bytes ? (float*)space.data_ptr() : nullptr,
+                            stream_of(like)));
   }
   return out;
 }
@@ -534,7 +552,9 @@ std::vector<Tensor> linear8_packed(Tensor x, Tensor wcodes, Tensor wscales,
     if (b8_packs_on_the_way(&a)) {
       std::vector<Tensor> out;
       a = gemm_args(mat8(w), M, counts, 0, torch::kBFloat16, x, &out);
-      launch_b8_gemm_bf16(&a, x.data_ptr(), ld(x), (int)K, stream_of(x));
+      launched("linear8",
+               launch_b8_gemm_bf16(&a, x.data_ptr(), ld(x), (int)K,
+                                   stream_of(x)));
       return out;
     }
   }

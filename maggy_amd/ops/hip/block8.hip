@@ -531,17 +531,17 @@ static inline int unit_blocks(long long R, int Q) {
 
 // dtype: 0 bf16, 1 fp16, 2 fp32; vec: kOdd, kVec or kStream
 #define B8_VEC(vec, ...)                                              \
-  do {                                                                \
-    if (vec == kStream) { constexpr int V = kStream; __VA_ARGS__; }   \
-    else if (vec == kVec) { constexpr int V = kVec; __VA_ARGS__; }    \
-    else { constexpr int V = kOdd; __VA_ARGS__; }                     \
-  } while (0)
+  if (vec == kStream) { constexpr int V = kStream; return __VA_ARGS__; } \
+  if (vec == kVec) { constexpr int V = kVec; return __VA_ARGS__; }    \
+  constexpr int V = kOdd;                                             \
+  return __VA_ARGS__
 #define B8_TYPED(dtype, vec, ...)                                     \
-  do {                                                                \
+  [&]() -> hipError_t {                                               \
     if (dtype == 0) { using T = Bf16; B8_VEC(vec, __VA_ARGS__); }     \
-    else if (dtype == 1) { using T = Fp16; B8_VEC(vec, __VA_ARGS__); } \
-    else { using T = Fp32; B8_VEC(vec, __VA_ARGS__); }                \
-  } while (0)
+    if (dtype == 1) { using T = Fp16; B8_VEC(vec, __VA_ARGS__); }     \
+    using T = Fp32;                                                   \
+    B8_VEC(vec, __VA_ARGS__);                                         \
+  }()
 
 // for results of n values
 static inline int stores_of(int vec, int dtype, long long n) {
@@ -550,52 +550,50 @@ static inline int stores_of(int vec, int dtype, long long n) {
 }
 
 template <class T, int V, int WPR, int NI>
-static void rms_fwd_run(int blocks, hipStream_t st, const void* x,
+static hipError_t rms_fwd_run(int blocks, hipStream_t st, const void* x,
                         long long ldx, const float* w, long long R, int C,
                         float eps, void* y, float* inv, uint8_t* codes,
                         int Cp, uint32_t* scales, long long Rp) {
-  launch(rms_fwd<T, V, WPR, NI>, blocks, kThreads, st,
+  return launch(rms_fwd<T, V, WPR, NI>, blocks, kThreads, 0, st,
       (const typename T::raw*)x, ldx, w, R, C, eps, (typename T::raw*)y, inv,
       codes, Cp, scales, Rp);
 }
 
 template <class T, int V, int WPR, int NI>
-static void rms_bwd_run(int blocks, hipStream_t st, const void* dy,
+static hipError_t rms_bwd_run(int blocks, hipStream_t st, const void* dy,
                         long long ldy, const uint8_t* codes, int Cp,
                         const uint32_t* scales, long long Rp, const float* w,
                         const float* inv, long long R, int C, void* dx,
                         float* partials) {
-  launch(rms_bwd<T, V, WPR, NI>, blocks, kThreads, st,
+  return launch(rms_bwd<T, V, WPR, NI>, blocks, kThreads, 0, st,
       (const typename T::raw*)dy, ldy, codes, Cp, scales, Rp, w, inv, R, C,
       (typename T::raw*)dx, partials);
 }
 
 // rows of up to 16384 columns: the caller refuses longer ones
 #define B8_ROWS(RUN, C, ...)                                   \
-  do {                                                         \
-    if (C <= 512) RUN<T, V, 1, 1>(__VA_ARGS__);                \
-    else if (C <= 1024) RUN<T, V, 1, 2>(__VA_ARGS__);          \
-    else if (C <= 2048) RUN<T, V, 1, 4>(__VA_ARGS__);          \
-    else if (C <= 4096) RUN<T, V, 4, 2>(__VA_ARGS__);          \
-    else if (C <= 8192) RUN<T, V, 4, 4>(__VA_ARGS__);          \
-    else RUN<T, V, 4, 8>(__VA_ARGS__);                         \
-  } while (0)
+  (C <= 512    ? RUN<T, V, 1, 1>(__VA_ARGS__)                  \
+   : C <= 1024 ? RUN<T, V, 1, 2>(__VA_ARGS__)                  \
+   : C <= 2048 ? RUN<T, V, 1, 4>(__VA_ARGS__)                  \
+   : C <= 4096 ? RUN<T, V, 4, 2>(__VA_ARGS__)                  \
+   : C <= 8192 ? RUN<T, V, 4, 4>(__VA_ARGS__)                  \
+               : RUN<T, V, 4, 8>(__VA_ARGS__))
 
 }  // namespace b8
 
 using namespace b8;
 
-extern "C" void launch_b8_pack(int dtype, int vec, const void* x,
+extern "C" hipError_t launch_b8_pack(int dtype, int vec, const void* x,
                                long long ldx, long long R, int C,
                                uint8_t* codes, int Cp, uint32_t* scales,
                                long long Rp, hipStream_t st) {
   const int Q = (Cp + 511) / 512;
-  B8_TYPED(dtype, vec,
+  return B8_TYPED(dtype, vec,
            (launch(pack_rows<T, V ? kVec : kOdd>, unit_blocks(R, Q), kThreads,
-               st, (const T::raw*)x, ldx, R, C, codes, Cp, scales, Rp, Q)));
+               0, st, (const T::raw*)x, ldx, R, C, codes, Cp, scales, Rp, Q)));
 }
 
-extern "C" void launch_b8_unpack(int dtype, int vec, const uint8_t* codes,
+extern "C" hipError_t launch_b8_unpack(int dtype, int vec, const uint8_t* codes,
                                  int Cp, const uint32_t* scales,
                                  long long Rp, long long R, int C, void* out,
                                  hipStream_t st) {
@@ -603,12 +601,12 @@ extern "C" void launch_b8_unpack(int dtype, int vec, const uint8_t* codes,
   const float most =
       dtype == 0 ? 0x1.fep127f : dtype == 1 ? 65504.f : 0x1.fffffep127f;
   vec = stores_of(vec, dtype, R * C);
-  B8_TYPED(dtype, vec,
-           (launch(unpack_rows<T, V>, unit_blocks(R, Q), kThreads, st,
+  return B8_TYPED(dtype, vec,
+           (launch(unpack_rows<T, V>, unit_blocks(R, Q), kThreads, 0, st,
                codes, Cp, scales, Rp, Q, R, C, (T::raw*)out, most)));
 }
 
-extern "C" bool launch_b8_tiles(TileJobs* jobs, hipStream_t st) {
+extern "C" long long b8_tile_blocks(TileJobs* jobs) {
   long long blocks = 0;
   for (int j = 0; j < jobs->count; ++j) {
     TileJob& a = jobs->job[j];
@@ -617,13 +615,16 @@ extern "C" bool launch_b8_tiles(TileJobs* jobs, hipStream_t st) {
       a.vec = kStream;
     blocks += (a.R + 127ll) / 128 * ((a.C + 127ll) / 128);
     // a launch has fewer than 2^32 threads
-    if (blocks >= 1ll << 23) return false;
+    if (blocks >= 1ll << 23) return -1;
   }
-  if (blocks) launch(pack_tiles, blocks, 512, st, *jobs);
-  return true;
+  return blocks;
+}
+extern "C" hipError_t launch_b8_tiles(const TileJobs* jobs, long long blocks,
+                                      hipStream_t st) {
+  return launch(pack_tiles, blocks, 512, 0, st, *jobs);
 }
 
-extern "C" void launch_b8_swiglu_fwd(int dtype, int vec, const void* g,
+extern "C" hipError_t launch_b8_swiglu_fwd(int dtype, int vec, const void* g,
                                      long long ldg, const void* u,
                                      long long ldu, long long R, int C,
                                      void* h, uint8_t* gc, uint8_t* uc,
@@ -631,13 +632,13 @@ extern "C" void launch_b8_swiglu_fwd(int dtype, int vec, const void* g,
                                      long long Rp, hipStream_t st) {
   vec = stores_of(vec, dtype, R * C);
   const int Q = (Cp + 511) / 512;
-  B8_TYPED(dtype, vec,
-           (launch(swiglu_fwd<T, V>, unit_blocks(R, Q), kThreads, st,
+  return B8_TYPED(dtype, vec,
+           (launch(swiglu_fwd<T, V>, unit_blocks(R, Q), kThreads, 0, st,
                (const T::raw*)g, ldg, (const T::raw*)u, ldu, R, C,
                (T::raw*)h, gc, uc, Cp, gs, us, Rp, Q)));
 }
 
-extern "C" void launch_b8_swiglu_bwd(int dtype, int vec, const void* dh,
+extern "C" hipError_t launch_b8_swiglu_bwd(int dtype, int vec, const void* dh,
                                      long long ldh, const uint8_t* gc,
                                      const uint8_t* uc, int Cp,
                                      const uint32_t* gs, const uint32_t* us,
@@ -645,13 +646,13 @@ extern "C" void launch_b8_swiglu_bwd(int dtype, int vec, const void* dh,
                                      void* dg, void* du, hipStream_t st) {
   vec = stores_of(vec, dtype, 2 * R * C);
   const int Q = (Cp + 511) / 512;
-  B8_TYPED(dtype, vec,
-           (launch(swiglu_bwd<T, V>, unit_blocks(R, Q), kThreads, st,
+  return B8_TYPED(dtype, vec,
+           (launch(swiglu_bwd<T, V>, unit_blocks(R, Q), kThreads, 0, st,
                (const T::raw*)dh, ldh, gc, uc, Cp, gs, us, Rp, Q, R, C,
                (T::raw*)dg, (T::raw*)du)));
 }
 
-extern "C" void launch_b8_rms_fwd(int dtype, int vec, const void* x,
+extern "C" hipError_t launch_b8_rms_fwd(int dtype, int vec, const void* x,
                                   long long ldx, const float* w, long long R,
                                   int C, float eps, void* y, float* inv,
                                   uint8_t* codes, int Cp, uint32_t* scales,
@@ -659,7 +660,7 @@ extern "C" void launch_b8_rms_fwd(int dtype, int vec, const void* x,
   vec = stores_of(vec, dtype, R * C);
   const long long groups = C <= 2048 ? (R + 3) / 4 : R;
   const int blocks = (int)(groups < 8192 ? groups : 8192);
-  B8_TYPED(dtype, vec,
+  return B8_TYPED(dtype, vec,
            B8_ROWS(rms_fwd_run, C, blocks, st, x, ldx, w, R, C, eps, y, inv,
                    codes, Cp, scales, Rp));
 }
@@ -676,7 +677,7 @@ extern "C" int b8_rms_bwd_partials(long long R, int C) {
   return b8_rms_bwd_blocks(R, C) * (C <= 2048 ? 4 : 1);
 }
 
-extern "C" void launch_b8_rms_bwd(int dtype, int vec, const void* dy,
+extern "C" hipError_t launch_b8_rms_bwd(int dtype, int vec, const void* dy,
                                   long long ldy, const uint8_t* codes,
                                   int Cp, const uint32_t* scales,
                                   long long Rp, const float* w,
@@ -685,10 +686,10 @@ extern "C" void launch_b8_rms_bwd(int dtype, int vec, const void* dy,
                                   hipStream_t st) {
   vec = stores_of(vec, dtype, R * C);
   const int blocks = b8_rms_bwd_blocks(R, C);
-  B8_TYPED(dtype, vec,
+  const hipError_t e = B8_TYPED(dtype, vec,
            B8_ROWS(rms_bwd_run, C, blocks, st, dy, ldy, codes, Cp, scales,
                    Rp, w, inv, R, C, dx, partials));
-  if (partials)
-    launch(fold_rows, (C + 63) / 64, 1024, st,
-        partials, b8_rms_bwd_partials(R, C), C, dw);
+  if (e != hipSuccess || !partials) return e;
+  return launch(fold_rows, (C + 63) / 64, 1024, 0, st, partials,
+                b8_rms_bwd_partials(R, C), C, dw);
 }

@@ -3,6 +3,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <cstdint>
+#include <tuple>
 
 namespace b8 {
 
@@ -78,42 +79,55 @@ struct GemmArgs {
 };
 
 #ifdef __HIPCC__
-// arguments are converted to what the kernel takes
+// Arguments are converted to what the kernel takes.  The status is this
+// launch's own, not one that an earlier call left.
 template <class... P, class... A>
-static inline void launch(void (*kernel)(P...), long long blocks, int threads,
-                          hipStream_t st, A... args) {
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st,
-                     static_cast<P>(args)...);
+static inline hipError_t launch(void (*kernel)(P...), long long blocks,
+                                int threads, int lds, hipStream_t st,
+                                A... args) {
+  std::tuple<P...> values(static_cast<P>(args)...);
+  const hipError_t e = std::apply(
+      [&](P&... v) {
+        void* at[] = {(void*)&v...};
+        return hipLaunchKernel((const void*)kernel, dim3((unsigned)blocks),
+                               dim3(threads), at, lds, st);
+      },
+      values);
+  if (e != hipSuccess) (void)hipGetLastError();  // it is reported here
+  return e;
 }
 #endif
 
 }  // namespace b8
 
+// every launch returns its status
 extern "C" {
-void launch_b8_pack(int dtype, int vec, const void* x, long long ldx,
+hipError_t launch_b8_pack(int dtype, int vec, const void* x, long long ldx,
                     long long R, int C, uint8_t* codes, int Cp,
                     uint32_t* scales, long long Rp, hipStream_t st);
-void launch_b8_unpack(int dtype, int vec, const uint8_t* codes, int Cp,
+hipError_t launch_b8_unpack(int dtype, int vec, const uint8_t* codes, int Cp,
                       const uint32_t* scales, long long Rp, long long R,
                       int C, void* out, hipStream_t st);
-// sets the jobs' first blocks; false if there are too many tiles
-bool launch_b8_tiles(b8::TileJobs* jobs, hipStream_t st);
-void launch_b8_swiglu_fwd(int dtype, int vec, const void* g, long long ldg,
+// sets the jobs' first blocks; returns how many there are, -1 if too many
+long long b8_tile_blocks(b8::TileJobs* jobs);
+hipError_t launch_b8_tiles(const b8::TileJobs* jobs, long long blocks,
+                           hipStream_t st);
+hipError_t launch_b8_swiglu_fwd(int dtype, int vec, const void* g, long long ldg,
                           const void* u, long long ldu, long long R, int C,
                           void* h, uint8_t* gc, uint8_t* uc, int Cp,
                           uint32_t* gs, uint32_t* us, long long Rp,
                           hipStream_t st);
-void launch_b8_swiglu_bwd(int dtype, int vec, const void* dh, long long ldh,
+hipError_t launch_b8_swiglu_bwd(int dtype, int vec, const void* dh, long long ldh,
                           const uint8_t* gc, const uint8_t* uc, int Cp,
                           const uint32_t* gs, const uint32_t* us,
                           long long Rp, long long R, int C, void* dg,
                           void* du, hipStream_t st);
-void launch_b8_rms_fwd(int dtype, int vec, const void* x, long long ldx,
+hipError_t launch_b8_rms_fwd(int dtype, int vec, const void* x, long long ldx,
                        const float* w, long long R, int C, float eps, void* y,
                        float* inv, uint8_t* codes, int Cp, uint32_t* scales,
                        long long Rp, hipStream_t st);
 int b8_rms_bwd_partials(long long R, int C);
-void launch_b8_rms_bwd(int dtype, int vec, const void* dy, long long ldy,
+hipError_t launch_b8_rms_bwd(int dtype, int vec, const void* dy, long long ldy,
                        const uint8_t* codes, int Cp, const uint32_t* scales,
                        long long Rp, const float* w, const float* inv,
                        long long R, int C, void* dx, float* partials,
@@ -121,10 +135,10 @@ void launch_b8_rms_bwd(int dtype, int vec, const void* dy, long long ldy,
 // bytes of workspace that the product wants (-1: too large a product for a
 // launch), and the product
 long long b8_gemm_workspace(const b8::GemmArgs* args);
-void launch_b8_gemm(const b8::GemmArgs* args, float* workspace,
+hipError_t launch_b8_gemm(const b8::GemmArgs* args, float* workspace,
                     hipStream_t st);
 // the same with x in bf16, packed on the way, if that is the better choice
 bool b8_packs_on_the_way(const b8::GemmArgs* args);
-void launch_b8_gemm_bf16(const b8::GemmArgs* args, const void* x,
+hipError_t launch_b8_gemm_bf16(const b8::GemmArgs* args, const void* x,
                          long long ldx, int K, hipStream_t st);
 }

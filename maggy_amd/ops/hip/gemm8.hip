@@ -648,13 +648,12 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
 }
 
 template <int FM, int FN, int U, int WAVES, bool FUSED>
-static void split_run(SplitArgs sa, hipStream_t st) {
+static hipError_t split_run(SplitArgs sa, hipStream_t st) {
   constexpr int kLds = WAVES * FM * FN * 64 * 16;
   const auto kernel = gemm_split<FM, FN, U, WAVES, FUSED>;
   sa.tiles_n = (sa.g.N + 16 * FN - 1) / (16 * FN);
   const long long tiles_m = (sa.g.M + 16 * FM - 1) / (16 * FM);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * sa.tiles_n)),
-                     dim3(WAVES * 64), kLds, st, sa);
+  return launch(kernel, tiles_m * sa.tiles_n, WAVES * 64, kLds, st, sa);
 }
 
 // --------------------------------------------------------------- the choice
@@ -741,12 +740,15 @@ static Plan plan_of(const GemmArgs& a) {
 }
 
 template <int FX, int FW, int NBUF>
-static void tile_run(const GemmArgs& a, const Plan& p, hipStream_t st) {
-  launch(gemm_tile<FX, FW, NBUF>, p.work.items, 256, st, a, p.work);
+static hipError_t tile_run(const GemmArgs& a, const Plan& p,
+                           hipStream_t st) {
+  const hipError_t e =
+      launch(gemm_tile<FX, FW, NBUF>, p.work.items, 256, 0, st, a, p.work);
   const long long rest =
       (long long)p.work.tiles_m * p.work.tiles_n - p.work.full;
-  if (rest)
-    launch(join_splits<FX, FW>, rest * 4 * FX * FW, 256, st, a, p.work);
+  if (e != hipSuccess || !rest) return e;
+  return launch(join_splits<FX, FW>, rest * 4 * FX * FW, 256, 0, st, a,
+                p.work);
 }
 
 }  // namespace b8
@@ -758,21 +760,20 @@ extern "C" long long b8_gemm_workspace(const GemmArgs* args) {
   return p.kind < 0 ? -1 : p.workspace;
 }
 
-extern "C" void launch_b8_gemm(const GemmArgs* args, float* workspace,
-                               hipStream_t st) {
+extern "C" hipError_t launch_b8_gemm(const GemmArgs* args, float* workspace,
+                                     hipStream_t st) {
   const GemmArgs a = *args;
   Plan p = plan_of(a);
   p.work.partials = workspace;
   if (p.kind == 0)
-    tile_run<4, 4, 2>(a, p, st);
-  else if (p.kind == 1)
-    tile_run<2, 4, 3>(a, p, st);
-  else if (p.kind == 2)
-    tile_run<2, 2, 4>(a, p, st);
-  else if (p.kind == 3)
-    tile_run<1, 1, 8>(a, p, st);
-  else
-    split_run<2, 1, 1, 16, false>(SplitArgs{a}, st);
+    return tile_run<4, 4, 2>(a, p, st);
+  if (p.kind == 1)
+    return tile_run<2, 4, 3>(a, p, st);
+  if (p.kind == 2)
+    return tile_run<2, 2, 4>(a, p, st);
+  if (p.kind == 3)
+    return tile_run<1, 1, 8>(a, p, st);
+  return split_run<2, 1, 1, 16, false>(SplitArgs{a}, st);
 }
 
 // Whether x in bf16 is packed on the way: up to 16 rows always, up to 32 where
@@ -791,17 +792,14 @@ extern "C" bool b8_packs_on_the_way(const GemmArgs* args) {
 // the packing of x, fewer are more workgroups.  Measured with 1, 2 and 4:
 // 1x2048x2048 4.4, 5.1 and 7.2 us; 16x8192x2048 11.7, 8.7 and 10.3;
 // 8x14336x4096 31, 23.7 and 22.2; 24x8192x2048 12.7, 9.0 and 17.5.
-extern "C" void launch_b8_gemm_bf16(const GemmArgs* args, const void* x,
-                                    long long ldx, int K, hipStream_t st) {
+extern "C" hipError_t launch_b8_gemm_bf16(const GemmArgs* args, const void* x,
+                                          long long ldx, int K,
+                                          hipStream_t st) {
   const SplitArgs sa{*args, (const uint16_t*)x, ldx, K};
-  if (args->M > 16 && args->N <= 4096)
-    split_run<2, 1, 1, 16, true>(sa, st);
-  else if (args->M > 16)
-    split_run<2, 2, 1, 16, true>(sa, st);
-  else if (args->N <= 6144)
-    split_run<1, 1, 1, 16, true>(sa, st);
-  else if (args->N <= 12288)
-    split_run<1, 2, 1, 16, true>(sa, st);
-  else
-    split_run<1, 4, 1, 16, true>(sa, st);
+  if (args->M > 16)
+    return args->N <= 4096 ? split_run<2, 1, 1, 16, true>(sa, st)
+                           : split_run<2, 2, 1, 16, true>(sa, st);
+  if (args->N <= 6144) return split_run<1, 1, 1, 16, true>(sa, st);
+  if (args->N <= 12288) return split_run<1, 2, 1, 16, true>(sa, st);
+  return split_run<1, 4, 1, 16, true>(sa, st);
 }

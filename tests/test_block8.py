@@ -729,3 +729,42 @@ def test_forward_mode_is_refused(grad):
             ops.linear8(x, forward_ad.make_dual(w, torch.ones_like(w)))
         with pytest.raises((RuntimeError, NotImplementedError)):
             ops.rms_norm8(x, forward_ad.make_dual(n, torch.ones_like(n)))
+
+
+# ------------------------------------------------------------------ launches
+def _launchers():
+    """The extension's launch functions, and a call of each on rows of one
+    value and no memory."""
+    import ctypes
+
+    if not ops.has_ext():
+        pytest.skip("the extension is not built")
+    lib = ctypes.CDLL(ops.require_ext().__file__)
+    i, n, p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
+    # r stands for the number of rows
+    r = type("Rows", (n,), {})
+    calls = {
+        "launch_b8_pack": (i, i, p, n, r, i, p, i, p, n, p),
+        "launch_b8_unpack": (i, i, p, i, p, n, r, i, p, p),
+        "launch_b8_swiglu_fwd": (i, i, p, n, p, n, r, i, p, p, p, i, p, p, n,
+                                 p),
+        "launch_b8_swiglu_bwd": (i, i, p, n, p, p, i, p, p, n, r, i, p, p, p),
+        "launch_b8_rms_fwd": (i, i, p, n, p, r, i, ctypes.c_float, p, p, p, i,
+                              p, n, p),
+        "launch_b8_rms_bwd": (i, i, p, n, p, i, p, n, p, p, r, i, p, p, p, p)}
+
+    def call(name, rows):
+        f, types = getattr(lib, name), calls[name]
+        f.restype = i
+        f.argtypes = [n if t is r else t for t in types]
+        return f(*(None if t is p else rows if t is r else 1 for t in types))
+
+    return lib, list(calls), call
+
+
+@pytest.mark.skipif(torch.cuda.is_available(),
+                    reason="without a GPU every launch is refused")
+def test_a_refused_launch_is_reported():
+    _, names, call = _launchers()
+    for name in names:
+        assert call(name, 1) != 0, name

@@ -936,3 +936,16 @@ def test_gradients_of_several_weights_are_tensors_of_their_own(M, K, Ns,
     (300, 130, (700, 60, 129)), (6000, 130, (60,))])
 def test_gradients_of_fp32_weights_over_the_kernels(M, K, Ns):
     _check_linear(*_linear_inputs(M, K, Ns, torch.float32))
+
+
+def test_a_refused_launch_is_reported_and_not_left_behind():
+    """A grid of no workgroups, which the runtime refuses."""
+    from tests.test_block8 import _launchers
+
+    lib, names, call = _launchers()
+    torch.cuda.synchronize()
+    lib.hipGetLastError()
+    for name in names:
+        assert call(name, 0) != 0, name
+        assert lib.hipGetLastError() == 0, name
+    torch.cuda.synchronize()
