@@ -670,7 +670,9 @@ void no_second_derivative(const char* name) {
 
 // A leaf whose eager graph lives accumulates on that graph's stream.  If that
 // is the default stream, capturing this pass would end in the runtime: no
-// capture can wait for it.
+// capture can wait for it.  Between the leaf and this node there may be views
+// and conversions, a call's own (leading axes, a norm's weight in bf16) among
+// them: whatever has one input.
 void no_eager_leaves(const char* name) {
   if (at::cuda::currentStreamCaptureStatusMayInitCtx() ==
       c10::cuda::CaptureStatus::None)
@@ -678,9 +680,11 @@ void no_eager_leaves(const char* name) {
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
   for (const auto& edge : node->next_edges()) {
-    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()))
-      continue;
-    const auto stream = edge.function->stream();
+    torch::autograd::Node* at = edge.function.get();
+    while (at && at->next_edges().size() == 1)
+      at = at->next_edge(0).function.get();
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(at)) continue;
+    const auto stream = at->stream();
     TORCH_CHECK(!stream || stream->id() != 0, name,
                 ": a backward pass cannot be captured while an eager graph "
                 "of the same leaf, made on the default stream, lives");

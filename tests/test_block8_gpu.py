@@ -949,3 +949,30 @@ def test_a_refused_launch_is_reported_and_not_left_behind():
         assert call(name, 0) != 0, name
         assert lib.hipGetLastError() == 0, name
     torch.cuda.synchronize()
+
+
+def test_capture_beside_an_eager_graph_is_refused_behind_views():
+    """Leaves that a call reshapes or converts before its kernels."""
+    x = _normal((2, 4, 256), 1).requires_grad_(True)
+    w = _normal((64, 256), 2, 0.1)
+    n = torch.ones(256, device="cuda", dtype=torch.bfloat16,
+                   requires_grad=True)
+    far = _normal((4, 2, 256), 3).requires_grad_(True)
+    wide = _normal((8, 256), 4, dtype=torch.float32).requires_grad_(True)
+    for call, leaf, shape in (
+            (lambda: ops.linear8(x, w), x, (2, 4, 64)),
+            (lambda: ops.rms_norm8(x.detach(), n), n, (2, 4, 256)),
+            (lambda: ops.swiglu8(x, x.detach()), x, (2, 4, 256)),
+            (lambda: ops.linear8(far.transpose(0, 1)[..., :], w), far,
+             (2, 4, 64)),
+            (lambda: ops.linear8(wide.bfloat16(), w), wide, (8, 64))):
+        dy = _normal(shape, 5)
+        eager = call()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            y = call()
+            with pytest.raises(RuntimeError, match="eager graph"):
+                y.backward(dy)
+        eager.backward(dy)  # not hurt by it
+        torch.cuda.synchronize()
+        assert leaf.grad.isfinite().all()
