@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256) void join_splits(GemmArgs a,
 // ------------------------------------------------------- K over the waves
 // Small products, few rows among them: what counts is how soon all of w and
 // x is under way.  A workgroup takes 16 FM rows of x by 16 FN rows of w; its
-// waves share K, U steps at a time, and load their operands straight from
+// waves share K, a step at a time, and load their operands straight from
 // global memory: within a workgroup nothing is read twice, so LDS would save
 // nothing, and there is no barrier before the sums meet in LDS, added in the
 // order of the waves.  With FUSED, for up to 32 rows of bf16, x is packed on
@@ -527,7 +527,7 @@ __device__ __forceinline__ i32x8 pack_step(const u32x4 (&v)[4], int* scale) {
   return code;
 }
 
-template <int FM, int FN, int U, int WAVES, bool FUSED>
+template <int FM, int FN, int WAVES, bool FUSED>
 __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
   const GemmArgs& a = sa.g;
   extern __shared__ f32x4 sums[];  // [WAVES][FM * FN][64]
@@ -559,74 +559,54 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
   f32x4 acc[FM * FN];
 #pragma unroll
   for (int i = 0; i < FM * FN; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  static_assert(4 % U == 0);  // so that U steps have one scale dword a row
-  for (int k0 = wave * U; k0 < a.KT; k0 += WAVES * U) {
-    i32x4 wv[U][FN][2], xv[U][FUSED ? 1 : FM][2];
-    u32x4 raw[FUSED ? U : 1][FM][4];
+  for (int kt = wave; kt < a.KT; kt += WAVES) {
+    i32x4 wv[FN][2], xv[FM][2];
+    u32x4 raw[FM][4];
     uint32_t wq[FN], xq[FM];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      wq[j] = ws[j][(k0 >> 2) * a.wsp];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const i32x4* p =
-            (const i32x4*)(w[j] + min(k0 + u, a.KT - 1) * a.wn * 128);
-        wv[u][j][0] = p[0];
-        wv[u][j][1] = p[1];
-      }
+      wq[j] = ws[j][(kt >> 2) * a.wsp];
+      const i32x4* p = (const i32x4*)(w[j] + kt * a.wn * 128);
+      wv[j][0] = p[0];
+      wv[j][1] = p[1];
     }
     if constexpr (FUSED) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int k = (k0 + u) * 128 + g * 32 + c * 8, m = i * 16 + r;
-            raw[u][i][c] = m < a.M && k < sa.K
-                               ? *(const u32x4*)(sa.x + m * sa.ldx + k)
-                               : u32x4{0, 0, 0, 0};
-          }
+        for (int c = 0; c < 4; ++c) {
+          const int k = kt * 128 + g * 32 + c * 8, m = i * 16 + r;
+          raw[i][c] = m < a.M && k < sa.K
+                          ? *(const u32x4*)(sa.x + m * sa.ldx + k)
+                          : u32x4{0, 0, 0, 0};
+        }
     } else {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        xq[i] = xs[i][(k0 >> 2) * a.xsp];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const i32x4* p =
-              (const i32x4*)(x[i] + min(k0 + u, a.KT - 1) * a.xn * 128);
-          xv[u][i][0] = p[0];
-          xv[u][i][1] = p[1];
-        }
+        xq[i] = xs[i][(kt >> 2) * a.xsp];
+        const i32x4* p = (const i32x4*)(x[i] + kt * a.xn * 128);
+        xv[i][0] = p[0];
+        xv[i][1] = p[1];
       }
     }
+    const int shift = 8 * (kt & 3);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // past the end w repeats its last block, against zeros; scales there
-      // may never have been written
-      const bool inside = k0 + u < a.KT;
-      const int shift = 8 * ((k0 + u) & 3);
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        int sx;
-        i32x8 xf;
-        if constexpr (FUSED) {
-          xf = pack_step(raw[u][i], &sx);
-        } else {
-          const i32x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-          xf = inside ? __builtin_shufflevector(xv[u][i][0], xv[u][i][1], 0,
-                                                1, 2, 3, 4, 5, 6, 7)
-                      : zero;
-          sx = inside ? (int)(xq[i] >> shift) : 1;
-        }
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i * FN + j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              __builtin_shufflevector(wv[u][j][0], wv[u][j][1], 0, 1, 2, 3, 4,
-                                      5, 6, 7),
-              xf, acc[i * FN + j], 0, 0, 0,
-              inside ? (int)(wq[j] >> shift) : 1, 0, sx);
+    for (int i = 0; i < FM; ++i) {
+      int sx;
+      i32x8 xf;
+      if constexpr (FUSED) {
+        xf = pack_step(raw[i], &sx);
+      } else {
+        xf = __builtin_shufflevector(xv[i][0], xv[i][1], 0, 1, 2, 3, 4, 5, 6,
+                                     7);
+        sx = (int)(xq[i] >> shift);
       }
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i * FN + j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            __builtin_shufflevector(wv[j][0], wv[j][1], 0, 1, 2, 3, 4, 5, 6,
+                                    7),
+            xf, acc[i * FN + j], 0, 0, 0, (int)(wq[j] >> shift), 0, sx);
     }
   }
 #pragma unroll
@@ -647,10 +627,10 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_split(SplitArgs sa) {
   }
 }
 
-template <int FM, int FN, int U, int WAVES, bool FUSED>
+template <int FM, int FN, int WAVES, bool FUSED>
 static hipError_t split_run(SplitArgs sa, hipStream_t st) {
   constexpr int kLds = WAVES * FM * FN * 64 * 16;
-  const auto kernel = gemm_split<FM, FN, U, WAVES, FUSED>;
+  const auto kernel = gemm_split<FM, FN, WAVES, FUSED>;
   sa.tiles_n = (sa.g.N + 16 * FN - 1) / (16 * FN);
   const long long tiles_m = (sa.g.M + 16 * FM - 1) / (16 * FM);
   return launch(kernel, tiles_m * sa.tiles_n, WAVES * 64, kLds, st, sa);
@@ -773,7 +753,7 @@ extern "C" hipError_t launch_b8_gemm(const GemmArgs* args, float* workspace,
     return tile_run<2, 2, 4>(a, p, st);
   if (p.kind == 3)
     return tile_run<1, 1, 8>(a, p, st);
-  return split_run<2, 1, 1, 16, false>(SplitArgs{a}, st);
+  return split_run<2, 1, 16, false>(SplitArgs{a}, st);
 }
 
 // Whether x in bf16 is packed on the way: up to 16 rows always, up to 32 where
@@ -797,9 +777,9 @@ extern "C" hipError_t launch_b8_gemm_bf16(const GemmArgs* args, const void* x,
                                           hipStream_t st) {
   const SplitArgs sa{*args, (const uint16_t*)x, ldx, K};
   if (args->M > 16)
-    return args->N <= 4096 ? split_run<2, 1, 1, 16, true>(sa, st)
-                           : split_run<2, 2, 1, 16, true>(sa, st);
-  if (args->N <= 6144) return split_run<1, 1, 1, 16, true>(sa, st);
-  if (args->N <= 12288) return split_run<1, 2, 1, 16, true>(sa, st);
-  return split_run<1, 4, 1, 16, true>(sa, st);
+    return args->N <= 4096 ? split_run<2, 1, 16, true>(sa, st)
+                           : split_run<2, 2, 16, true>(sa, st);
+  if (args->N <= 6144) return split_run<1, 1, 16, true>(sa, st);
+  if (args->N <= 12288) return split_run<1, 2, 16, true>(sa, st);
+  return split_run<1, 4, 16, true>(sa, st);
 }
