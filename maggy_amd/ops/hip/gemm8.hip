@@ -367,6 +367,8 @@ __global__ __launch_bounds__(256, 1) void gemm_tile(GemmArgs a,
     return;
   }
   const Out o = out_of(a, m0 + wm, n0 + wn);
+  // straight from the accumulators: dW of 14336 x 4096, K 24576, takes 27 us
+  // more than in bf16, and 117 MB more to write are 24
   if (o.f32) {
 #pragma unroll
     for (int i = 0; i < FX; ++i) {
@@ -474,8 +476,10 @@ __global__ __launch_bounds__(256) void join_splits(GemmArgs a,
 // order of the waves.  With FUSED, for up to 32 rows of bf16, x is packed on
 // the way: each lane needs 32 neighbouring values a step, which four lanes
 // share a scale for, so the codes are those of pack_rows and a launch is
-// saved.  Bound by the read of w: 8 x 14336, K 4096 takes 13 us (4.5
-// TB/s of 59 MB); 1 x 2048, K 2048 4.5, all of it latency.
+// saved.  Bound by the read of w: a call of 8 x 14336, K 4096 takes 13.5 us
+// (4.4 TB/s of 59 MB) on one weight, which the last cache holds, and 15.1
+// (3.9 TB/s) on weights in turn that come from memory, as a decoded token's
+// do; 1 x 2048, K 2048 3.8 and 4.7, all of it latency.
 struct SplitArgs {
   GemmArgs g;
   const uint16_t* x;  // FUSED: bf16, rows of ldx elements, K columns
@@ -653,7 +657,9 @@ static hipError_t split_run(SplitArgs sa, hipStream_t st) {
 // Joining the splits costs a launch, about 2.5 us, and their traffic at about
 // 5 TB/s.  gemm_split takes 0.6 + 0.16 steps us for each 256 workgroups.
 // Over 220 products of up to 24576 x 14336 the choice is within 1 % of the
-// best on average.  Measured either way (M x N, K), in us:
+// best on average.  All of it was measured on operands that the caches hold
+// as far as they fit, the model's figures too.  Measured either way (M x N,
+// K), in us:
 //   24576 x 4096, 14336: 1014 by 256 x 256 and 1500 by 128 x 128
 //   4096 x 2048, 16384: 135 by 256 x 256, 117 with K split in two, 116 by
 //     128 x 256, 133 by 128 x 128
@@ -757,10 +763,13 @@ extern "C" hipError_t launch_b8_gemm(const GemmArgs* args, float* workspace,
 }
 
 // Whether x in bf16 is packed on the way: up to 16 rows always, up to 32 where
-// few workgroups repeat the packing.  Measured with a launch for packing and
-// without, 24 rows (N x K): 2048 x 2048 8.0 and 7.1 us, 8192 x 2048 11.0 and
-// 9.0, 8192 x 512 6.9 and 4.9; but 4096 x 4096 11.1 and 11.9, 14336 x 4096
-// 16.9 and 27.9.
+// few workgroups repeat the packing.  A call with a launch for packing and
+// without, in us, on weights in turn that come from memory: 24 rows (N x K)
+// 2048 x 2048 8.0 and 7.6, 8192 x 2048 10.6 and 9.3, 8192 x 512 6.8 and 5.2;
+// but 4096 x 4096 10.6 and 12.0, 14336 x 4096 17.1 and 27.6.  8 rows
+// 4096 x 4096 9.5 and 8.4, 8192 x 4096 15.7 and 10.3, 14336 x 4096 16.6 and
+// 15.2; where K is long 16 rows lose: 4096 x 4096 9.9 and 9.8, 4096 x 14336
+// 21.1 and 26.7.
 extern "C" bool b8_packs_on_the_way(const GemmArgs* args) {
   // a launch has fewer than 2^32 threads, 16 a row of w
   return args->M <= 16 ? args->N < 1 << 28
@@ -769,9 +778,18 @@ extern "C" bool b8_packs_on_the_way(const GemmArgs* args) {
 
 // x in rows of K columns, K and ldx multiples of 8; the codes of x in args
 // are not read.  A workgroup takes 16 columns of y for each FN: more share
-// the packing of x, fewer are more workgroups.  Measured with 1, 2 and 4:
-// 1x2048x2048 4.4, 5.1 and 7.2 us; 16x8192x2048 11.7, 8.7 and 10.3;
-// 8x14336x4096 31, 23.7 and 22.2; 24x8192x2048 12.7, 9.0 and 17.5.
+// the packing of x, fewer are more workgroups.  A call with 1, 2 and 4 in us,
+// on one weight, which the last cache holds / on weights in turn from memory:
+//   1 x 2048, K 2048     3.8,  4.6,  6.7 /  4.7,  5.6,  7.7
+//   8 x 4096, K 4096     6.7,  8.1, 11.9 /  8.4,  9.7, 13.5
+//   8 x 6144, K 4096    11.4,  8.2, 12.0 / 14.0, 10.0, 13.7
+//   16 x 8192, K 2048    8.4,  6.1,  7.9 / 10.8,  8.1,  9.8
+//   8 x 14336, K 4096   23.4, 16.0, 13.7 / 25.7, 18.3, 15.2
+//   24 x 4096, K 2048    6.5,  7.4       /  7.8,  8.9
+//   24 x 8192, K 2048   11.3,  7.5       / 13.2,  9.3
+// 1 is best up to 256 workgroups (4096 columns), one a CU, 2 up to 512 (8192).
+// The limits here lie halfway to the next such width, so that just below them
+// a narrower kernel runs than the best: 1 at 6144 columns.
 extern "C" hipError_t launch_b8_gemm_bf16(const GemmArgs* args, const void* x,
                                           long long ldx, int K,
                                           hipStream_t st) {
