@@ -67,6 +67,7 @@ from maggy_amd.ops.block8 import (  # noqa: E402,F401
     rms_norm8,
     swiglu8,
     unpack8,
+    weights_written,
 )
 from maggy_amd.ops.reduce import grad_l2norm, metric_mean, metric_sum  # noqa: E402,F401
 
@@ -75,5 +76,5 @@ __all__ = [
     "require_ext", "ext_or_none", "has_ext",
     "pack8", "unpack8", "swiglu8", "rms_norm8", "linear8", "pack_weight8",
     "Block8", "Weight8", "MaggyLinear8", "MaggyRMSNorm8",
-    "MaggyFeedForward8", "pack8_model", "drop8_model",
+    "MaggyFeedForward8", "pack8_model", "drop8_model", "weights_written",
 ]
