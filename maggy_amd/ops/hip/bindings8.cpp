@@ -39,6 +39,7 @@ int type_of(const Tensor& t, const char* name) {
 
 // a 2-D matrix on the GPU whose columns are contiguous
 Tensor matrix(const Tensor& t, const char* name) {
+  if (t.is_neg()) return matrix(t.resolve_neg(), name);
   TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
   TORCH_CHECK(t.dim() == 2, name, " must be 2-D, got ", t.dim(), "-D");
   type_of(t, name);
@@ -736,6 +737,7 @@ Tensor rms_norm8(Tensor x, Tensor w, double eps) {
   no_forward_mode("rms_norm8", {x, w});
   const auto lead = x.sizes().slice(0, x.dim() - 1).vec();
   x = as_rows(x);
+  w = w.resolve_neg();
   return as_shape(wants_grad({&x, &w}) ? RMSNorm8::apply(x, w, eps)
                                        : rms8_fwd(x, w, eps, false)[0],
                   lead);

@@ -976,3 +976,30 @@ def test_capture_beside_an_eager_graph_is_refused_behind_views():
         eager.backward(dy)  # not hurt by it
         torch.cuda.synchronize()
         assert leaf.grad.isfinite().all()
+
+
+def test_negative_views():
+    """Tensors whose sign is a bit of the tensor, as the imaginary part of a
+    conjugate has it."""
+    neg = torch._neg_view
+    x, w = _normal((5, 200), 1), _normal((60, 200), 2, 0.1)
+    n, dy = torch.randn(200, device="cuda"), _normal((5, 200), 3)
+    assert neg(x).is_neg()
+    assert torch.equal(ops.unpack8(ops.pack8(neg(x))),
+                       ops.unpack8(ops.pack8(-x)))
+    for grad in (False, True):
+        x = x.detach().requires_grad_(grad)
+        for a, b in ((ops.linear8(neg(x), neg(w)), ops.linear8(-x, -w)),
+                     (ops.swiglu8(neg(x), neg(dy)), ops.swiglu8(-x, -dy)),
+                     (ops.rms_norm8(neg(x), neg(n)), ops.rms_norm8(-x, -n))):
+            assert torch.equal(a, b)
+            if grad:
+                d = torch.randn_like(a)
+                da, = torch.autograd.grad(a, x, neg(d), retain_graph=True)
+                db, = torch.autograd.grad(b, x, -d, retain_graph=True)
+                assert torch.equal(da, db)
+    z = torch.randn(7, 1, device="cuda", dtype=torch.complex64)
+    part = z.conj().imag
+    assert part.is_neg()
+    assert torch.equal(ops.unpack8(ops.pack8(part)),
+                       ops.unpack8(ops.pack8(-z.imag.clone())))
