@@ -1003,3 +1003,27 @@ def test_negative_views():
     assert part.is_neg()
     assert torch.equal(ops.unpack8(ops.pack8(part)),
                        ops.unpack8(ops.pack8(-z.imag.clone())))
+
+
+def test_gradients_past_32_bits_of_several_weights():
+    """The second weight's rows lie beyond 2^31 values of the product."""
+    M, K, Ns = 70, 16384, (139990, 300)
+    x = _normal((M, K), 1)
+    ws = [torch.empty(n, K, device="cuda", dtype=torch.bfloat16)
+          .normal_(0.0, 0.02, generator=_gen(2 + i)).requires_grad_(True)
+          for i, n in enumerate(Ns)]
+    dys = [_normal((M, n), 5 + i, 1e-3) for i, n in enumerate(Ns)]
+    ys = ops.linear8(x, *ws)
+    dws = torch.autograd.grad(ys, ws, dys)
+    for y, dw, w, dy in zip(ys, dws, ws, dys):
+        for rows in (slice(0, 40), slice(w.shape[0] - 40, w.shape[0])):
+            # whole blocks of 128 rows, as the weights are packed
+            lo = rows.start // 128 * 128
+            wq = oracle.held_weight(w.detach()[lo:rows.stop])
+            xq = oracle.held(x)
+            skip = rows.start - lo
+            oracle.assert_within(y[:, rows], xq @ wq[skip:].t(),
+                                 oracle.product_bound(xq, wq[skip:]))
+            _, _, ((want, bound),) = oracle.linear(
+                x, [w.detach()[rows]], [dy[:, rows]])
+            oracle.assert_within(dw[rows], want, bound)
