@@ -1027,3 +1027,29 @@ def test_gradients_past_32_bits_of_several_weights():
             _, _, ((want, bound),) = oracle.linear(
                 x, [w.detach()[rows]], [dy[:, rows]])
             oracle.assert_within(dw[rows], want, bound)
+
+
+@torch.no_grad()
+def test_ablated_and_hooked_layers_decode():
+    from maggy_amd.ablation.ablationstudy import drop_layers
+
+    m = _llama().eval()
+    tokens = torch.randint(0, 256, (2, 8), device="cuda")
+    before, seen = m(tokens), []
+    drop_layers(m, "layers.0.attn.wo")
+    hook = m.layers[1].ffn.w3.register_forward_hook(
+        lambda mod, args, out: seen.append(out))
+    for _ in range(2):
+        logits = m(tokens)
+        assert not torch.equal(logits, before)
+        out = m.generate(tokens, 5)
+        assert seen and seen[0].dtype == torch.bfloat16
+        ops.pack8_model(m)
+        assert torch.equal(m(tokens), logits)
+        assert torch.equal(m.generate(tokens, 5), out)
+    hook.remove()
+    seen.clear()
+    ops.drop8_model(m)
+    logits = m(tokens)
+    ops.pack8_model(m)
+    assert torch.equal(m(tokens), logits) and not seen
